@@ -257,6 +257,91 @@ int32_t hk_sample(const void *logits, int32_t n, float temperature, float topp, 
 int32_t hk_sample_static(const void *logits, int32_t n, float temperature, float topp, double random, int32_t *token,
                          void *stream);
 
+/* ---- a cache held in 8 bits, and the attention over it (no counterpart in the reference: its caches are float32 and
+ * float16, public/forward.js:762) ----
+ *
+ * One layer's cache. Positions lie in blocks of HK_CACHE_BLOCK. A block that is complete is held in 8 bits with one
+ * float32 scale a kv head for its keys and one for its values: s = max|x| / 127 rounded to float32, and x / s rounded to
+ * the nearest integer, ties to even (0 where s is 0). The block that is being filled, and the latest HK_CACHE_RECENT
+ * positions, are held in float32 besides. A token at position p attends to the positions before its own block by their
+ * 8-bit values, and to its own block's up to p by their float32 rows: its result depends neither on how the tokens before
+ * it were split into calls nor on any token after it.
+ *
+ * The buffers are the caller's (device memory, 16-byte aligned, zeroed before the first call), of
+ * blocks = ceil(seq_len / HK_CACHE_BLOCK):
+ *   keys   int8  [n_kv_heads][blocks][head_size / 16][32][16]: channel 16 c + i of the block's position t at [c][t][i]
+ *   values uint8 [n_kv_heads][blocks][head_size][32]: 128 + the value of position t at byte
+ *                16 (t / 4 % 2) + 8 (t / 16) + 4 (t / 8 % 2) + t % 4 of its channel
+ *   scales float [n_kv_heads][blocks][2]: the block's key scale, then its value scale
+ *   recent_keys, recent_values float [HK_CACHE_RECENT + HK_CACHE_BLOCK][n_kv_heads][head_size]: position p's row at
+ *                p % HK_CACHE_RECENT; the last HK_CACHE_BLOCK rows take the earlier rows of a long call's first block
+ * head_size is one of 16, 32, 48, 64, 96, 128, 256; seq_len at most HK_CACHE_MOST. Calls on one cache are ordered by the
+ * caller (one stream, or events). None of these calls allocates or waits: they may be captured into a graph. */
+#define HK_CACHE_BLOCK 32
+#define HK_CACHE_RECENT 128
+#define HK_CACHE_MOST 16777216
+#define HK_CACHE_GROUP_MOST 32 /* query heads a kv head at most */
+typedef struct hk_cache {
+  void *keys;
+  void *values;
+  void *scales;
+  void *recent_keys;
+  void *recent_values;
+  int32_t n_kv_heads;
+  int32_t head_size;
+  int32_t seq_len;
+} hk_cache;
+
+/* The rows of count tokens at positions pos.. into the cache: k and v float32, a token's kv heads side by side
+ * (n_kv_heads * head_size values), kv_stride floats a row (a multiple of 4; k and v 16-byte aligned). Every block that
+ * becomes complete is quantized; rows of other positions stay as they are. pos is where the last call ended, or any
+ * position of the latest HK_CACHE_RECENT - HK_CACHE_BLOCK (tokens taken again), or the first of a block; before one
+ * anywhere else, hk_cache_rewind. A value that is not finite leaves its block's scale (for its head) not finite: the block
+ * stands for NaN from then on, for the tokens of later blocks. */
+int32_t hk_cache_append(const hk_cache *cache, const void *k, const void *v, int32_t kv_stride, int32_t count,
+                        int32_t pos, void *stream);
+
+/* The attention of count tokens at positions pos.., once their rows (and every earlier position's) are in the cache:
+ * out[t][h] = softmax_j(q[t][h] . k_j / sqrt(head_size)) v_j over j <= pos + t, query head h with kv head
+ * h / (n_heads / n_kv_heads). q and out float32 with rows of n_heads * head_size values, q_stride and out_stride floats
+ * apart; k and v the tokens' own rows as hk_cache_append took them with the same count and pos. Strides are multiples of
+ * 4, pointers 16-byte aligned; n_heads is a multiple of n_kv_heads, at most HK_CACHE_GROUP_MOST times it. A q that is not
+ * finite makes its own row NaN, a key or value the rows of the tokens that see it; no other row changes. workspace: at
+ * least hk_cache_workspace bytes of device memory (16-byte aligned; nothing in it is kept from one call to the next), not
+ * shared by calls that may overlap. */
+int32_t hk_cache_attention(void *out, const void *q, const void *k, const void *v, const hk_cache *cache,
+                           int32_t n_heads, int32_t q_stride, int32_t kv_stride, int32_t out_stride, int32_t count,
+                           int32_t pos, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* the bytes of workspace an hk_cache_attention of count tokens takes at most, at any position (negative: HE_E_ARG) */
+int64_t hk_cache_workspace(const hk_cache *cache, int32_t n_heads, int32_t count);
+
+/* Positions from..from + count - 1 as a token at position end (from + count <= end) would read them: those before end's
+ * block by their 8-bit values, that block's by their float32 rows; keys and values float32
+ * [count][n_kv_heads * head_size]. */
+int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t from, int32_t count, int32_t end,
+                      void *stream);
+
+/* Goes back to position pos (any before where the last call ended), where its block's earlier float32 rows are no longer
+ * held: they are taken from the block's 8-bit values. The next hk_cache_append is at pos. */
+int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
+
+/* The log probabilities of tokens under softmax(logits) of m rows of n float32 logits, stride floats apart (stride >= n,
+ * any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens given [m][n_given] int32
+ * (NaN where one is outside 0..n-1; null with n_given 0), the entropy [m] in nats (or null), and the `top`
+ * (0..HK_LOGPROBS_TOP_MOST) largest alternatives, ids [m][top] int32 and logps [m][top], the lowest index first among
+ * equals. A logit of minus infinity has probability 0: log probability minus infinity, nothing of the entropy, and no
+ * alternative (id -1, log probability minus infinity, behind the others). A row whose largest logit is not finite has no
+ * probabilities: NaN and id -1 throughout. All pointers are device memory. workspace: at least hk_logprobs_workspace bytes
+ * (16-byte aligned), not shared by calls that may overlap. Neither allocates nor waits. */
+#define HK_LOGPROBS_TOP_MOST 32
+int32_t hk_logprobs(void *logp, void *entropy, void *ids, void *logps, const void *logits, int64_t stride,
+                    const void *given, int32_t n_given, int32_t m, int32_t n, int32_t top, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+
+/* the bytes of workspace an hk_logprobs of these sizes takes (negative: HE_E_ARG) */
+int64_t hk_logprobs_workspace(int32_t m, int32_t n, int32_t top);
+
 /* The memory's read ceiling, kernels/ceilings.ts:9-25 read(p, bytes, passes) on the device: bytes (a multiple of 64)
  * at the device pointer p read by a streaming kernel in each of a few launch shapes (8 to 16 loads of 16 bytes a lane
  * in flight, 256 to 2048 blocks), one untimed pass then passes timed ones a shape. *checksum is read()'s: the xor of

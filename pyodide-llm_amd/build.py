@@ -28,7 +28,7 @@ ORDER = os.path.join(CSRC, "decode_order.txt")
 ORDER_FLAGS = ["-ffunction-sections", "-Xoffload-linker", f"--symbol-ordering-file={ORDER}", "-Xoffload-linker",
                "--no-warn-symbol-ordering"]
 SOURCES = ["gemv.hip", "gemm.hip", "gemm_chains.hip", "misc.hip", "forms.hip", "attention.hip", "attention_tokens.hip", "sampling.hip",
-           "ceilings.hip", "engine.cpp"]
+           "cache.hip", "cache_attention.hip", "logprobs.hip", "ceilings.hip", "operators.cpp", "engine.cpp"]
 
 
 def run(cmd):

@@ -138,6 +138,10 @@ int32_t dev_alloc(T **p, size_t bytes) {
 
 }  // namespace
 
+namespace ple {
+int32_t failed(int32_t code, const std::string &what) { return fail(code, what); }
+}  // namespace ple
+
 struct he_engine {
   he_config c{};
   he_tensor t[HE_T_COUNT]{};

@@ -5,7 +5,12 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <string>
+
 namespace ple {
+
+// a failed call: its code, with the message he_last_error() gives (this thread's)
+int32_t failed(int32_t code, const std::string &what);
 
 // one matrix of a GEMV/GEMM launch: rows [rows][K] int8 (or int6 groups of 24 bytes), scales [rows][K/32]; the
 // output y[t * y_stride + r] for token t, row r (accumulate: y = y + result, the residual add of kernels/kernel.ts:
@@ -191,6 +196,59 @@ int32_t attention_most_positions();
 // whether launch_attention takes a.xq and writes quantize_x of its output (the prompt's kernels: in place of a.out): head
 // sizes that are a multiple of 32 (a block holds a whole group)
 bool attention_quantizes(const AttnArgs &a);
+
+// ---- the cache held in 8 bits (cache.hpp) ----
+// one layer's cache: hk_cache's buffers, and the blocks of 32 positions it holds (seq_len rounded up)
+struct CacheView {
+  int8_t *keys;
+  uint8_t *values;
+  float *scales;
+  float *recent_keys, *recent_values;
+  int32_t nkv, hs, blocks;
+};
+// whether a call of count tokens at pos displaces earlier recent rows of its first block (of 32), which are then set
+// apart behind the 128
+inline bool cache_displaces(int32_t pos, int32_t count) { return (int64_t)pos + count > pos / 32 * 32 + 128; }
+// count tokens' rows at pos.. (k, v: [count][x_stride], kv heads side by side) into the cache
+struct CacheRows {
+  CacheView c;
+  const float *k, *v;
+  int32_t x_stride, count, pos;
+  const int32_t *dpos;  // one token's position in device memory (a replayed decode step), or null: pos
+  int32_t displaced;    // set by the launch
+};
+hipError_t launch_cache_append(const CacheRows &a, hipStream_t s);
+// positions from..from + count - 1: those before bound by their 8-bit values, the others (within the latest 128) by their
+// float32 rows, into keys / values [count][nkv * hs] (null: into the recent rows)
+hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t bound,
+                             hipStream_t s);
+// the attention of count tokens at pos.. whose rows (and every earlier one) are in the cache; k, v are the tokens' own
+// rows in float32
+struct CacheAttn {
+  CacheRows rows;
+  const float *q;
+  float *out;
+  int32_t nh, q_stride, out_stride;
+  float *workspace;  // cache_attention_workspace() bytes
+};
+hipError_t launch_cache_attention(const CacheAttn &a, hipStream_t s);
+int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count);
+
+// the log probabilities of given tokens [m][n_given], the entropy [m] and the top alternatives [m][top] of m rows of
+// logits (stride floats apart) over n tokens
+constexpr int32_t LOGPROBS_TOP_MOST = 32;
+struct LogprobArgs {
+  float *logp, *entropy;
+  int32_t *ids;
+  float *logps;
+  const float *logits;
+  int64_t stride;
+  const int32_t *given;
+  int32_t n_given, m, n, top;
+  uint8_t *workspace;  // logprobs_workspace() bytes
+};
+hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s);
+int64_t logprobs_workspace(int32_t m, int32_t n, int32_t top);
 
 // a streaming read of bytes (a multiple of 16) at p in launch shape `shape` (0 .. read_ceiling_shapes() - 1: loads a
 // lane per tile, blocks): block b's sums of its 32-bit words lane by lane (j = word index % 4) into partial[4 b + j],

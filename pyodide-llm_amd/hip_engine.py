@@ -44,6 +44,25 @@ class HeTensor(ctypes.Structure):
 TensorArray = HeTensor * len(TENSORS)
 
 
+class HkCache(ctypes.Structure):
+    """hk_cache: one layer's cache held in 8 bits, by the device addresses of its buffers (cache_shapes() sizes them)"""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("keys", "values", "scales", "recent_keys", "recent_values")] + [
+        (name, ctypes.c_int32) for name in ("n_kv_heads", "head_size", "seq_len")]
+
+
+CACHE_BLOCK, CACHE_RECENT = 32, 128  # HK_CACHE_BLOCK, HK_CACHE_RECENT
+
+
+def cache_shapes(n_kv_heads, head_size, seq_len):
+    """{buffer of HkCache: (shape, NumPy dtype)} (include/pyodide_llm_hip.h hk_cache)"""
+    blocks = -(-seq_len // CACHE_BLOCK)
+    recent = (CACHE_RECENT + CACHE_BLOCK, n_kv_heads, head_size)
+    return {"keys": ((n_kv_heads, blocks, head_size // 16, CACHE_BLOCK, 16), "int8"),
+            "values": ((n_kv_heads, blocks, head_size, CACHE_BLOCK), "uint8"),
+            "scales": ((n_kv_heads, blocks, 2), "float32"),
+            "recent_keys": (recent, "float32"), "recent_values": (recent, "float32")}
+
+
 def config(**fields):
     """an HeConfig from keyword fields; relaxed defaults to 1 (bias 64, the reference's default path), eps 1e-5;
     outliers takes a list of channels"""
@@ -104,6 +123,13 @@ def library():
             "hk_ordered_sum": (I32, [P, I32, I32, P, P, P]),
             "hk_sample": (I32, [P, I32, F, F, ctypes.c_double, P, P]),
             "hk_sample_static": (I32, [P, I32, F, F, ctypes.c_double, P, P]),
+            "hk_cache_append": (I32, [P, P, P, I32, I32, I32, P]),
+            "hk_cache_attention": (I32, [P, P, P, P, P, I32, I32, I32, I32, I32, I32, P, I64, P]),
+            "hk_cache_workspace": (I64, [P, I32, I32]),
+            "hk_cache_read": (I32, [P, P, P, I32, I32, I32, P]),
+            "hk_cache_rewind": (I32, [P, I32, P]),
+            "hk_logprobs": (I32, [P, P, P, P, P, I64, P, I32, I32, I32, I32, P, I64, P]),
+            "hk_logprobs_workspace": (I64, [I32, I32, I32]),
             "hk_read_ceiling": (I32, [P, ctypes.c_int64, I32, P, P, P]),
             "hk_read_floor": (I32, [P, ctypes.c_int64, ctypes.c_int64, I32, P, P]),
             "hk_valu_ceiling": (I32, [I32, F, F, F, P, P, P, P]),
@@ -112,7 +138,6 @@ def library():
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-        del I64
         _lib = lib
     return _lib
 
