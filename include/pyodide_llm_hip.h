@@ -261,7 +261,7 @@ int32_t hk_sample_static(const void *logits, int32_t n, float temperature, float
  * float16, public/forward.js:762) ----
  *
  * One layer's cache. Positions lie in blocks of HK_CACHE_BLOCK. A block that is complete is held in 8 bits with one
- * float32 scale a kv head for its keys and one for its values: s = max|x| / 127 rounded to float32, and x / s rounded to
+ * float32 scale a kv head for its keys and one for its values: s = max|x| * float32(1 / 127) in float32, and x / s rounded to
  * the nearest integer, ties to even (0 where s is 0). The block that is being filled, and the latest HK_CACHE_RECENT
  * positions, are held in float32 besides. A token at position p attends to the positions before its own block by their
  * 8-bit values, and to its own block's up to p by their float32 rows: its result depends neither on how the tokens before
@@ -326,8 +326,8 @@ int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t f
  * held: they are taken from the block's 8-bit values. The next hk_cache_append is at pos. */
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
 
-/* The log probabilities of tokens under softmax(logits) of m rows of n float32 logits, stride floats apart (stride >= n,
- * any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens given [m][n_given] int32
+/* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats apart
+ * (stride >= n, any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens given [m][n_given] int32
  * (NaN where one is outside 0..n-1; null with n_given 0), the entropy [m] in nats (or null), and the `top`
  * (0..HK_LOGPROBS_TOP_MOST) largest alternatives, ids [m][top] int32 and logps [m][top], the lowest index first among
  * equals. A logit of minus infinity has probability 0: log probability minus infinity, nothing of the entropy, and no

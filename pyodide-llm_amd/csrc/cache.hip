@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void append_kernel(const CacheRows a) {
     for (int o = 32; o; o >>= 1) top = wmax(top, __shfl_xor(top, o));
     if (tid % 64 == 0) tops[tid / 64] = top;
     __syncthreads();
-    const float s = wmax(wmax(tops[0], tops[1]), wmax(tops[2], tops[3])) / 127.0f;
+    const float s = wmax(wmax(tops[0], tops[1]), wmax(tops[2], tops[3])) * (1.0f / 127.0f);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int f = tid + 256 * i, t = f / (HS / 4), d = f % (HS / 4) * 4;

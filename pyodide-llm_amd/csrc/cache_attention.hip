@@ -11,6 +11,8 @@
 // Maxima are rounded up to whole powers of two, so that every rescaling is exact; the products' scale (2^mw - 14) follows
 // the largest probability times its block's value scale, so that halves neither overflow nor lose bits where the blocks'
 // scales differ.
+#include <algorithm>
+
 #include "cache.hpp"
 
 namespace ple {
@@ -70,61 +72,76 @@ struct Running {
   float mw;    // the products' reference: O holds sum of 2^(score - mw + 14) value
 };
 
+// A wave's 32 rows: the tokens and query heads of its lanes' columns, the queries' digits, the running statistics and the
+// output's columns
 template <int HS>
-__global__ __launch_bounds__(256) void attend_kernel(const CacheAttn a, int tokens_log2) {
-  constexpr int STEPS = (HS + 31) / 32, TILES = (HS + 31) / 32;
-  const CacheView &c = a.rows.c;
-  const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32, head = blockIdx.y;
-  const int pos = a.rows.dpos ? *a.rows.dpos : a.rows.pos, end = pos + a.rows.count;
-  const int group = a.nh / c.nkv, first_token = ((pos >> tokens_log2) + blockIdx.x * 4 + threadIdx.x / 64) << tokens_log2;
-  if (first_token >= end) return;
-  const int last_token = min(end, first_token + (1 << tokens_log2)) - 1;
-  const int own = first_token / CACHE_BLOCK;  // the tile's tokens lie in one block
-  const int token = first_token + col / group;
-  const bool row = col / group < (1 << tokens_log2) && token >= pos && token < end;
-  const int qhead = head * group + col % group;
-  const float *q = a.q + (int64_t)(row ? token - pos : 0) * a.q_stride + qhead * HS;
-
-  // the query's digits: lane (row, half) holds channels 32 s + 16 half .. + 15 of step s
+struct Tile {
+  static constexpr int STEPS = (HS + 31) / 32, TILES = (HS + 31) / 32;
+  int lane, col, half, head, pos, group, first_token, last_token, own, token, qhead;
+  bool row;
+  const float *q;
+  float unit, from_digits;
   i32x4 q0[STEPS], q1[STEPS], q2[STEPS];
-  float largest = 0.0f;
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = 32 * s + 16 * half + 4 * j;
-      if (!row || d >= HS) continue;
-      const float4 x = *reinterpret_cast<const float4 *>(q + d);
-      largest = wmax(largest, wmax(wmax(__builtin_fabsf(x.x), __builtin_fabsf(x.y)),
-                                   wmax(__builtin_fabsf(x.z), __builtin_fabsf(x.w))));
-    }
-  largest = wmax(largest, other_half(largest));
-  // (below 2^-100 a query is taken as zero; one that is not finite makes its row's scores not a number)
-  const bool finite = largest < __builtin_inff(), some = finite && largest > 0x1p-100f;
-  const float to_digits = some ? 8355000.0f / largest : 0.0f;
-  const float unit = LOG2E / __builtin_sqrtf((float)HS);
-  const float from_digits = finite ? largest / 8355000.0f * unit : __builtin_nanf("");
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = 32 * s + 16 * half + 4 * j;
-      float4 x = make_float4(0, 0, 0, 0);
-      if (row && d < HS && some) x = *reinterpret_cast<const float4 *>(q + d);
-      int32_t d0, d1, d2;
-      digits(x, to_digits, d0, d1, d2);
-      q0[s][j] = d0;
-      q1[s][j] = d1;
-      q2[s][j] = d2;
-    }
-
-  Running run = {NONE, 0.0f, NONE};
+  Running run;
   f32x16 o[TILES];
+
+  // the rows of tile `index` (of 2^tokens_log2 tokens, from the multiple that holds pos on)
+  __device__ __forceinline__ void place(const CacheAttn &a, int index, int tokens_log2) {
+    lane = threadIdx.x % 64;
+    col = lane % 32;
+    half = lane / 32;
+    pos = a.rows.dpos ? *a.rows.dpos : a.rows.pos;
+    const int end = pos + a.rows.count;
+    group = a.nh / a.rows.c.nkv;
+    first_token = ((pos >> tokens_log2) + index) << tokens_log2;
+    last_token = min(end, first_token + (1 << tokens_log2)) - 1;
+    own = first_token / CACHE_BLOCK;  // the tile's tokens lie in one block
+    token = first_token + col / group;
+    row = col / group < (1 << tokens_log2) && token >= pos && token < end;
+    qhead = head * group + col % group;
+    q = a.q + (int64_t)(row ? token - pos : 0) * a.q_stride + qhead * HS;
+    unit = LOG2E / __builtin_sqrtf((float)HS);
+    run = {NONE, 0.0f, NONE};
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) o[t] = (f32x16)(0.0f);
-  // the statistics after a tile whose largest score is `top`, of values up to 2^bits: the factor of a probability in the
-  // products
-  auto advance = [&](float top, float bits) {
+    for (int t = 0; t < TILES; ++t) o[t] = (f32x16)(0.0f);
+  }
+
+  // the queries' digits: lane (row, half) holds channels 32 s + 16 half .. + 15 of step s
+  __device__ __forceinline__ void read_queries() {
+    float largest = 0.0f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 32 * s + 16 * half + 4 * j;
+        if (!row || d >= HS) continue;
+        const float4 x = *reinterpret_cast<const float4 *>(q + d);
+        largest = wmax(largest, wmax(wmax(__builtin_fabsf(x.x), __builtin_fabsf(x.y)),
+                                     wmax(__builtin_fabsf(x.z), __builtin_fabsf(x.w))));
+      }
+    largest = wmax(largest, other_half(largest));
+    // (below 2^-100 a query is taken as zero; one that is not finite makes its row's scores not a number)
+    const bool finite = largest < __builtin_inff(), some = finite && largest > 0x1p-100f;
+    const float to_digits = some ? 8355000.0f / largest : 0.0f;
+    from_digits = finite ? largest / 8355000.0f * unit : __builtin_nanf("");
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = 32 * s + 16 * half + 4 * j;
+        float4 x = make_float4(0, 0, 0, 0);
+        if (row && d < HS && some) x = *reinterpret_cast<const float4 *>(q + d);
+        int32_t d0, d1, d2;
+        digits(x, to_digits, d0, d1, d2);
+        q0[s][j] = d0;
+        q1[s][j] = d1;
+        q2[s][j] = d2;
+      }
+  }
+
+  // the statistics after positions whose largest score is `top`, of values up to 2^bits: the factor of a probability in
+  // the products
+  __device__ __forceinline__ float advance(float top, float bits) {
     const float up = __builtin_ceilf(top), m = __builtin_fmaxf(run.m, up), mw = __builtin_fmaxf(run.mw, up + bits);
     run.l *= __builtin_amdgcn_exp2f(run.m - m);
     const float gamma = __builtin_amdgcn_exp2f(run.mw - mw);
@@ -135,68 +152,89 @@ __global__ __launch_bounds__(256) void attend_kernel(const CacheAttn a, int toke
     run.m = m;
     run.mw = mw;
     return __builtin_amdgcn_exp2f(__builtin_fminf(m - mw + 14.0f, 126.0f));
-  };
+  }
 
-  const int64_t at = (int64_t)head * c.blocks;
-  const int8_t *kp = c.keys + at * (CACHE_BLOCK * HS) + half * (CACHE_BLOCK * 16) + col * 16;
-  const uint8_t *vp = c.values + at * (CACHE_BLOCK * HS) + col * CACHE_BLOCK + half * 16;
-  for (int b = 0; b < own; ++b) {
-    i32x16 s0 = (i32x16)(0), s1 = (i32x16)(0), s2 = (i32x16)(0);
+  // blocks first, first + step, .. below to, by their 8-bit values
+  __device__ __forceinline__ void blocks(const CacheView &c, int first, int to, int step) {
+    if (first >= to) return;
+    const int64_t at = (int64_t)head * c.blocks;
+    const int8_t *kp = c.keys + at * (CACHE_BLOCK * HS) + half * (CACHE_BLOCK * 16) + col * 16;
+    const uint8_t *vp = c.values + at * (CACHE_BLOCK * HS) + col * CACHE_BLOCK + half * 16;
+    const float2 *sp = reinterpret_cast<const float2 *>(c.scales) + at;
+    // keys are read a block ahead (once the products have taken this block's), values while this block's scores are made
+    i32x4 k[STEPS], v[TILES];
+    auto load_keys = [&](int b) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      i32x4 k = (i32x4)(0);
-      if (HS % 32 == 0 || 32 * s + 16 * half < HS)
-        k = *reinterpret_cast<const i32x4 *>(kp + (int64_t)b * (CACHE_BLOCK * HS) + s * (CACHE_BLOCK * 32));
-      s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q0[s], s0, 0, 0, 0);
-      s1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q1[s], s1, 0, 0, 0);
-      s2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, q2[s], s2, 0, 0, 0);
-    }
-    const float ks = c.scales[(at + b) * 2], vs = c.scales[(at + b) * 2 + 1];
-    const float each = from_digits * ks;
-    float p[16], top = -__builtin_inff();
+      for (int s = 0; s < STEPS; ++s) {
+        k[s] = (i32x4)(0);
+        if (HS % 32 == 0 || 32 * s + 16 * half < HS)
+          k[s] = *reinterpret_cast<const i32x4 *>(kp + (int64_t)b * (CACHE_BLOCK * HS) + s * (CACHE_BLOCK * 32));
+      }
+    };
+    load_keys(first);
+    for (int b = first; b < to; b += step) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      p[r] = __builtin_fmaf((float)s0[r], 65536.0f, __builtin_fmaf((float)s1[r], 256.0f, (float)s2[r])) * each;
-      top = __builtin_fmaxf(top, p[r]);
-    }
-    top = __builtin_fmaxf(top, other_half(top));
-    const float bits = vs > 0.0f ? (float)((int)(__float_as_uint(vs) >> 23) - 126) : -200.0f;
-    const float factor = advance(top, bits) * vs;
-    f16x8 hi[2], lo[2];
+      for (int t = 0; t < TILES; ++t) {
+        v[t] = (i32x4)(0);
+        if (HS % 32 == 0 || 32 * t + col < HS)
+          v[t] = *reinterpret_cast<const i32x4 *>(vp + (int64_t)b * (CACHE_BLOCK * HS) + t * (32 * CACHE_BLOCK));
+      }
+      const float2 scale = sp[b];
+      i32x16 s0 = (i32x16)(0), s1 = (i32x16)(0), s2 = (i32x16)(0);
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      const float e0 = __builtin_amdgcn_exp2f(p[r] - run.m), e1 = __builtin_amdgcn_exp2f(p[r + 1] - run.m);
-      run.l += e0;
-      run.l += e1;
-      f16x2 h, l;
-      split(e0 * factor, e1 * factor, h, l);
-      hi[r / 8][r % 8] = h[0];
-      hi[r / 8][r % 8 + 1] = h[1];
-      lo[r / 8][r % 8] = l[0];
-      lo[r / 8][r % 8 + 1] = l[1];
-    }
+      for (int s = 0; s < STEPS; ++s) {
+        s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q0[s], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q1[s], s1, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q2[s], s2, 0, 0, 0);
+      }
+      const float ks = scale.x, vs = scale.y;
+      load_keys(b + step < to ? b + step : b);  // (the last one again: no use of it)
+      const float each = from_digits * ks;
+      float p[16], top = -__builtin_inff();
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (HS % 32 == 0 || 32 * t + col < HS)
-        w = *reinterpret_cast<const uint4 *>(vp + (int64_t)b * (CACHE_BLOCK * HS) + t * (32 * CACHE_BLOCK));
-      f16x2 h[8];
-      widen(w.x, h[0], h[1]);
-      widen(w.y, h[2], h[3]);
-      widen(w.z, h[4], h[5]);
-      widen(w.w, h[6], h[7]);
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_fmaf((float)s0[r], 65536.0f, __builtin_fmaf((float)s1[r], 256.0f, (float)s2[r])) * each;
+        top = __builtin_fmaxf(top, p[r]);
+      }
+      top = __builtin_fmaxf(top, other_half(top));
+      const float bits = vs > 0.0f ? (float)((int)(__float_as_uint(vs) >> 23) - 126) : -200.0f;
+      const float factor = advance(top, bits) * vs;
+      f16x8 hi[2], lo[2];
+      float sum = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const f16x8 v = {h[4 * s][0], h[4 * s][1], h[4 * s + 1][0], h[4 * s + 1][1],
-                         h[4 * s + 2][0], h[4 * s + 2][1], h[4 * s + 3][0], h[4 * s + 3][1]};
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, hi[s], o[t], 0, 0, 0);
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo[s], o[t], 0, 0, 0);
+      for (int r = 0; r < 16; r += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(p[r] - run.m), e1 = __builtin_amdgcn_exp2f(p[r + 1] - run.m);
+        sum += e0 + e1;
+        f16x2 h, l;
+        split(e0 * factor, e1 * factor, h, l);
+        hi[r / 8][r % 8] = h[0];
+        hi[r / 8][r % 8 + 1] = h[1];
+        lo[r / 8][r % 8] = l[0];
+        lo[r / 8][r % 8 + 1] = l[1];
+      }
+      run.l += sum;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        f16x2 h[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) widen((uint32_t)v[t][j], h[2 * j], h[2 * j + 1]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const f16x8 x = {h[4 * s][0], h[4 * s][1], h[4 * s + 1][0], h[4 * s + 1][1],
+                           h[4 * s + 2][0], h[4 * s + 2][1], h[4 * s + 3][0], h[4 * s + 3][1]};
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, hi[s], o[t], 0, 0, 0);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, lo[s], o[t], 0, 0, 0);
+        }
       }
     }
   }
 
-  // the tile's own block by its float32 rows, up to the tile's last token, on float32 MFMA
-  {
+  // the tile's own block by its float32 rows, up to the tile's last token, on float32 MFMA. PARTS waves share it (wave
+  // `part`): each takes its share of the channels of the products of keys and queries, whose parts are added through
+  // `shared` (PARTS x 64 x 16 floats), and of the output's; the sums of probabilities count with part 0
+  template <int PARTS>
+  __device__ __forceinline__ void own_block(const CacheAttn &a, int part, float *shared) {
+    const CacheView &c = a.rows.c;
     const int p0 = own * CACHE_BLOCK;
     auto source = [&](const float *x, const float *recent, int p) {
       if (p >= pos) return x + (int64_t)(p - pos) * a.rows.x_stride + head * HS;
@@ -206,13 +244,26 @@ __global__ __launch_bounds__(256) void attend_kernel(const CacheAttn a, int toke
     const float *k = source(a.rows.k, c.recent_keys, key ? p0 + col : last_token) + half * (HS / 2);
     const float *qh = q + half * (HS / 2);
     f32x16 s = (f32x16)(0.0f);
-#pragma unroll 2
-    for (int i = 0; i < HS / 2; i += 4) {
+#pragma unroll 4
+    for (int n = 0; n < (HS / 8 + PARTS - 1) / PARTS; ++n) {
+      const int i = 4 * (n * PARTS + part);
+      if (HS / 8 % PARTS && i >= HS / 2) break;  // (the same in the whole wave)
       const float4 x = *reinterpret_cast<const float4 *>(k + i), y = *reinterpret_cast<const float4 *>(qh + i);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s, 0, 0, 0);
+    }
+    if (PARTS > 1) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) shared[(part * 16 + r) * 64 + lane] = s[r];
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = shared[r * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < PARTS; ++w) s[r] += shared[(w * 16 + r) * 64 + lane];
+      }
     }
     float p[16], top = -__builtin_inff();
 #pragma unroll
@@ -223,18 +274,19 @@ __global__ __launch_bounds__(256) void attend_kernel(const CacheAttn a, int toke
     }
     top = __builtin_fmaxf(top, other_half(top));
     const float factor = advance(top, 1.0f);
-    float bad = 0.0f;
+    float bad = 0.0f, sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = p0 + 8 * (r / 4) + 4 * half + r % 4;
       const bool there = j <= last_token;
       const float *v = source(a.rows.v, c.recent_values, there ? j : last_token);
       const float e = j <= token ? __builtin_amdgcn_exp2f(p[r] - run.m) : 0.0f;
-      run.l += e;
+      sum += e;
       const float w = e * factor;
       bool strange = false;
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
+        if (PARTS > 1 && t % PARTS != part) continue;  // (the same in the whole wave)
         float x = 0.0f;
         if (there && (HS % 32 == 0 || 32 * t + col < HS)) x = v[32 * t + col];
         const bool fine = __builtin_fabsf(x) < __builtin_inff();
@@ -247,49 +299,244 @@ __global__ __launch_bounds__(256) void attend_kernel(const CacheAttn a, int toke
       const int j0 = p0 + 8 * (r / 4) + r % 4;
       if (((uint32_t)any && j0 <= token) || ((uint32_t)(any >> 32) && j0 + 4 <= token)) bad = __builtin_nanf("");
     }
-    run.l += bad;
+    run.l = (PARTS > 1 && part ? 0.0f : run.l + sum) + bad;
   }
+};
 
+// Many tiles: one a wave, over all its blocks
+template <int HS>
+__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const CacheAttn a, int tokens_log2) {
+  Tile<HS> tile;
+  tile.head = blockIdx.y;
+  tile.place(a, blockIdx.x * 4 + threadIdx.x / 64, tokens_log2);
+  if (tile.first_token > tile.last_token) return;
+  tile.read_queries();
+  tile.blocks(a.rows.c, 0, tile.own, 1);
+  tile.template own_block<1>(a, 0, nullptr);
+  const Running &run = tile.run;
   const float sum = run.l + other_half(run.l);
   const float scale = __builtin_amdgcn_exp2f(run.mw - run.m - 14.0f) / sum;
-  if (!row) return;
-  float *out = a.out + (int64_t)(token - pos) * a.out_stride + qhead * HS;
+  if (!tile.row) return;
+  float *out = a.out + (int64_t)(tile.token - tile.pos) * a.out_stride + tile.qhead * HS;
 #pragma unroll
-  for (int t = 0; t < TILES; ++t)
+  for (int t = 0; t < Tile<HS>::TILES; ++t)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * t + 8 * (r / 4) + 4 * half;
+      const int d = 32 * t + 8 * (r / 4) + 4 * tile.half;
+      const f32x16 &o = tile.o[t];
       if (HS % 32 == 0 || d < HS)
         *reinterpret_cast<float4 *>(out + d) =
-            make_float4(o[t][r] * scale, o[t][r + 1] * scale, o[t][r + 2] * scale, o[t][r + 3] * scale);
+            make_float4(o[r] * scale, o[r + 1] * scale, o[r + 2] * scale, o[r + 3] * scale);
     }
+}
+
+// Few tiles: the blocks of a tile in `splits` parts, one a workgroup, whose four waves take them in turn, and one part more
+// for the tile's own block (the first, which takes the longest). A part's statistics (m, l, mw) and outputs go to the
+// workspace: outputs [tile][kv head][part][rows][HS], then statistics [tile][kv head][part][rows] of 4 floats.
+template <int HS>
+__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(const CacheAttn a, int tokens_log2, int rows, int splits) {
+  extern __shared__ float4 lds[];
+  constexpr int STRIDE = HS + 4;  // (rows of a wave's outputs 4 banks apart)
+  float *const shared = reinterpret_cast<float *>(lds);
+  __shared__ float stats[4][32][3];
+  const int wave = threadIdx.x / 64, part = blockIdx.x;
+  Tile<HS> tile;
+  tile.head = blockIdx.z;
+  tile.place(a, blockIdx.y, tokens_log2);
+  if (part == 0) {
+    tile.template own_block<4>(a, wave, shared);
+    __syncthreads();  // (shared holds the outputs next)
+  } else {
+    const int from = (int)((int64_t)tile.own * (part - 1) / splits), to = (int)((int64_t)tile.own * part / splits);
+    if (from + wave < to) {
+      tile.read_queries();
+      tile.blocks(a.rows.c, from + wave, to, 4);
+    }
+  }
+  const Running &run = tile.run;
+  const float sum = run.l + other_half(run.l);
+  if (tile.half == 0) {
+    stats[wave][tile.col][0] = run.m;
+    stats[wave][tile.col][1] = sum;
+    stats[wave][tile.col][2] = run.mw;
+  }
+  __syncthreads();
+  // the four waves' statistics as one, and each wave's outputs on it
+  float m = NONE, l = 0.0f, mw = NONE;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    m = __builtin_fmaxf(m, stats[w][tile.col][0]);
+    mw = __builtin_fmaxf(mw, stats[w][tile.col][2]);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) l += stats[w][tile.col][1] * __builtin_amdgcn_exp2f(stats[w][tile.col][0] - m);
+  const float scale = __builtin_amdgcn_exp2f(run.mw - mw);
+  if (tile.col < rows) {
+#pragma unroll
+    for (int t = 0; t < Tile<HS>::TILES; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * t + 8 * (r / 4) + 4 * tile.half;
+        const f32x16 &o = tile.o[t];
+        if (HS % 32 == 0 || d < HS)
+          *reinterpret_cast<float4 *>(shared + (wave * rows + tile.col) * STRIDE + d) =
+              make_float4(o[r] * scale, o[r + 1] * scale, o[r + 2] * scale, o[r + 3] * scale);
+      }
+  }
+  __syncthreads();
+  const int64_t at = ((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * gridDim.x + part;
+  float4 *const out = reinterpret_cast<float4 *>(a.workspace) + at * rows * (HS / 4);
+  for (int i = threadIdx.x; i < rows * (HS / 4); i += 256) {
+    const float *x = shared + i / (HS / 4) * STRIDE + i % (HS / 4) * 4;
+    float4 y = *reinterpret_cast<const float4 *>(x);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 z = *reinterpret_cast<const float4 *>(x + w * rows * STRIDE);
+      y.x += z.x;
+      y.y += z.y;
+      y.z += z.z;
+      y.w += z.w;
+    }
+    out[i] = y;
+  }
+  if (threadIdx.x < rows)  // (wave 0: lane = column)
+    (reinterpret_cast<float4 *>(a.workspace) + (int64_t)gridDim.x * gridDim.y * gridDim.z * rows * (HS / 4))[
+        at * rows + tile.col] = make_float4(m, l, mw, 0.0f);
+}
+
+// A row's parts together: one (tile row, kv head, tile) a workgroup
+template <int HS>
+__global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int tokens_log2, int rows, int parts) {
+  constexpr int QUADS = HS / 4, GROUPS = 256 / QUADS;
+  __shared__ float4 sums[GROUPS * QUADS];
+  __shared__ float scales[256];
+  __shared__ float tops[2][4], total[4];
+  const int tid = threadIdx.x, r = blockIdx.x, head = blockIdx.y, tile = blockIdx.z;
+  const int pos = a.rows.dpos ? *a.rows.dpos : a.rows.pos, group = a.nh / a.rows.c.nkv;
+  const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + r / group;
+  if (token < pos || token >= pos + a.rows.count) return;  // (the whole workgroup)
+  const int64_t at = ((int64_t)tile * gridDim.y + head) * parts;
+  const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (at * rows + r) * QUADS;
+  const float4 *stats = reinterpret_cast<const float4 *>(a.workspace) + (int64_t)parts * gridDim.y * gridDim.z * rows * QUADS +
+                        at * rows + r;
+  const float4 mine = tid < parts ? stats[(int64_t)tid * rows] : make_float4(NONE, 0.0f, NONE, 0.0f);
+  float m = mine.x, mw = mine.z;
+#pragma unroll
+  for (int x = 32; x; x >>= 1) {
+    m = __builtin_fmaxf(m, __shfl_xor(m, x));
+    mw = __builtin_fmaxf(mw, __shfl_xor(mw, x));
+  }
+  if (tid % 64 == 0) {
+    tops[0][tid / 64] = m;
+    tops[1][tid / 64] = mw;
+  }
+  __syncthreads();
+  m = __builtin_fmaxf(__builtin_fmaxf(tops[0][0], tops[0][1]), __builtin_fmaxf(tops[0][2], tops[0][3]));
+  mw = __builtin_fmaxf(__builtin_fmaxf(tops[1][0], tops[1][1]), __builtin_fmaxf(tops[1][2], tops[1][3]));
+  float l = mine.y * __builtin_amdgcn_exp2f(mine.x - m);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
+  if (tid % 64 == 0) total[tid / 64] = l;
+  scales[tid] = __builtin_amdgcn_exp2f(mine.z - mw);
+  __syncthreads();
+  l = (total[0] + total[1]) + (total[2] + total[3]);
+  if (tid < GROUPS * QUADS) {
+    float4 y = make_float4(0, 0, 0, 0);
+    for (int p = tid / QUADS; p < parts; p += GROUPS) {
+      const float4 x = o[(int64_t)p * rows * QUADS + tid % QUADS];
+      const float f = scales[p];
+      y.x = __builtin_fmaf(x.x, f, y.x);
+      y.y = __builtin_fmaf(x.y, f, y.y);
+      y.z = __builtin_fmaf(x.z, f, y.z);
+      y.w = __builtin_fmaf(x.w, f, y.w);
+    }
+    sums[tid] = y;
+  }
+  __syncthreads();
+  if (tid >= QUADS) return;
+  float4 y = sums[tid];
+  for (int g = 1; g < GROUPS; ++g) {
+    const float4 x = sums[g * QUADS + tid];
+    y.x += x.x;
+    y.y += x.y;
+    y.z += x.z;
+    y.w += x.w;
+  }
+  const float scale = __builtin_amdgcn_exp2f(mw - m - 14.0f) / l;
+  float *out = a.out + (int64_t)(token - pos) * a.out_stride + (head * group + r % group) * HS + 4 * tid;
+  *reinterpret_cast<float4 *>(out) = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
+}
+
+// How a call is laid out: the tokens a tile takes (2^log2: the largest power of two whose rows, token and query head, are at
+// most 32, so that tiles, which start at its multiples, never straddle two blocks), and the parts a tile's blocks are split
+// into where there are too few tiles for the card's 1024 SIMDs (0: one wave a tile)
+struct Layout {
+  int log2, rows, tiles, splits;
+};
+constexpr int PARTS_MOST = 255;  // parts that attend_join_kernel takes, less the own block's
+int tokens_log2(int group) {
+  int log2 = 0;
+  while (log2 < 5 && (2 << log2) * group <= 32) ++log2;
+  return log2;
+}
+int splits_for(int64_t waves, int blocks) {
+  if (waves >= 2048) return 0;
+  const int64_t wanted = std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(wanted, (blocks + 3) / 4));
+}
+Layout layout_of(const CacheAttn &a) {
+  Layout l;
+  l.log2 = tokens_log2(a.nh / a.rows.c.nkv);
+  l.rows = a.nh / a.rows.c.nkv << l.log2;
+  const int last = a.rows.pos + a.rows.count - 1;
+  l.tiles = (last >> l.log2) - (a.rows.pos >> l.log2) + 1;
+  l.splits = splits_for((int64_t)l.tiles * a.rows.c.nkv, last / CACHE_BLOCK);
+  return l;
+}
+
+template <int HS>
+hipError_t launch(const CacheAttn &a, hipStream_t s) {
+  const Layout l = layout_of(a);
+  if (!l.splits) {
+    hipLaunchKernelGGL(attend_kernel<HS>, dim3((l.tiles + 3) / 4, a.rows.c.nkv), dim3(256), 0, s, a, l.log2);
+    return hipGetLastError();
+  }
+  const size_t bytes = std::max<size_t>(4 * l.rows * (HS + 4), 4 * 16 * 64) * sizeof(float);
+  if (bytes > 65536) {
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(attend_part_kernel<HS>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (err != hipSuccess) return err;
+  }
+  hipLaunchKernelGGL(attend_part_kernel<HS>, dim3(l.splits + 1, l.tiles, a.rows.c.nkv), dim3(256), bytes, s, a, l.log2,
+                     l.rows, l.splits);
+  hipLaunchKernelGGL(attend_join_kernel<HS>, dim3(l.rows, a.rows.c.nkv, l.tiles), dim3(256), 0, s, a, l.log2, l.rows,
+                     l.splits + 1);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t cache_attention_workspace(const CacheView &, int32_t, int32_t) { return 0; }
+// (the most over the positions: the fewest tiles that count tokens make give the most parts, the most tiles the most rows)
+int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count) {
+  const int log2 = tokens_log2(nh / c.nkv);
+  const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2;
+  const int splits = splits_for(fewest * c.nkv, c.blocks);
+  return splits ? (fewest + 1) * c.nkv * (splits + 1) * rows * (c.hs + 4) * (int64_t)sizeof(float) : 0;
+}
 
 hipError_t launch_cache_attention(const CacheAttn &args, hipStream_t s) {
   CacheAttn a = args;
   a.rows.displaced = cache_displaces(a.rows.pos, a.rows.count);
-  // tokens a tile: the largest power of two whose rows (token, query head) are at most 32, so that tiles that start at its
-  // multiples never straddle two blocks
-  const int group = a.nh / a.rows.c.nkv;
-  int log2 = 0;
-  while (log2 < 5 && (2 << log2) * group <= 32) ++log2;
-  const int tiles = ((a.rows.pos + a.rows.count - 1) >> log2) - (a.rows.pos >> log2) + 1;
-  const dim3 grid((tiles + 3) / 4, a.rows.c.nkv);
   switch (a.rows.c.hs) {
-    case 16: hipLaunchKernelGGL(attend_kernel<16>, grid, dim3(256), 0, s, a, log2); break;
-    case 32: hipLaunchKernelGGL(attend_kernel<32>, grid, dim3(256), 0, s, a, log2); break;
-    case 48: hipLaunchKernelGGL(attend_kernel<48>, grid, dim3(256), 0, s, a, log2); break;
-    case 64: hipLaunchKernelGGL(attend_kernel<64>, grid, dim3(256), 0, s, a, log2); break;
-    case 96: hipLaunchKernelGGL(attend_kernel<96>, grid, dim3(256), 0, s, a, log2); break;
-    case 128: hipLaunchKernelGGL(attend_kernel<128>, grid, dim3(256), 0, s, a, log2); break;
-    case 256: hipLaunchKernelGGL(attend_kernel<256>, grid, dim3(256), 0, s, a, log2); break;
-    default: return hipErrorInvalidValue;
+    case 16: return launch<16>(a, s);
+    case 32: return launch<32>(a, s);
+    case 48: return launch<48>(a, s);
+    case 64: return launch<64>(a, s);
+    case 96: return launch<96>(a, s);
+    case 128: return launch<128>(a, s);
+    case 256: return launch<256>(a, s);
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 }  // namespace ple

@@ -17,7 +17,7 @@ def value_byte(t):
 def quantize(x):
     """(int values, float32 scale) of a block's values of one head"""
     with np.errstate(invalid="ignore", divide="ignore"):
-        s = np.float32(np.max(np.abs(x))) / np.float32(127)
+        s = np.float32(np.max(np.abs(x))) * np.float32(1 / 127)
         if not np.isfinite(s) or s == 0:
             return np.zeros(x.shape, dtype=np.int64), s
     return np.rint(x.astype(np.float64) / np.float64(s)).astype(np.int64), s

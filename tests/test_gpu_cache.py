@@ -63,12 +63,14 @@ def test_quantization_at_its_borders():
     for b in range(6):
         for h in range(nkv):
             for x in (k, v):
-                s = np.float32(rng.choice([1.0, 0.37, 2.0 ** -126, 1e-41, 1e36, 3.7e-9]))
+                largest = np.float32(rng.choice([127.0, 0.37, 2.0 ** -120, 1e-39, 1e38, 3.7e-9]))
+                s = largest * np.float32(1 / 127)
                 steps = rng.integers(-126, 126, (32, hs)) + 0.5
                 near = (steps * np.float64(s)).astype(np.float32)
                 for other in (np.nextafter(near, np.float32(1e38)), np.nextafter(near, np.float32(-1e38))):
                     near = np.where(rng.random(near.shape) < 0.3, other, near)
-                near[0, 0] = np.float32(127) * s
+                near = np.clip(near, -largest, largest)
+                near[0, 0] = largest
                 x[b * 32:b * 32 + 32, h] = near
     k[64:96, 1] = 0
     cache, model = Cache(nkv, hs, n), Model(nkv, hs, n)
