@@ -39,6 +39,13 @@ extern "C" {
 #define HE_ARCH_NEOX 2  /* "neox": GPT-2's layer with RoPE over the first `rotary` values of every head */
 #define HE_OUTLIERS_MOST 8 /* OUTLIER_CHANNELS (public/llama2_numpy.py:561) */
 
+/* he_config.half_kv for a cache held in 8 bits (hk_cache): a quarter of float32's bytes a position, and contexts of up to
+ * HK_CACHE_MOST positions. Its attention is hk_cache_attention's, in float32 accuracy over what the cache stands for, not
+ * the reference's order: logits follow the reference's with the cache's rounding. A token's numbers do not depend on how
+ * the tokens before it were split into calls, to the rounding of float32 sums. A step back to a position of the latest 96
+ * finds its block's float32 rows; further back, the block's earlier positions stand as their 8-bit values. */
+#define HE_KV_EIGHT 8
+
 /* The model: the fields of `plan` (public/llama2_numpy.py:1261-1270) the forward reads. */
 typedef struct he_config {
   int32_t dim;               /* plan.dim */
@@ -53,7 +60,8 @@ typedef struct he_config {
   int32_t six;               /* the matrices are int6 (Tensor kind "int6"), else int8 */
   int32_t qkv_bias;          /* Qwen2: bq, bk, bv are added after the q, k, v matmuls (public/forward.js:1038-1042) */
   int32_t relaxed;           /* 1: activations with bias 64, matmul_q8r order; 0: bias 0, matmul_q8 lane order */
-  int32_t half_kv;           /* keys and values kept in float16 (public/forward.js:762, kernels/kernel.ts:570-608) */
+  int32_t half_kv;           /* keys and values kept in float16 (public/forward.js:762, kernels/kernel.ts:570-608);
+                                HE_KV_EIGHT: in 8 bits (below), a form of the engine's own */
   float rms_norm_eps;        /* plan.rms_norm_eps (RMSNorm; LayerNorm's is 1e-5, kernels/kernel.ts:627) */
   int32_t arch;              /* plan.arch: HE_ARCH_* */
   int32_t rotary;            /* plan.rotary: the values of each head RoPE turns (neox); 0 or head_size: all */
@@ -110,7 +118,7 @@ const char *he_last_error(void);
 /* start(plan) (public/forward.js:571-590, createForward :626): uploads `size` bytes of checkpoint (host memory) to the
  * device, the RoPE tables plan.derived.freq_cis_real/imag ([seq_len][head_size/2] float32, host), and makes the
  * KV cache for the whole context. max_block: the most tokens one he_forward_many call takes (promptBlock).
- * seq_len may be at most 40,704 positions (HE_E_ARG past it): a (token, head)'s exponentials are held in one
+ * seq_len may be at most 40,704 positions (HE_E_ARG past it; HK_CACHE_MOST with HE_KV_EIGHT): a (token, head)'s exponentials are held in one
  * workgroup's 160 KiB of LDS for their ordered sum (kernels/kernel.ts:499-520). */
 int32_t he_open(const he_config *cfg, const he_tensor *tensors, const void *checkpoint, uint64_t size,
                 const float *rope_cos, const float *rope_sin, int32_t max_block, he_engine **out);
@@ -158,8 +166,22 @@ int32_t he_generate_many(he_engine *e, int32_t token, int32_t pos, const int32_t
 /* engine.logits() (public/forward.js:1936): the logits of the last step with logits, vocab_size floats (host). */
 int32_t he_logits(he_engine *e, float *out);
 
+/* No counterpart in the reference: he_forward_many, and for each token the log probabilities of what follows it. With row
+ * i of the logits those he_forward gives token i: logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens given
+ * [count][n_given], the entropy [count] (or null), and the top (0..32) most probable tokens, ids [count][top] and logps
+ * [count][top], as hk_logprobs gives them (host arrays). To score a text: given[i] = tokens[i + 1]. count <=
+ * he_prompt_block(e). The first call allocates a piece's logits (256 rows). he_logits is not changed. Blocks until done. */
+int32_t he_score(he_engine *e, const int32_t *tokens, int32_t count, int32_t pos, const int32_t *given, int32_t n_given,
+                 int32_t top, float *logp, float *entropy, int32_t *ids, float *logps);
+
+/* No counterpart in the reference: the log probabilities under the logits that he_logits gives (after the repetition
+ * penalty, where the last step applied one): of the n_given tokens given, the entropy (or null), and the top most probable
+ * tokens (host arrays), as hk_logprobs gives them. Blocks until done. */
+int32_t he_logprobs(he_engine *e, const int32_t *given, int32_t n_given, int32_t top, float *logp, float *entropy,
+                    int32_t *ids, float *logps);
+
 /* engine.keysAndValues(from, count) (public/forward.js:1939-1953): the cache at positions from..from+count-1 as
- * float32 [layers][count][kv_dim], keys then values (host). */
+ * float32 [layers][count][kv_dim], keys then values (host). A cache in 8 bits: as the next token would read them. */
 int32_t he_kv_read(he_engine *e, int32_t from, int32_t count, float *keys, float *values);
 
 /* external().read(offset, length) (public/forward.js:574): bytes of the checkpoint as the device holds them. */

@@ -99,15 +99,15 @@ __global__ __launch_bounds__(256) void set_apart_kernel(const CacheView c, int f
   }
 }
 
-// positions from.. as float32 rows: those before `bound` by their 8-bit values, the others from the recent rows; into
+// positions from.. as float32 rows: by their 8-bit values, those of block `recent_block` from the recent rows; into
 // k / v [count][n_kv * hs], or (k null) into the recent rows
-__global__ __launch_bounds__(256) void read_kernel(const CacheView c, float *k, float *v, int from, int bound) {
+__global__ __launch_bounds__(256) void read_kernel(const CacheView c, float *k, float *v, int from, int recent_block) {
   const int p = from + blockIdx.x, width = c.nkv * c.hs, block = p / CACHE_BLOCK, t = p % CACHE_BLOCK;
   const int64_t recent = (int64_t)(p % CACHE_RECENT) * width;
   for (int i = threadIdx.x; i < width; i += 256) {
     const int head = i / c.hs, d = i % c.hs;
     float kv, vv;
-    if (p < bound) {
+    if (block != recent_block) {
       const int64_t at = (int64_t)head * c.blocks + block, base = at * CACHE_BLOCK * c.hs;
       kv = (float)c.keys[base + (d / 16 * CACHE_BLOCK + t) * 16 + d % 16] * c.scales[at * 2];
       vv = (float)((int)c.values[base + (int64_t)d * CACHE_BLOCK + value_byte(t)] - 128) * c.scales[at * 2 + 1];
@@ -152,9 +152,9 @@ hipError_t launch_cache_append(const CacheRows &rows, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t bound,
+hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t recent,
                              hipStream_t s) {
-  hipLaunchKernelGGL(read_kernel, dim3(count), dim3(256), 0, s, c, keys, values, from, bound);
+  hipLaunchKernelGGL(read_kernel, dim3(count), dim3(256), 0, s, c, keys, values, from, recent);
   return hipGetLastError();
 }
 

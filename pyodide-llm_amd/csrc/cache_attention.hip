@@ -330,11 +330,15 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const Ca
     }
 }
 
-// Few tiles: the blocks of a tile in `splits` parts, one a workgroup, whose four waves take them in turn, and one part more
-// for the tile's own block (the first, which takes the longest). A part's statistics (m, l, mw) and outputs go to the
+// the parts a tile's `own` earlier blocks are split into, of `most` at most: a block for each of a part's four waves at
+// least. (By the tile alone, not by the launch, which may not know its position: the same sums either way.)
+__device__ __forceinline__ int parts_of(int own, int most) { return max(1, min(most, (own + 3) / 4)); }
+
+// Few tiles: the blocks of a tile in parts, one a workgroup, whose four waves take them in turn, and one part more for the
+// tile's own block (the first, which takes the longest). A part's statistics (m, l, mw) and outputs go to the
 // workspace: outputs [tile][kv head][part][rows][HS], then statistics [tile][kv head][part][rows] of 4 floats.
 template <int HS>
-__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(const CacheAttn a, int tokens_log2, int rows, int splits) {
+__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(const CacheAttn a, int tokens_log2, int rows, int most) {
   extern __shared__ float4 lds[];
   constexpr int STRIDE = HS + 4;  // (rows of a wave's outputs 4 banks apart)
   float *const shared = reinterpret_cast<float *>(lds);
@@ -343,6 +347,8 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
   Tile<HS> tile;
   tile.head = blockIdx.z;
   tile.place(a, blockIdx.y, tokens_log2);
+  const int splits = parts_of(tile.own, most);
+  if (part > splits) return;  // (the whole workgroup)
   if (part == 0) {
     tile.template own_block<4>(a, wave, shared);
     __syncthreads();  // (shared holds the outputs next)
@@ -406,7 +412,7 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
 
 // A row's parts together: one (tile row, kv head, tile) a workgroup
 template <int HS>
-__global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int tokens_log2, int rows, int parts) {
+__global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int tokens_log2, int rows, int most, int stride) {
   constexpr int QUADS = HS / 4, GROUPS = 256 / QUADS;
   __shared__ float4 sums[GROUPS * QUADS];
   __shared__ float scales[256];
@@ -415,9 +421,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
   const int pos = a.rows.dpos ? *a.rows.dpos : a.rows.pos, group = a.nh / a.rows.c.nkv;
   const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + r / group;
   if (token < pos || token >= pos + a.rows.count) return;  // (the whole workgroup)
-  const int64_t at = ((int64_t)tile * gridDim.y + head) * parts;
+  const int parts = parts_of(token / CACHE_BLOCK, most) + 1;
+  const int64_t at = ((int64_t)tile * gridDim.y + head) * stride;
   const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (at * rows + r) * QUADS;
-  const float4 *stats = reinterpret_cast<const float4 *>(a.workspace) + (int64_t)parts * gridDim.y * gridDim.z * rows * QUADS +
+  const float4 *stats = reinterpret_cast<const float4 *>(a.workspace) + (int64_t)stride * gridDim.y * gridDim.z * rows * QUADS +
                         at * rows + r;
   const float4 mine = tid < parts ? stats[(int64_t)tid * rows] : make_float4(NONE, 0.0f, NONE, 0.0f);
   float m = mine.x, mw = mine.z;
@@ -468,10 +475,10 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
 }
 
 // How a call is laid out: the tokens a tile takes (2^log2: the largest power of two whose rows, token and query head, are at
-// most 32, so that tiles, which start at its multiples, never straddle two blocks), and the parts a tile's blocks are split
-// into where there are too few tiles for the card's 1024 SIMDs (0: one wave a tile)
+// most 32, so that tiles, which start at its multiples, never straddle two blocks), and the most parts a tile's blocks are
+// split into where there are too few tiles for the card's 1024 SIMDs (0: one wave a tile)
 struct Layout {
-  int log2, rows, tiles, splits;
+  int log2, rows, tiles, most;
 };
 constexpr int PARTS_MOST = 255;  // parts that attend_join_kernel takes, less the own block's
 int tokens_log2(int group) {
@@ -479,25 +486,23 @@ int tokens_log2(int group) {
   while (log2 < 5 && (2 << log2) * group <= 32) ++log2;
   return log2;
 }
-int splits_for(int64_t waves, int blocks) {
-  if (waves >= 2048) return 0;
-  const int64_t wanted = std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(wanted, (blocks + 3) / 4));
+int most_parts(int64_t waves) {
+  return waves >= 2048 ? 0 : (int)std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves);
 }
 Layout layout_of(const CacheAttn &a) {
   Layout l;
-  l.log2 = tokens_log2(a.nh / a.rows.c.nkv);
-  l.rows = a.nh / a.rows.c.nkv << l.log2;
-  const int last = a.rows.pos + a.rows.count - 1;
-  l.tiles = (last >> l.log2) - (a.rows.pos >> l.log2) + 1;
-  l.splits = splits_for((int64_t)l.tiles * a.rows.c.nkv, last / CACHE_BLOCK);
+  const int group = a.nh / a.rows.c.nkv;
+  l.log2 = tokens_log2(group);
+  l.rows = group << l.log2;
+  l.tiles = ((a.rows.pos + a.rows.count - 1) >> l.log2) - (a.rows.pos >> l.log2) + 1;
+  l.most = most_parts((int64_t)l.tiles * a.rows.c.nkv);
   return l;
 }
 
 template <int HS>
 hipError_t launch(const CacheAttn &a, hipStream_t s) {
   const Layout l = layout_of(a);
-  if (!l.splits) {
+  if (!l.most) {
     hipLaunchKernelGGL(attend_kernel<HS>, dim3((l.tiles + 3) / 4, a.rows.c.nkv), dim3(256), 0, s, a, l.log2);
     return hipGetLastError();
   }
@@ -507,10 +512,11 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (err != hipSuccess) return err;
   }
-  hipLaunchKernelGGL(attend_part_kernel<HS>, dim3(l.splits + 1, l.tiles, a.rows.c.nkv), dim3(256), bytes, s, a, l.log2,
-                     l.rows, l.splits);
+  const int last = (a.rows.pos + a.rows.count - 1) / CACHE_BLOCK, stride = std::max(1, std::min(l.most, (last + 3) / 4)) + 1;
+  hipLaunchKernelGGL(attend_part_kernel<HS>, dim3(stride, l.tiles, a.rows.c.nkv), dim3(256), bytes, s, a, l.log2, l.rows,
+                     l.most);
   hipLaunchKernelGGL(attend_join_kernel<HS>, dim3(l.rows, a.rows.c.nkv, l.tiles), dim3(256), 0, s, a, l.log2, l.rows,
-                     l.splits + 1);
+                     l.most, stride);
   return hipGetLastError();
 }
 
@@ -520,8 +526,8 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
 int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count) {
   const int log2 = tokens_log2(nh / c.nkv);
   const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2;
-  const int splits = splits_for(fewest * c.nkv, c.blocks);
-  return splits ? (fewest + 1) * c.nkv * (splits + 1) * rows * (c.hs + 4) * (int64_t)sizeof(float) : 0;
+  const int most = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4);
+  return most ? (fewest + 1) * c.nkv * (most + 1) * rows * (c.hs + 4) * (int64_t)sizeof(float) : 0;
 }
 
 hipError_t launch_cache_attention(const CacheAttn &args, hipStream_t s) {

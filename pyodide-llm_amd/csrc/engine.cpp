@@ -93,6 +93,9 @@ Shape shape_of(const he_config &c, int id) {
   return {0, 0, 0, 0};
 }
 
+// the cache held in 8 bits (cache.hpp), in place of float32 or float16
+bool eight(const he_config &c) { return c.half_kv == HE_KV_EIGHT; }
+
 bool layer_norm(const he_config &c) { return c.arch == HE_ARCH_GPT2 || c.arch == HE_ARCH_NEOX; }
 
 // the tensors of the form (public/llama2_convert.py:32-83): Llama's with Qwen2's biases and Qwen3's head norms where
@@ -154,6 +157,16 @@ struct he_engine {
   const float *scales[HE_T_COUNT]{};
   float *cos_t = nullptr, *sin_t = nullptr;
   void *keys = nullptr, *vals = nullptr;  // keys [layers][seq_len][kv_dim], values [layers][kv_dim][value_stride]
+  // the cache in 8 bits: the scales and the recent float32 rows of every layer (keys and vals hold the bytes), the
+  // attention's workspace; positions rows_from..rows_to - 1 have their float32 rows among the recent ones, and the next
+  // token is taken to stand at cache_end
+  float *cache_scales = nullptr, *recent_keys = nullptr, *recent_values = nullptr, *cache_space = nullptr;
+  int32_t rows_from = 0, rows_to = 0, cache_end = 0;
+  // he_score and he_logprobs (made at their first call): a piece's logits, the log probabilities' workspace, what is asked
+  // and what comes back
+  float *score_logits = nullptr;
+  uint8_t *score_space = nullptr, *score_io = nullptr;
+  int64_t score_space_bytes = 0, score_io_bytes = 0;
   int32_t qdim = 0, kvdim = 0, bias = 64, max_block = 1, chunk = 1, xw = 0, widest = 0;
   // activations of `chunk` tokens
   float *x = nullptr, *xb = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *hb = nullptr, *hb2 = nullptr;
@@ -224,6 +237,31 @@ struct he_engine {
 
 namespace {
 
+// layer l of the cache in 8 bits
+CacheView cache_view(const he_engine *e, int32_t l) {
+  const he_config &c = e->c;
+  const int32_t blocks = (c.seq_len + 31) / 32;
+  const size_t bytes = (size_t)l * blocks * 32 * e->kvdim, rows = (size_t)l * CACHE_ROWS * e->kvdim;
+  return {reinterpret_cast<int8_t *>(e->keys) + bytes, reinterpret_cast<uint8_t *>(e->vals) + bytes,
+          e->cache_scales + (size_t)l * blocks * c.n_kv_heads * 2, e->recent_keys + rows, e->recent_values + rows,
+          c.n_kv_heads, c.head_size, blocks};
+}
+
+// the cache in 8 bits before count tokens at pos: where their block's earlier float32 rows are no longer held (a step far
+// back), they are taken from its 8-bit values
+int32_t cache_moves(he_engine *e, int32_t pos, int32_t count) {
+  if (!eight(e->c)) return HE_OK;
+  const int32_t first = pos / 32 * 32;
+  const bool held = e->rows_from <= first && pos <= e->rows_to;
+  if (!held && pos > first)
+    for (int32_t l = 0; l < e->c.n_layers; ++l)
+      HIP_TRY(launch_cache_read(cache_view(e, l), nullptr, nullptr, first, pos - first, -1, e->stream));
+  if (!held) e->rows_from = first;
+  e->rows_to = e->cache_end = pos + count;
+  e->rows_from = std::max(e->rows_from, e->rows_to - 128);
+  return HE_OK;
+}
+
 constexpr int32_t STEPS_A_ROUND = 64;      // replayed steps between two reads of their tokens
 constexpr int32_t STOP_ROUND = 16;         // the same where a stop token may end the call early (the round's later
                                            // replays are then spent for nothing)
@@ -240,7 +278,8 @@ void destroy(he_engine *e) {
                   e->xq, e->xs, e->scores, e->tilemax, e->logits, e->tokens, e->amax_v, e->amax_i,
                   e->best_v, e->best_i, e->state, e->step_ids, e->step_values, e->sample_probs, e->sample_index,
                   e->window, e->sample_token, e->sample_best, e->before, e->columns, e->picked, e->sink,
-                  e->run_params, e->kept_logits, e->sample_parts};
+                  e->run_params, e->kept_logits, e->sample_parts, e->cache_scales, e->recent_keys, e->recent_values,
+                  e->cache_space, e->score_logits, e->score_space, e->score_io};
   for (void *p : ptrs)
     if (p) (void)hipFree(p);
   void *pinned[] = {e->host_ids, e->host_state, e->host_values, e->host_window, e->host_params};
@@ -262,7 +301,9 @@ int32_t check_config(const he_config &c) {
   if (!attention_supported(c.head_size, c.n_heads, c.n_kv_heads))
     return fail(HE_E_ARG, "attention takes head sizes 16, 32, 48, 64, 96, 128, 256 and at most 8 query heads a kv head");
   if (c.seq_len % 4) return fail(HE_E_ARG, "seq_len must be a multiple of 4");
-  if (c.seq_len > attention_most_positions())
+  if (eight(c) && c.seq_len > HK_CACHE_MOST)
+    return fail(HE_E_ARG, "seq_len is longer than the cache in 8 bits takes (16777216 positions)");
+  if (!eight(c) && c.seq_len > attention_most_positions())
     return fail(HE_E_ARG, "seq_len is longer than the attention kernels take (" +
                               std::to_string(attention_most_positions()) + " positions)");
   if (c.arch != HE_ARCH_LLAMA && c.arch != HE_ARCH_GPT2 && c.arch != HE_ARCH_NEOX)
@@ -365,8 +406,22 @@ int32_t allocate_state(he_engine *e, const float *rope_cos, const float *rope_si
   ALLOC(e->sin_t, table);
   HIP_TRY(hipMemcpy(e->cos_t, rope_cos, table, hipMemcpyHostToDevice));
   HIP_TRY(hipMemcpy(e->sin_t, rope_sin, table, hipMemcpyHostToDevice));
-  const size_t kv = (size_t)c.n_layers * c.seq_len * e->kvdim * (c.half_kv ? 2 : 4);
-  const size_t kv_values = (size_t)c.n_layers * value_stride(c.seq_len) * e->kvdim * (c.half_kv ? 2 : 4);
+  size_t kv = (size_t)c.n_layers * c.seq_len * e->kvdim * (c.half_kv ? 2 : 4);
+  size_t kv_values = (size_t)c.n_layers * value_stride(c.seq_len) * e->kvdim * (c.half_kv ? 2 : 4);
+  if (eight(c)) {
+    const CacheView v = cache_view(e, 0);
+    const size_t blocks = (size_t)c.n_layers * v.blocks, rows = (size_t)c.n_layers * CACHE_ROWS * e->kvdim * sizeof(float);
+    kv = kv_values = blocks * 32 * e->kvdim;
+    ALLOC(e->cache_scales, blocks * c.n_kv_heads * 2 * sizeof(float));
+    ALLOC(e->recent_keys, rows);
+    ALLOC(e->recent_values, rows);
+    HIP_TRY(hipMemset(e->cache_scales, 0, blocks * c.n_kv_heads * 2 * sizeof(float)));
+    HIP_TRY(hipMemset(e->recent_keys, 0, rows));
+    HIP_TRY(hipMemset(e->recent_values, 0, rows));
+    int64_t space = 1;
+    for (int32_t m = 1; m <= T; ++m) space = std::max(space, cache_attention_workspace(v, c.n_heads, m));
+    ALLOC(e->cache_space, (size_t)space);
+  }
   ALLOC(e->keys, kv);
   ALLOC(e->vals, kv_values);
   HIP_TRY(hipMemset(e->keys, 0, kv));
@@ -381,8 +436,10 @@ int32_t allocate_state(he_engine *e, const float *rope_cos, const float *rope_si
   ALLOC(e->xq, (size_t)T * e->widest);
   ALLOC(e->xs, sizeof(float) * T * (e->widest / 32));
   const size_t rows = std::min(T, ATTN_ROWS);  // launch_attention's pieces reuse these rows
-  ALLOC(e->scores, sizeof(float) * rows * c.n_heads * (size_t)c.seq_len);
-  ALLOC(e->tilemax, sizeof(float) * rows * c.n_heads * (size_t)(c.seq_len / 64 + 1));
+  if (!eight(c)) {
+    ALLOC(e->scores, sizeof(float) * rows * c.n_heads * (size_t)c.seq_len);
+    ALLOC(e->tilemax, sizeof(float) * rows * c.n_heads * (size_t)(c.seq_len / 64 + 1));
+  }
   ALLOC(e->logits, sizeof(float) * c.vocab_size);
   ALLOC(e->tokens, sizeof(int32_t) * T);
   ALLOC(e->amax_v, sizeof(float) * 256);
@@ -637,6 +694,10 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
   const int32_t W = e->widest;
   const size_t esz = c.half_kv ? 2 : 4;
   const int32_t *dpos = e->replayable ? e->state : nullptr;  // a replayed step: the position in device memory
+  if (!e->replayable) {
+    const int32_t rc = cache_moves(e, pos0, m);
+    if (rc) return rc;
+  }
   if (!e->replayable) HIP_TRY(hipMemcpyAsync(e->tokens, tokens, sizeof(int32_t) * m, hipMemcpyHostToDevice, s));
   const bool ln = layer_norm(c);  // GPT-2 / GPT-NeoX: LayerNorm, GELU, biases after every matrix
   Positions positions{};
@@ -663,8 +724,10 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
     qp.bv = biases ? e->vec(HE_T_BV, (int64_t)l * kvdim) : nullptr;
     qp.cos_t = e->cos_t;
     qp.sin_t = e->sin_t;
-    qp.kcache = reinterpret_cast<uint8_t *>(e->keys) + (size_t)l * c.seq_len * kvdim * esz;
-    qp.vcache = reinterpret_cast<uint8_t *>(e->vals) + (size_t)l * value_stride(c.seq_len) * kvdim * esz;
+    if (!eight(c)) {
+      qp.kcache = reinterpret_cast<uint8_t *>(e->keys) + (size_t)l * c.seq_len * kvdim * esz;
+      qp.vcache = reinterpret_cast<uint8_t *>(e->vals) + (size_t)l * value_stride(c.seq_len) * kvdim * esz;
+    }
     qp.nh = c.n_heads;
     qp.nkv = c.n_kv_heads;
     qp.hs = hs;
@@ -683,7 +746,7 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
     }
     // the q/k/v matmul adds the biases, rotates q and k and writes k and v into the cache itself where it can (Qwen3's
     // head norms stand between them)
-    const bool fuse_qkv = !c.qk_norm && (use_gemm(e, dim, m) ? gemm_finishes(qdim + 2 * kvdim, m, c.relaxed != 0)
+    const bool fuse_qkv = !c.qk_norm && !eight(c) && (use_gemm(e, dim, m) ? gemm_finishes(qdim + 2 * kvdim, m, c.relaxed != 0)
                                                              : m == 1 && decode_fuses_qkv(dim, c.six != 0, c.relaxed != 0));
     // one token of a small model (dim <= 1024): the q/k/v and w1/w3 GEMVs take the float32 token and run rmsnorm and
     // quantize_x in each block (an ordered sum of 256 steps at most), two launches a layer fewer. (At dim 4096 each
@@ -715,6 +778,17 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
       HIP_TRY(timed(e, HE_K_ELEMENTWISE, (double)m * (qdim + 2 * kvdim) * 8 + (double)m * 2 * kvdim * esz,
                     [&] { return launch_qkv_post(qp, s); }));
     }
+    CacheAttn ca{};
+    if (eight(c)) {
+      ca.rows = {cache_view(e, l), e->k, e->v, kvdim, m, pos0, dpos, 0};
+      ca.q = e->q;
+      ca.out = e->xb;
+      ca.nh = c.n_heads;
+      ca.q_stride = qdim;
+      ca.out_stride = e->xw;
+      ca.workspace = e->cache_space;
+      HIP_TRY(timed(e, HE_K_ELEMENTWISE, (double)m * kvdim * 2 * (8 + 1), [&] { return launch_cache_append(ca.rows, s); }));
+    }
     AttnArgs at{};
     at.q = e->q;
     at.q_stride = qdim;
@@ -743,7 +817,7 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
     // attention runs blocks of 16 columns); else the attention writes quantize_x of its output too where it can
     const bool wo_quantizes = quantizes_itself(e, qdim, m, dim);
     if (wo_quantizes) at.xq = nullptr;
-    const bool quantized = at.xq && attention_quantizes(at);
+    const bool quantized = at.xq && !eight(c) && attention_quantizes(at);
     if (!quantized) at.xq = nullptr;
     double kv_rows = 0;
     for (int32_t t = 0; t < m; ++t) kv_rows += pos0 + t + 1;
@@ -755,8 +829,8 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
     // where the GEMM finishes the FFN's activation and its quantize_x, its bytes and scales go where h1 and h3 would (hb
     // and hb2 hold [chunk][W] bytes and [chunk][W / 32] floats: ffn_in_gemm checks), apart from its input in xq / xs
     int8_t *const gq = reinterpret_cast<int8_t *>(e->hb);
-    HIP_TRY(timed(e, HE_K_ATTENTION, kv_rows * 2 * kvdim * esz + (double)m * qdim * 8,
-                  [&] { return launch_attention(at, s); }));
+    HIP_TRY(timed(e, HE_K_ATTENTION, kv_rows * 2 * kvdim * (eight(c) ? 1 : esz) + (double)m * qdim * 8,
+                  [&] { return eight(c) ? launch_cache_attention(ca, s) : launch_attention(at, s); }));
     if (quantized) {
       HIP_TRY(matmul(e, wo, 1, qdim, m, e->xq, e->xs));
     } else if (wo_quantizes) {
@@ -854,12 +928,18 @@ int32_t run_chunk(he_engine *e, const int32_t *tokens, int32_t m, int32_t pos0, 
   return HE_OK;
 }
 
-int32_t run_tokens(he_engine *e, const int32_t *tokens, int32_t count, int32_t pos0, bool need_logits) {
+int32_t tokens_fit(const he_engine *e, const int32_t *tokens, int32_t count, int32_t pos0) {
   if (count < 1) return fail(HE_E_ARG, "no tokens");
   if (pos0 < 0 || (int64_t)pos0 + count > e->c.seq_len)
     return fail(HE_E_STATE, "the positions run past the context (seq_len)");
   for (int32_t i = 0; i < count; ++i)
     if (tokens[i] < 0 || tokens[i] >= e->c.vocab_size) return fail(HE_E_ARG, "a token is outside the vocabulary");
+  return HE_OK;
+}
+
+int32_t run_tokens(he_engine *e, const int32_t *tokens, int32_t count, int32_t pos0, bool need_logits) {
+  const int32_t fits = tokens_fit(e, tokens, count, pos0);
+  if (fits) return fits;
   for (int32_t at = 0; at < count; at += e->chunk) {
     const int32_t m = std::min(e->chunk, count - at);
     const int32_t rc = run_chunk(e, tokens + at, m, pos0 + at, need_logits && at + m == count);
@@ -1119,6 +1199,8 @@ int32_t he_generate_many(he_engine *e, int32_t token, int32_t pos, const int32_t
     const int32_t n = std::min(round, count - done);
     for (int32_t i = 0; i < RUN_RANDOMS; ++i) hp.randoms[i] = temperature > 0.0f && i < n ? randoms[done + i] : 0.0;
     hp.steps = n;
+    const int32_t moved = cache_moves(e, pos + done, n);
+    if (moved) return moved;
     hs[STATE_WORDS] = token;
     hs[STATE_POS] = pos + done;
     hs[STATE_STEP] = 0;
@@ -1136,6 +1218,7 @@ int32_t he_generate_many(he_engine *e, int32_t token, int32_t pos, const int32_t
                            e->stream));
     HIP_TRY(hipStreamSynchronize(e->stream));
     const int32_t halted = hs[STATE_WORDS + 1];
+    if (halted) e->cache_end = pos + done + halted;
     for (int32_t j = 0; j < (halted ? halted : n); ++j) {
       const int32_t id = e->host_ids[j];
       if (halted && j == halted - 1) {
@@ -1272,9 +1355,32 @@ int32_t he_logits(he_engine *e, float *out) {
   return HE_OK;
 }
 
+namespace {
+// he_kv_read of the cache in 8 bits: as the token at cache_end reads the positions
+int32_t eight_read(he_engine *e, int32_t from, int32_t count, float *keys, float *values) {
+  if (count == 0) return HE_OK;
+  const size_t floats = (size_t)count * e->kvdim;
+  float *rows = nullptr;
+  int32_t rc = dev_alloc(&rows, 2 * floats * sizeof(float));
+  if (rc) return rc;
+  hipError_t err = hipSuccess;
+  for (int32_t l = 0; l < e->c.n_layers && err == hipSuccess; ++l) {
+    err = launch_cache_read(cache_view(e, l), rows, rows + floats, from, count, e->cache_end / 32, e->stream);
+    if (err == hipSuccess)
+      err = hipMemcpyAsync(keys + l * floats, rows, floats * sizeof(float), hipMemcpyDeviceToHost, e->stream);
+    if (err == hipSuccess)
+      err = hipMemcpyAsync(values + l * floats, rows + floats, floats * sizeof(float), hipMemcpyDeviceToHost, e->stream);
+    if (err == hipSuccess) err = hipStreamSynchronize(e->stream);
+  }
+  (void)hipFree(rows);
+  return err == hipSuccess ? HE_OK : fail(HE_E_HIP, std::string("he_kv_read: ") + hipGetErrorString(err));
+}
+}  // namespace
+
 int32_t he_kv_read(he_engine *e, int32_t from, int32_t count, float *keys, float *values) {
   if (!e || !keys || !values) return fail(HE_E_ARG, "a required pointer is null");
   if (from < 0 || count < 0 || (int64_t)from + count > e->c.seq_len) return fail(HE_E_ARG, "positions out of range");
+  if (eight(e->c)) return eight_read(e, from, count, keys, values);
   const size_t esz = e->c.half_kv ? 2 : 4, kvdim = e->kvdim, vs = value_stride(e->c.seq_len);
   std::vector<uint8_t> rows((size_t)count * kvdim * esz);
   auto widen = [&](size_t i) {  // element i of rows as float32
@@ -1312,6 +1418,124 @@ int32_t he_kv_read(he_engine *e, int32_t from, int32_t count, float *keys, float
       for (size_t p = 0; p < (size_t)count; ++p) vo[p * kvdim + col] = widen(col * count + p);
   }
   return HE_OK;
+}
+
+namespace {
+constexpr int32_t SCORE_ROWS = 256;  // tokens whose logits he_score holds at once (131 MB at a vocabulary of 128256)
+
+// the log probabilities of m rows of logits (device) for the host arrays of he_score / he_logprobs
+int32_t logprobs_to_host(he_engine *e, const float *logits, int32_t m, const int32_t *given, int32_t n_given, int32_t top,
+                         float *logp, float *entropy, int32_t *ids, float *logps) {
+  const int32_t n = e->c.vocab_size;
+  auto grown = [&](uint8_t *&p, int64_t &held, int64_t bytes) -> int32_t {
+    if (bytes <= held) return HE_OK;
+    if (p) (void)hipFree(p);
+    p = nullptr;
+    e->device_bytes -= held;
+    held = 0;
+    const int32_t rc = dev_alloc(&p, bytes);
+    if (rc == HE_OK) {
+      held = bytes;
+      e->device_bytes += bytes;
+    }
+    return rc;
+  };
+  const size_t asked = (size_t)m * n_given, told = (size_t)m * top;
+  int32_t rc = grown(e->score_space, e->score_space_bytes, logprobs_workspace(m, n, top));
+  if (!rc) rc = grown(e->score_io, e->score_io_bytes, 4 * (int64_t)(2 * asked + m + 2 * told));
+  if (rc) return rc;
+  int32_t *given_d = reinterpret_cast<int32_t *>(e->score_io), *ids_d = given_d + asked;
+  float *logp_d = reinterpret_cast<float *>(ids_d + told), *logps_d = logp_d + asked, *entropy_d = logps_d + told;
+  if (asked) HIP_TRY(hipMemcpyAsync(given_d, given, 4 * asked, hipMemcpyHostToDevice, e->stream));
+  const LogprobArgs a = {logp_d, entropy_d, ids_d, logps_d, logits, n, given_d, n_given, m, n, top, e->score_space};
+  HIP_TRY(launch_logprobs(a, e->stream));
+  if (asked) HIP_TRY(hipMemcpyAsync(logp, logp_d, 4 * asked, hipMemcpyDeviceToHost, e->stream));
+  if (entropy) HIP_TRY(hipMemcpyAsync(entropy, entropy_d, 4 * (size_t)m, hipMemcpyDeviceToHost, e->stream));
+  if (told) {
+    HIP_TRY(hipMemcpyAsync(ids, ids_d, 4 * told, hipMemcpyDeviceToHost, e->stream));
+    HIP_TRY(hipMemcpyAsync(logps, logps_d, 4 * told, hipMemcpyDeviceToHost, e->stream));
+  }
+  HIP_TRY(hipStreamSynchronize(e->stream));
+  return HE_OK;
+}
+
+int32_t asked_for(const char *what, const int32_t *given, int32_t n_given, int32_t top, const float *logp,
+                  const float *entropy, const int32_t *ids, const float *logps) {
+  if (n_given < 0 || (n_given > 0 && (!given || !logp)))
+    return fail(HE_E_ARG, std::string(what) + ": given tokens need given and logp");
+  if (top < 0 || top > LOGPROBS_TOP_MOST || (top > 0 && (!ids || !logps)))
+    return fail(HE_E_ARG, std::string(what) + ": top is in 0..32, and alternatives need ids and logps");
+  if (!n_given && !top && !entropy) return fail(HE_E_ARG, std::string(what) + ": nothing is asked for");
+  return HE_OK;
+}
+
+// the logits of rows at..at + m - 1 of a pass's m_all tokens, once run_chunk has run them, into score_logits: the bits that
+// run_chunk's own classifier gives each row
+int32_t score_classifier(he_engine *e, int32_t at, int32_t m) {
+  const he_config &c = e->c;
+  const int32_t dim = c.dim, W = e->widest, vocab = c.vocab_size;
+  const bool ln = layer_norm(c), apart = c.n_outliers > 0;
+  const float *x = e->x + (int64_t)at * dim;
+  hipStream_t s = e->stream;
+  HIP_TRY(ln ? launch_layernorm_quant(e->xq, e->xs, apart ? e->xb : nullptr, nullptr, x, e->vec(HE_T_RMS_FINAL, 0),
+                                      e->vec(HE_T_LN_FINAL_BIAS, 0), m, dim, dim, W, W / 32, e->xw, e->bias, s)
+             : launch_rmsnorm_quant(e->xq, e->xs, apart ? e->xb : nullptr, x, e->vec(HE_T_RMS_FINAL, 0), m, dim, dim, W,
+                                    W / 32, e->xw, c.rms_norm_eps, e->bias, s));
+  const uint8_t *w = e->mat(HE_T_WCLS, 0);
+  const float *ws = e->mat_scales(HE_T_WCLS, 0);
+  if (!apart) {
+    const MatSeg cls[1] = {{w, ws, e->score_logits, vocab, vocab, 0}};
+    HIP_TRY(matmul(e, cls, 1, dim, m, e->xq, e->xs));
+    return HE_OK;
+  }
+  for (int32_t i = 0; i < m; ++i) {  // (the outlier channels are taken out of one row at a time)
+    float *y = e->score_logits + (int64_t)i * vocab, *row = e->xb + (int64_t)i * e->xw;
+    const MatSeg cls[1] = {{w, ws, y, vocab, 0, 0}};
+    HIP_TRY(launch_pick(row, e->picked, e->outliers, s));
+    HIP_TRY(launch_quantize(e->xq, e->xs, row, 1, dim, e->xw, W, W / 32, e->bias, s));
+    HIP_TRY(matmul(e, cls, 1, dim, 1, e->xq, e->xs));
+    HIP_TRY(launch_add_columns(y, e->columns, e->picked, c.n_outliers, vocab, s));
+  }
+  return HE_OK;
+}
+}  // namespace
+
+int32_t he_score(he_engine *e, const int32_t *tokens, int32_t count, int32_t pos, const int32_t *given, int32_t n_given,
+                 int32_t top, float *logp, float *entropy, int32_t *ids, float *logps) {
+  if (!e || !tokens) return fail(HE_E_ARG, "engine or tokens is null");
+  if (count > e->max_block) return fail(HE_E_ARG, "more tokens than the prompt block");
+  int32_t rc = asked_for("he_score", given, n_given, top, logp, entropy, ids, logps);
+  if (!rc) rc = tokens_fit(e, tokens, count, pos);
+  if (rc) return rc;
+  const int32_t rows = std::min(SCORE_ROWS, e->chunk);
+  if (!e->score_logits) {
+    const size_t bytes = sizeof(float) * rows * (size_t)e->c.vocab_size;
+    if ((rc = dev_alloc(&e->score_logits, bytes))) return rc;
+    e->device_bytes += bytes;
+  }
+  for (int32_t at = 0; at < count; at += e->chunk) {
+    const int32_t m = std::min(e->chunk, count - at);
+    if ((rc = run_chunk(e, tokens + at, m, pos + at, false))) return rc;
+    for (int32_t i = 0; i < m; i += rows) {
+      const int32_t n = std::min(rows, m - i);
+      const int64_t r = at + i;
+      if ((rc = score_classifier(e, i, n))) return rc;
+      if ((rc = logprobs_to_host(e, e->score_logits, n, given ? given + r * n_given : nullptr, n_given, top,
+                                 logp ? logp + r * n_given : nullptr, entropy ? entropy + r : nullptr,
+                                 ids ? ids + r * top : nullptr, logps ? logps + r * top : nullptr)))
+        return rc;
+    }
+  }
+  return HE_OK;
+}
+
+int32_t he_logprobs(he_engine *e, const int32_t *given, int32_t n_given, int32_t top, float *logp, float *entropy,
+                    int32_t *ids, float *logps) {
+  if (!e) return fail(HE_E_ARG, "engine is null");
+  const int32_t rc = asked_for("he_logprobs", given, n_given, top, logp, entropy, ids, logps);
+  if (rc) return rc;
+  if (!e->have_logits) return fail(HE_E_STATE, "no step with logits has run");
+  return logprobs_to_host(e, e->logits_kept ? e->kept_logits : e->logits, 1, given, n_given, top, logp, entropy, ids, logps);
 }
 
 int32_t he_checkpoint_read(he_engine *e, uint64_t offset, uint64_t length, void *out) {

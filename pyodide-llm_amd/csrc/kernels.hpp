@@ -156,7 +156,7 @@ struct QkvPost {
   int32_t q_stride, kv_stride;
   const float *bq, *bk, *bv;
   const float *cos_t, *sin_t;  // [seq_len][hs/2]
-  void *kcache, *vcache;       // this layer's keys [seq_len][kv_dim] and values [kv_dim][vstride]
+  void *kcache, *vcache;       // this layer's keys [seq_len][kv_dim] and values [kv_dim][vstride]; null: k and v in place only
   int32_t nh, nkv, hs, pos0, m, half, vstride;
   const int32_t *dpos;  // the first position in device memory (a replayed decode step), or null: pos0
   int32_t rot;          // the values of each head RoPE turns (kernels/kernel.ts:344-357): hs all, 0 none (GPT-2)
@@ -206,6 +206,7 @@ struct CacheView {
   float *recent_keys, *recent_values;
   int32_t nkv, hs, blocks;
 };
+constexpr int32_t CACHE_ROWS = 128 + 32;  // the recent float32 rows a layer's cache holds
 // whether a call of count tokens at pos displaces earlier recent rows of its first block (of 32), which are then set
 // apart behind the 128
 inline bool cache_displaces(int32_t pos, int32_t count) { return (int64_t)pos + count > pos / 32 * 32 + 128; }
@@ -218,12 +219,13 @@ struct CacheRows {
   int32_t displaced;    // set by the launch
 };
 hipError_t launch_cache_append(const CacheRows &a, hipStream_t s);
-// positions from..from + count - 1: those before bound by their 8-bit values, the others (within the latest 128) by their
-// float32 rows, into keys / values [count][nkv * hs] (null: into the recent rows)
-hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t bound,
+// positions from..from + count - 1 by their 8-bit values, those of block `recent` (-1: none) by their float32 rows, into
+// keys / values [count][nkv * hs] (null: into the recent rows)
+hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t recent,
                              hipStream_t s);
 // the attention of count tokens at pos.. whose rows (and every earlier one) are in the cache; k, v are the tokens' own
-// rows in float32
+// rows in float32. With rows.dpos, rows.pos is the largest position the launch may see; the results are those of a launch
+// at the position itself
 struct CacheAttn {
   CacheRows rows;
   const float *q;

@@ -383,6 +383,59 @@ static napi_value js_logits(napi_env env, napi_callback_info info) {
   return undefined(env);
 }
 
+/* what score and logprobs ask for and get, argv[0..6]: given: Int32Array, nGiven, top, logp: Float32Array, entropy:
+ * Float32Array, ids: Int32Array, logps: Float32Array, of `rows` rows */
+typedef struct probabilities {
+  int32_t n_given, top;
+  void *given, *logp, *entropy, *ids, *logps;
+} probabilities;
+static int probabilities_of(napi_env env, napi_value *argv, uint64_t rows, probabilities *p) {
+  size_t given, logp, entropy, ids, logps;
+  if (!bytes_of(env, argv[0], napi_int32_array, &p->given, &given) || !get_i32(env, argv[1], &p->n_given) ||
+      !get_i32(env, argv[2], &p->top) || !bytes_of(env, argv[3], napi_float32_array, &p->logp, &logp) ||
+      !bytes_of(env, argv[4], napi_float32_array, &p->entropy, &entropy) ||
+      !bytes_of(env, argv[5], napi_int32_array, &p->ids, &ids) ||
+      !bytes_of(env, argv[6], napi_float32_array, &p->logps, &logps))
+    return 0;
+  if (p->n_given < 0 || p->top < 0 || given < 4 * rows * (uint64_t)p->n_given || logp < 4 * rows * (uint64_t)p->n_given ||
+      entropy < 4 * rows || ids < 4 * rows * (uint64_t)p->top || logps < 4 * rows * (uint64_t)p->top) {
+    napi_throw_type_error(env, NULL, "hip_engine: an array of probabilities is shorter than its rows");
+    return 0;
+  }
+  return 1;
+}
+
+/* score(engine, tokens: Int32Array, pos, given, nGiven, top, logp, entropy, ids, logps) */
+static napi_value js_score(napi_env env, napi_callback_info info) {
+  napi_value argv[10];
+  if (!args_of(env, info, 10, argv)) return NULL;
+  he_engine *e = engine_of(env, argv[0]);
+  void *d;
+  size_t n;
+  int32_t pos;
+  probabilities p;
+  if (!e || !bytes_of(env, argv[1], napi_int32_array, &d, &n) || !get_i32(env, argv[2], &pos) ||
+      !probabilities_of(env, argv + 3, n / 4, &p))
+    return NULL;
+  const int32_t rc = he_score(e, (const int32_t *)d, (int32_t)(n / 4), pos, (const int32_t *)p.given, p.n_given, p.top,
+                              (float *)p.logp, (float *)p.entropy, (int32_t *)p.ids, (float *)p.logps);
+  if (rc) return throw_engine(env, rc);
+  return undefined(env);
+}
+
+/* logprobs(engine, given, nGiven, top, logp, entropy, ids, logps) */
+static napi_value js_logprobs(napi_env env, napi_callback_info info) {
+  napi_value argv[8];
+  if (!args_of(env, info, 8, argv)) return NULL;
+  he_engine *e = engine_of(env, argv[0]);
+  probabilities p;
+  if (!e || !probabilities_of(env, argv + 1, 1, &p)) return NULL;
+  const int32_t rc = he_logprobs(e, (const int32_t *)p.given, p.n_given, p.top, (float *)p.logp, (float *)p.entropy,
+                                 (int32_t *)p.ids, (float *)p.logps);
+  if (rc) return throw_engine(env, rc);
+  return undefined(env);
+}
+
 /* kvRead(engine, from, count, keys: Float32Array, values: Float32Array) */
 static napi_value js_kv_read(napi_env env, napi_callback_info info) {
   napi_value argv[5];
@@ -483,6 +536,8 @@ static napi_value init(napi_env env, napi_value exports) {
       {"forwardMany", NULL, js_forward_many, NULL, NULL, NULL, napi_enumerable, NULL},
       {"generateMany", NULL, js_generate_many, NULL, NULL, NULL, napi_enumerable, NULL},
       {"logits", NULL, js_logits, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"score", NULL, js_score, NULL, NULL, NULL, napi_enumerable, NULL},
+      {"logprobs", NULL, js_logprobs, NULL, NULL, NULL, napi_enumerable, NULL},
       {"kvRead", NULL, js_kv_read, NULL, NULL, NULL, napi_enumerable, NULL},
       {"checkpointRead", NULL, js_checkpoint_read, NULL, NULL, NULL, napi_enumerable, NULL},
       {"promptBlock", NULL, js_prompt_block, NULL, NULL, NULL, napi_enumerable, NULL},

@@ -133,7 +133,7 @@ int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t f
   if (count == 0) return HE_OK;
   return launched("hk_cache_read",
                   launch_cache_read(v, reinterpret_cast<float *>(keys), reinterpret_cast<float *>(values), from, count,
-                                    end / HK_CACHE_BLOCK * HK_CACHE_BLOCK, reinterpret_cast<hipStream_t>(stream)));
+                                    end / HK_CACHE_BLOCK, reinterpret_cast<hipStream_t>(stream)));
 }
 
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream) {
@@ -144,7 +144,7 @@ int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream) {
   if (pos < 0 || pos >= cache->seq_len) return failed(HE_E_ARG, "hk_cache_rewind: pos is outside the context (seq_len)");
   if (pos % HK_CACHE_BLOCK == 0) return HE_OK;
   return launched("hk_cache_rewind",
-                  launch_cache_read(v, nullptr, nullptr, pos / HK_CACHE_BLOCK * HK_CACHE_BLOCK, pos % HK_CACHE_BLOCK, pos,
+                  launch_cache_read(v, nullptr, nullptr, pos / HK_CACHE_BLOCK * HK_CACHE_BLOCK, pos % HK_CACHE_BLOCK, -1,
                                     reinterpret_cast<hipStream_t>(stream)));
 }
 

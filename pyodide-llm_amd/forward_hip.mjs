@@ -29,6 +29,8 @@ const TENSORS = ["token_embedding_table", "rms_att_weight", "wq", "wk", "wv", "w
 // include/pyodide_llm_hip.h HE_ARCH_*, HE_OUTLIERS_MOST
 const ARCHS = { llama: 0, gpt2: 1, neox: 2 };
 const OUTLIERS_MOST = 8;
+const KV_EIGHT = 8; // HE_KV_EIGHT: config.half_kv of a cache held in 8 bits
+const TOP_MOST = 32; // HK_LOGPROBS_TOP_MOST
 // include/pyodide_llm_hip.h HE_K_*
 const KINDS = ["gemv", "gemm", "attention", "norm", "elementwise", "argmax"];
 
@@ -56,14 +58,20 @@ export function weightsMemory(size, { shared = false } = {}) {
  * bytes: the keys and values of the whole context (no growth steps), the RoPE tables, one pass's activations (up to
  * 1024 prompt tokens) and the scores of up to 512 of its tokens (the attention's
  * pieces), the logits and the sampler's buffers. header: [dim, hidden, layers, heads, kvHeads, signedVocab, seqLen] as the file's. */
-export function footprint(header, size, { halfKV = false, head_dim = 0, promptBlock = PROMPT_BLOCK } = {}) {
+export function footprint(header, size, { halfKV = false, eightBitCache = false, head_dim = 0,
+  promptBlock = PROMPT_BLOCK } = {}) {
   const [dim, hidden, layers, heads, kvHeads, signedVocab, seqLen] = header;
   const vocab = Math.abs(signedVocab), headSize = head_dim || dim / heads;
   const kvDim = kvHeads * headSize, qDim = heads * headSize, wide = Math.max(dim, qDim, hidden);
   const half = halfKV && kvHeads >= heads;
   // keys by position, values by column (each column's positions rounded up to 64)
-  const keys = layers * (seqLen + Math.ceil(seqLen / 64) * 64) * kvDim * (half ? 2 : 4);
-  const chunk = Math.min(promptBlock, 1024), rows = Math.min(chunk, 512);
+  let keys = layers * (seqLen + Math.ceil(seqLen / 64) * 64) * kvDim * (half ? 2 : 4);
+  const chunk = Math.min(promptBlock, 1024), rows = eightBitCache ? 0 : Math.min(chunk, 512);
+  if (eightBitCache) {
+    // the blocks' bytes and scales, 160 float32 rows a layer; the attention's workspace: at most 4096 parts of 32 rows
+    keys = layers * (Math.ceil(seqLen / 32) * (64 * kvDim + 8 * kvHeads) + 2 * 4 * 160 * kvDim) +
+      4096 * 32 * 4 * (headSize + 4);
+  }
   const frames = chunk * (4 * (dim + Math.max(dim, qDim) + qDim + 2 * kvDim + 2 * hidden) + wide + wide / 8) +
     rows * 4 * heads * (seqLen + Math.floor(seqLen / 64) + 1);
   // the logits, the sampler's probabilities and indices; 1 MiB for the small buffers and the regions' alignment
@@ -90,8 +98,9 @@ function floats(bytes, count, name) {
 
 /** The engine's config and tensor places from a plan (public/llama2_numpy.py:1261-1270): the llama form (Qwen2's
  * biases and Qwen3's head norms where the plan has those tensors), gpt2 and neox (public/forward.js:636). The forms the
- * engine does not run are refused by name, as public/forward.js refuses what its kernels cannot take. */
-export function planToConfig(plan, { relaxedKernels = true, halfKeys } = {}) {
+ * engine does not run are refused by name, as public/forward.js refuses what its kernels cannot take. eightBitCache:
+ * keys and values held in 8 bits (the engine's own form: a quarter of float32's bytes, longer contexts). */
+export function planToConfig(plan, { relaxedKernels = true, halfKeys, eightBitCache = false } = {}) {
   const arch = or(plan.arch, "llama");
   if (!(arch in ARCHS)) throw new Error(`the HIP engine runs the llama, gpt2 and neox forms, not ${arch}`);
   if (!plan.int8) throw new Error("the HIP engine multiplies int8/int6 matrices only (plan.int8)");
@@ -116,7 +125,7 @@ export function planToConfig(plan, { relaxedKernels = true, halfKeys } = {}) {
     // public/forward.js:650-652: bias 64 where the plan and the kernels allow relaxed SIMD
     relaxed: plan.relaxed !== false && relaxedKernels ? 1 : 0,
     // public/forward.js:762
-    half_kv: plan.half_kv && or(halfKeys, kvHeads >= heads) ? 1 : 0,
+    half_kv: eightBitCache ? KV_EIGHT : plan.half_kv && or(halfKeys, kvHeads >= heads) ? 1 : 0,
     rms_norm_eps: or(plan.rms_norm_eps, 1e-5),
     arch: ARCHS[arch], rotary: arch === "neox" ? rotary : 0,
     parallel_residual: layerNorm && plan.parallel_residual ? 1 : 0,
@@ -127,6 +136,12 @@ export function planToConfig(plan, { relaxedKernels = true, halfKeys } = {}) {
     return t ? [Number(t.offset), Number(t.scales || 0)] : [0, 0];
   });
   return { config, tensors };
+}
+
+function probabilities(rows, each, top) {
+  if (!(Number.isInteger(top) && top >= 0 && top <= TOP_MOST)) throw new Error(`top is in 0..${TOP_MOST}`);
+  return { logp: new Float32Array(rows * each), entropy: new Float32Array(rows), ids: new Int32Array(rows * top),
+    logps: new Float32Array(rows * top) };
 }
 
 function engineObject(handle, config) {
@@ -208,6 +223,28 @@ function engineObject(handle, config) {
       if (!haveLogits) addon.logits(handle, logits);
       return logits;
     },
+    /** tokens at pos, pos + 1, ... as forwardMany() runs them, and for each the log probabilities of what follows it: of
+     * the tokens given (given.length / tokens.length a token; by default the text's own next tokens, the last one's -1:
+     * NaN), the entropy and the top most probable ones: {logp, entropy, ids, logps}, a row a token */
+    score(tokens, pos, given, top = 0) {
+      const list = Int32Array.from(fromJs(tokens)), n = list.length;
+      const asked = given === undefined || given === null ? Int32Array.from([...list.subarray(1), -1])
+        : Int32Array.from(fromJs(given));
+      if (!n || asked.length % n) throw new Error("score takes at least one token, and as many tokens given for each");
+      const each = asked.length / n, got = probabilities(n, each, top);
+      for (let at = 0; at < n; at += promptBlock) {
+        const to = Math.min(n, at + promptBlock), part = (a, k) => a.subarray(at * k, to * k);
+        addon.score(handle, list.subarray(at, to), pos + at, part(asked, each), each, top, part(got.logp, each),
+          part(got.entropy, 1), part(got.ids, top), part(got.logps, top));
+      }
+      return got;
+    },
+    /** the log probabilities under logits(): of the tokens given, the entropy, the top most probable ones */
+    logprobs(given = [], top = 0) {
+      const asked = Int32Array.from(fromJs(given)), got = probabilities(1, asked.length, top);
+      addon.logprobs(handle, asked, asked.length, top, got.logp, got.entropy, got.ids, got.logps);
+      return got;
+    },
     /** the cache at positions from .. from + count - 1 as float32 [layers][count][kvDim] each
      * (public/forward.js:1939-1953) */
     keysAndValues(from, count) {
@@ -244,9 +281,10 @@ function ropeOf(plan, config) {
 }
 
 /** createForward (public/forward.js:626): the engine for a plan over a checkpoint of size bytes at base of memory */
-export function createForward({ memory, base, size, kernels, plan, halfKeys, promptBlock = PROMPT_BLOCK }) {
+export function createForward({ memory, base, size, kernels, plan, halfKeys, eightBitCache, promptBlock = PROMPT_BLOCK }) {
   plan = fromJs(plan);
-  const { config, tensors } = planToConfig(plan, { relaxedKernels: !kernels || Boolean(kernels.relaxed), halfKeys });
+  const { config, tensors } = planToConfig(plan,
+    { relaxedKernels: !kernels || Boolean(kernels.relaxed), halfKeys, eightBitCache });
   const [cos, sin] = ropeOf(plan, config);
   const handle = addon.open(config, tensors, memory.buffer, base, size, cos, sin, promptBlock);
   return engineObject(handle, config);
@@ -255,9 +293,9 @@ export function createForward({ memory, base, size, kernels, plan, halfKeys, pro
 /** The engine over a checkpoint made on the device from a seed (weights N(0, 0.02) quantized by the reference's rules,
  * norm weights 1.0) instead of uploaded: for measurements of models too large to make on the host. plan.tensors must
  * place every tensor as the file would (public/llama2_numpy.py:778-795, external_tensors). */
-export function syntheticForward({ plan, size, seed = 0, halfKeys, promptBlock = PROMPT_BLOCK }) {
+export function syntheticForward({ plan, size, seed = 0, halfKeys, eightBitCache, promptBlock = PROMPT_BLOCK }) {
   plan = fromJs(plan);
-  const { config, tensors } = planToConfig(plan, { halfKeys });
+  const { config, tensors } = planToConfig(plan, { halfKeys, eightBitCache });
   const [cos, sin] = ropeOf(plan, config);
   const handle = addon.openSynthetic(config, tensors, size, BigInt(seed), cos, sin, promptBlock);
   return engineObject(handle, config);
@@ -265,12 +303,12 @@ export function syntheticForward({ plan, size, seed = 0, halfKeys, promptBlock =
 
 /** external (public/forward.js:571-590): what Llama(external=) takes: the checkpoint's size, read() for the bytes
  * Python looks at itself, and start(plan), which makes the engine */
-export function external({ memory, base, size, kernels, halfKeys, promptBlock }) {
+export function external({ memory, base, size, kernels, halfKeys, eightBitCache, promptBlock }) {
   const outside = {
     size,
     read: (offset, length) => new Uint8Array(memory.buffer, base + offset, length).slice(),
     start: (plan) => {
-      outside.engine = createForward({ memory, base, size, kernels, plan, halfKeys, promptBlock });
+      outside.engine = createForward({ memory, base, size, kernels, plan, halfKeys, eightBitCache, promptBlock });
       return outside.engine;
     },
   };

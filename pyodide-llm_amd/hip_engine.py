@@ -51,6 +51,8 @@ class HkCache(ctypes.Structure):
 
 
 CACHE_BLOCK, CACHE_RECENT = 32, 128  # HK_CACHE_BLOCK, HK_CACHE_RECENT
+KV_EIGHT = 8  # HE_KV_EIGHT: HeConfig.half_kv of a cache held in 8 bits
+TOP_MOST = 32  # HK_LOGPROBS_TOP_MOST
 
 
 def cache_shapes(n_kv_heads, head_size, seq_len):
@@ -109,6 +111,8 @@ def library():
             "he_generate_many": (I32, [P, I32, I32, P, I32, I32, I32, F, F, F, P, I32, P, I32, P, P]),
             "he_logits": (I32, [P, P]),
             "he_kv_read": (I32, [P, I32, I32, P, P]),
+            "he_score": (I32, [P, P, I32, I32, P, I32, I32, P, P, P, P]),
+            "he_logprobs": (I32, [P, P, I32, I32, P, P, P, P]),
             "he_checkpoint_read": (I32, [P, U64, U64, P]),
             "he_prompt_block": (I32, [P]),
             "he_device_bytes": (U64, [P]),
@@ -155,11 +159,12 @@ def _ptr(a):
     return ctypes.c_void_p(a.ctypes.data) if a is not None else None
 
 
-def plan_to_config(plan, half_keys=None):
+def plan_to_config(plan, half_keys=None, eight_bit_cache=False):
     """he_config and he_tensor[] from a plan dict (public/llama2_numpy.py:1261-1270): the llama form (with Qwen2's
     biases and Qwen3's head norms where the tensors are there), gpt2 and neox (public/forward.js:636); forms the engine
     does not take are refused by name, as public/forward.js refuses what its kernels cannot run. Keys and values are
-    float16 where the plan allows it and every head has its own (or half_keys says so): public/forward.js:762"""
+    float16 where the plan allows it and every head has its own (or half_keys says so): public/forward.js:762; with
+    eight_bit_cache they are held in 8 bits (HE_KV_EIGHT)"""
     arch = plan.get("arch", "llama")
     if arch not in ARCHS:
         raise HipError(f"the engine runs the llama, gpt2 and neox forms, not {arch}")
@@ -183,7 +188,7 @@ def plan_to_config(plan, half_keys=None):
                n_kv_heads=plan["n_kv_heads"], head_size=plan["head_size"], vocab_size=plan["vocab_size"],
                seq_len=plan["seq_len"], shared_classifier=int(bool(plan["shared_classifier"])), six=int(six),
                qkv_bias=int("bq" in tensors), relaxed=int(bool(plan.get("relaxed", True))),
-               half_kv=int(bool(plan.get("half_kv", False)) and (
+               half_kv=KV_EIGHT if eight_bit_cache else int(bool(plan.get("half_kv", False)) and (
                    bool(half_keys) if half_keys is not None else plan["n_kv_heads"] >= plan["n_heads"])),
                rms_norm_eps=float(plan.get("rms_norm_eps", 1e-5)), arch=ARCHS[arch],
                rotary=rotary if arch == "neox" else 0,
@@ -273,6 +278,42 @@ class Engine:
     def logits(self):
         check(library().he_logits(self._h, _ptr(self._logits)))
         return self._logits
+
+    def _probabilities(self, rows, given, top, call):
+        """he_score's and he_logprobs' arrays: {"logp": [rows][n_given], "entropy": [rows], "ids": [rows][top], "logps":
+        [rows][top]} of the tokens given [rows][n_given] (or [rows], or None)"""
+        asked = None if given is None else np.ascontiguousarray(given, dtype=np.int32).reshape(rows, -1)
+        n = 0 if asked is None else asked.shape[1]
+        if not 0 <= int(top) <= TOP_MOST:
+            raise HipError(f"top is in 0..{TOP_MOST}")
+        logp, entropy = np.zeros((rows, n), dtype=np.float32), np.zeros(rows, dtype=np.float32)
+        ids, logps = np.zeros((rows, int(top)), dtype=np.int32), np.zeros((rows, int(top)), dtype=np.float32)
+        call(_ptr(asked) if n else None, n, int(top), _ptr(logp) if n else None, _ptr(entropy),
+             _ptr(ids) if top else None, _ptr(logps) if top else None)
+        return {"logp": logp, "entropy": entropy, "ids": ids, "logps": logps}
+
+    def score(self, tokens, pos, given=None, top=0):
+        """tokens at pos, pos + 1, ... as forwardMany runs them (any number), and for each the log probabilities of what
+        follows it: of the tokens given (one a token, or a row of them; a text's own next tokens by default, the last
+        token's -1: NaN), the entropy and the top most probable ones: {"logp", "entropy", "ids", "logps"}"""
+        ids = np.ascontiguousarray(np.asarray(list(tokens), dtype=np.int32))
+        if not ids.size:
+            raise HipError("no tokens")
+        if given is None:
+            given = np.append(ids[1:], -1)
+        asked = np.asarray(given, dtype=np.int32).reshape(ids.size, -1)
+        parts, block = [], self.promptBlock
+        for at in range(0, ids.size, block):
+            piece = np.ascontiguousarray(ids[at:at + block])
+            parts.append(self._probabilities(piece.size, asked[at:at + block], top, lambda g, n, *rest: check(
+                library().he_score(self._h, _ptr(piece), int(piece.size), int(pos) + at, g, n, *rest))))
+        return {name: np.concatenate([p[name] for p in parts]) for name in parts[0]}
+
+    def logprobs(self, given=None, top=0):
+        """the log probabilities under logits(): of the tokens given, the entropy, the top most probable ones"""
+        got = self._probabilities(1, given if given is None else np.atleast_1d(given), top, lambda *a: check(
+            library().he_logprobs(self._h, *a)))
+        return {name: x[0] for name, x in got.items()}
 
     def keysAndValues(self, start, count):
         c = self.config
@@ -436,9 +477,9 @@ def rope_tables(seq_len, head_size, theta, rotary=0):
     return cos, sin
 
 
-def start(plan, checkpoint, max_block=2048):
+def start(plan, checkpoint, max_block=2048, eight_bit_cache=False):
     """public/forward.js:571-590 start(plan) over checkpoint bytes (any buffer) that hold the file"""
-    c, t = plan_to_config(plan)
+    c, t = plan_to_config(plan, eight_bit_cache=eight_bit_cache)
     buf = np.frombuffer(checkpoint, dtype=np.uint8)
     derived = plan.get("derived") or {}
     if "freq_cis_real" not in derived:
@@ -477,19 +518,20 @@ def open_synthetic(cfg, tensors, size, seed, rope_cos, rope_sin, max_block=2048)
 class External:
     """public/forward.js:571-590 external(): the checkpoint's bytes, read(offset, length), start(plan)"""
 
-    def __init__(self, checkpoint, max_block=2048):
+    def __init__(self, checkpoint, max_block=2048, eight_bit_cache=False):
         self._bytes = checkpoint
         self.size = len(checkpoint)
         self.max_block = max_block
+        self.eight_bit_cache = eight_bit_cache
         self.engine = None
 
     def read(self, offset, length):
         return bytes(memoryview(self._bytes)[offset:offset + length])
 
     def start(self, plan):
-        self.engine = start(plan, self._bytes, self.max_block)
+        self.engine = start(plan, self._bytes, self.max_block, self.eight_bit_cache)
         return self.engine
 
 
-def external(checkpoint, max_block=2048):
-    return External(checkpoint, max_block)
+def external(checkpoint, max_block=2048, eight_bit_cache=False):
+    return External(checkpoint, max_block, eight_bit_cache)

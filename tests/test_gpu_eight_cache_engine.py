@@ -1,0 +1,339 @@
+"""The engine over the cache held in 8 bits (half_kv = HE_KV_EIGHT), and its log probabilities (he_score, he_logprobs)."""
+import ctypes
+import json
+import os
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+import cache_lib as cl
+import oracle_lib as ol
+from paths import REPO, package
+from plans import plan_of
+from tiny import sharp_checkpoint
+
+pytestmark = pytest.mark.gpu
+
+FIELDS = dict(dim=64, hidden_dim=128, n_layers=2, n_heads=4, n_kv_heads=2, head_size=16, vocab_size=320, seq_len=300,
+              shared_classifier=1)
+FORMS = {
+    "llama": FIELDS,
+    "qwen int6": dict(FIELDS, n_heads=2, n_kv_heads=1, head_size=32, six=1, qkv_bias=1, shared_classifier=0),
+    "qwen3": dict(FIELDS, qk_norm=1),
+    "gpt2": dict(FIELDS, n_kv_heads=4, arch=1, relaxed=0),
+    "neox": dict(FIELDS, n_kv_heads=4, arch=2, rotary=8, parallel_residual=1),
+    "wide heads": dict(FIELDS, dim=256, n_heads=2, n_kv_heads=1, head_size=128),
+}
+
+
+def opened(fields, kv, block=64, seed=7):
+    cfg = ol.config(**{**fields, "half_kv": kv})
+    tensors, size = ol.places(cfg)
+    ck = ol.synth_checkpoint(cfg, tensors, size, seed=seed)
+    ol.vary_vectors(cfg, tensors, ck, seed=13)
+    ol.sharpen(cfg, tensors, ck, 5.0)
+    cos, sin = ol.rope_tables(cfg.seq_len, cfg.head_size, 10000.0)
+    return package().open_config(cfg, tensors, ck, cos, sin, max_block=block), cfg, tensors, ck, cos, sin
+
+
+def tokens(n, vocab=320, seed=3):
+    return [1] + [int(t) for t in np.random.default_rng(seed).integers(3, vocab, size=n - 1)]
+
+
+def rows_of(kv, cfg, count):
+    return np.stack([kv[k].reshape(cfg.n_layers, count, cfg.n_kv_heads, cfg.head_size) for k in ("keys", "values")])
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("count", [31, 32, 100, 129])
+def test_the_first_layers_cache_is_the_float32_caches_in_8_bits(form, count):
+    """the first layer's keys and values do not depend on attention: the float32 cache's rows, quantized"""
+    full, cfg, *_ = opened(FORMS[form], 0)
+    eight = opened(FORMS[form], 8)[0]
+    ids = tokens(count)
+    for eng in (full, eight):
+        eng.forwardMany(ids, 0)
+    want = rows_of(full.keysAndValues(0, count), cfg, count)[:, 0]
+    got = rows_of(eight.keysAndValues(0, count), cfg, count)[:, 0]
+    model = cl.Model(cfg.n_kv_heads, cfg.head_size, cfg.seq_len)
+    model.append(want[0], want[1], 0)
+    np.testing.assert_array_equal(got, model.read(0, count, count).astype(np.float32))
+    assert eight.memoryBytes() < full.memoryBytes() + (4 << 20)
+
+
+class Forward:
+    """the llama form's forward pass by the oracle's kernels, one token at a time, with the attention over the NumPy cache
+    in float64"""
+
+    def __init__(self, cfg, tensors, ck, cos, sin):
+        self.c, self.t, self.ck, self.cos, self.sin = cfg, tensors, ck, cos, sin
+        self.caches = [cl.Model(cfg.n_kv_heads, cfg.head_size, cfg.seq_len) for _ in range(cfg.n_layers)]
+        self.bias = 64 if cfg.relaxed else 0
+
+    def matrix(self, name, layer, rows, k):
+        t = self.t[package().T[name]]
+        at, sa = t.offset + layer * rows * k, t.scales + layer * rows * (k // 32) * 4
+        return (self.ck[at:at + rows * k].view(np.int8).reshape(rows, k),
+                np.frombuffer(self.ck[sa:sa + rows * (k // 32) * 4].tobytes(), dtype=np.float32).reshape(rows, -1))
+
+    def vector(self, name, layer, n):
+        at = self.t[package().T[name]].offset + 4 * layer * n
+        return np.frombuffer(self.ck[at:at + 4 * n].tobytes(), dtype=np.float32)
+
+    def times(self, x, name, layer, rows):
+        w, ws = self.matrix(name, layer, rows, x.size)
+        return ol.matmul(*ol.quantize_x(x, self.bias), w, ws, rows, x.size, self.bias, 0)[0]
+
+    def rope(self, x, pos):
+        p = x.reshape(-1, self.c.head_size // 2, 2)
+        out = np.empty_like(p)
+        out[..., 0] = p[..., 0] * self.cos[pos] - p[..., 1] * self.sin[pos]
+        out[..., 1] = p[..., 0] * self.sin[pos] + p[..., 1] * self.cos[pos]
+        return out.reshape(-1)
+
+    def step(self, token, pos):
+        c = self.c
+        qd, kd = c.n_heads * c.head_size, c.n_kv_heads * c.head_size
+        e, es = self.matrix("token_embedding_table", 0, c.vocab_size, c.dim)
+        x = (e[token].reshape(-1, 32).astype(np.float32) * es[token][:, None]).reshape(-1)
+        for l in range(c.n_layers):
+            h = ol.rmsnorm(x, self.vector("rms_att_weight", l, c.dim), c.rms_norm_eps)
+            q, k, v = self.times(h, "wq", l, qd), self.times(h, "wk", l, kd), self.times(h, "wv", l, kd)
+            q, k = self.rope(q, pos), self.rope(k, pos)
+            self.caches[l].append(k[None], v[None], pos)
+            out, _ = self.caches[l].attention(q[None], pos, c.n_heads)
+            x = x + self.times(out.reshape(-1).astype(np.float32), "wo", l, c.dim)
+            h = ol.rmsnorm(x, self.vector("rms_ffn_weight", l, c.dim), c.rms_norm_eps)
+            a, b = self.times(h, "w1", l, c.hidden_dim), self.times(h, "w3", l, c.hidden_dim)
+            a64 = a.astype(np.float64)
+            x = x + self.times((a64 / (1 + np.exp(-a64)) * b).astype(np.float32), "w2", l, c.dim)
+        h = ol.rmsnorm(x, self.vector("rms_final_weight", 0, c.dim), c.rms_norm_eps)
+        return self.times(h, "token_embedding_table", 0, c.vocab_size)
+
+
+def test_logits_follow_the_forward_pass_over_the_quantized_cache():
+    """against the oracle's kernels with the attention over the NumPy cache: what is left are float32 roundings that now and
+    then move an activation to the next of its 63 steps, where the cache moves every key and value: less than a quarter of
+    what the cache itself changes, and nothing like it in the first block, where no position is in 8 bits"""
+    eight, cfg, tensors, ck, cos, sin = opened(FIELDS, 8)
+    full = opened(FIELDS, 0)[0]
+    ref, ids = Forward(cfg, tensors, ck, cos, sin), tokens(110)
+    apart, own = [], []
+    for i, t in enumerate(ids):
+        want = ref.step(t, i)
+        for eng in (eight, full):
+            eng.forward(t, i)
+        own.append(np.sqrt(np.mean((eight.logits() - want) ** 2)) / want.std())
+        apart.append(np.sqrt(np.mean((full.logits() - want) ** 2)) / want.std())
+    own, apart = np.array(own), np.array(apart)
+    assert np.mean(own[64:]) < np.mean(apart[64:]) / 4, (own, apart)
+    assert np.mean(own[:32]) < np.mean(apart[64:]) / 4
+    prompt = opened(FIELDS, 8)[0]
+    prompt.forwardMany(ids[:-1], 0)
+    prompt.forward(ids[-1], 109)
+    assert np.sqrt(np.mean((prompt.logits() - want) ** 2)) / want.std() < np.mean(apart[64:]) / 2
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+def test_replayed_steps_equal_eager_ones(form, monkeypatch):
+    """the same bits from replayed steps, from eager ones, and from one token at a time through forward()"""
+    got = []
+    for graph in ("1", "0"):
+        monkeypatch.setenv("PYODIDE_LLM_HIP_GRAPH", graph)
+        eng = opened(FORMS[form], 8)[0]
+        eng.forwardMany(tokens(40)[:-1], 0)
+        ids, token, pos = [], tokens(40)[-1], 39
+        while len(ids) < 150:
+            ids += eng.generateMany(token, pos, [], 0, min(50, 150 - len(ids)), 0.0, 0.9, 1.0, [], [])
+            token, pos = ids[-1], 39 + len(ids)
+        got.append((ids, np.array(eng.logits()), eng.keysAndValues(0, pos)))
+    assert got[0][0] == got[1][0]
+    np.testing.assert_array_equal(got[0][1], got[1][1])
+    for name in ("keys", "values"):
+        np.testing.assert_array_equal(got[0][2][name], got[1][2][name])
+    eng = opened(FORMS[form], 8)[0]
+    eng.forwardMany(tokens(40)[:-1], 0)
+    for i, t in enumerate([tokens(40)[-1]] + got[0][0][:-1]):
+        eng.forward(t, 39 + i)
+        assert int(np.argmax(eng.logits())) == got[0][0][i]
+    np.testing.assert_array_equal(eng.logits(), got[0][1])
+
+
+def test_steps_after_a_stopped_round_equal_steps_without_one(monkeypatch):
+    """a stop token ends a round whose later replays have written rows past it: the positions taken again hold what they
+    would have held"""
+    ids, randoms = None, [float(r) for r in np.random.default_rng(2).random(40)]
+    got = []
+    for stop in (False, True):
+        eng = opened(FIELDS, 8)[0]
+        eng.forwardMany(tokens(20)[:-1], 0)
+        if not stop:
+            ids = eng.generateMany(tokens(20)[-1], 19, tokens(20), 20, 40, 1.0, 1.0, 1.0, randoms, [])
+        else:
+            at = max(i for i in range(1, 30) if ids[i] not in ids[:i])
+            first = eng.generateMany(tokens(20)[-1], 19, tokens(20), 20, 40, 1.0, 1.0, 1.0, randoms, [ids[at]])
+            assert first == ids[:at + 1]
+            pos = 19 + len(first)
+            kv = eng.keysAndValues(0, pos)
+            rest = eng.generateMany(first[-1], pos, tokens(20) + first, pos, 40 - len(first), 1.0, 1.0, 1.0,
+                                    randoms[len(first):], [])
+            assert first + rest == ids
+            plain = opened(FIELDS, 8)[0]
+            plain.forwardMany(tokens(20)[:-1], 0)
+            for i, t in enumerate([tokens(20)[-1]] + first[:-1]):
+                plain.forward(t, 19 + i)
+            want = plain.keysAndValues(0, pos)
+            for name in kv:
+                np.testing.assert_array_equal(kv[name], want[name])
+        got.append((np.array(eng.logits()), eng.keysAndValues(0, 59)))
+    np.testing.assert_array_equal(got[0][0], got[1][0])
+    for name in ("keys", "values"):
+        np.testing.assert_array_equal(got[0][1][name], got[1][1][name])
+
+
+def test_a_turn_taken_again():
+    """back to an earlier position: within the latest ones the same bits as a conversation that never went on; further back
+    the block's earlier positions by their 8-bit values, finite and close"""
+    first, other = tokens(200), tokens(200, seed=9)
+    eng = opened(FIELDS, 8)[0]
+    eng.forwardMany(first[:150], 0)
+    for back, exact in ((100, True), (40, False)):
+        eng.forwardMany(other[back:back + 30], back)
+        eng.forward(other[back + 30], back + 30)
+        fresh = opened(FIELDS, 8)[0]
+        fresh.forwardMany((first[:100] if back == 100 else first[:40])[:back], 0)
+        fresh.forwardMany(other[back:back + 30], back)
+        fresh.forward(other[back + 30], back + 30)
+        a, b = np.array(eng.logits()), np.array(fresh.logits())
+        if exact:
+            assert np.max(np.abs(a - b)) <= 0.25 * b.std()
+            ka, kb = (rows_of(x.keysAndValues(0, 131), eng.config, 131)[:, 0] for x in (eng, fresh))
+            np.testing.assert_array_equal(ka, kb)
+        else:
+            assert np.isfinite(a).all() and np.sqrt(np.mean((a - b) ** 2)) < b.std()
+
+
+def test_a_context_past_the_float32_caches_limit():
+    """a context that the ordered attention refuses: opened, filled across its end, replayed"""
+    fields = dict(FIELDS, seq_len=45000)
+    with pytest.raises(package().HipError):
+        opened(fields, 0)
+    eng = opened(fields, 8, block=1024)[0]
+    ids = tokens(44990)
+    for at in range(0, 44989, 1024):
+        eng.forwardMany(ids[at:min(44989, at + 1024)], at)
+    got = eng.generateMany(ids[-1], 44989, [], 0, 11, 0.0, 0.9, 1.0, [], [])
+    assert len(got) == 11 and np.isfinite(eng.logits()).all()
+    with pytest.raises(package().HipError):
+        eng.forward(1, 45000)
+
+
+@pytest.mark.parametrize("kv", [0, 1, 8])
+@pytest.mark.parametrize("form", ["llama", "gpt2", "qwen int6"])
+def test_scores_are_those_of_the_steps_logits(form, kv):
+    """he_score's rows against the log softmax in float64 of the logits that forward() gives each token; float32 and float16
+    caches give each token's logits to the bit however it is run, and a log probability is then off by 2^-17 at most (its
+    sums) and its own rounding. Over 8 bits a token's attention is summed in another order alone or in a prompt: its rows
+    are held to those of the same pass"""
+    block = 64
+    ids = tokens(150)
+    eng, cfg = opened(FORMS[form], kv, block)[:2]
+    got = eng.score(ids, 0, top=5)
+    one = opened(FORMS[form], kv, block)[0]
+    worst = 0.0
+    for i, t in enumerate(ids):
+        one.forward(t, i)
+        x = one.logits().astype(np.float64)
+        lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+        if i + 1 < len(ids):
+            worst = max(worst, abs(got["logp"][i, 0] - lp[ids[i + 1]]))
+        if kv != 8:
+            assert abs(got["entropy"][i] + (np.exp(lp) * lp).sum()) < 1e-4
+            np.testing.assert_array_equal(got["ids"][i], np.argsort(-x, kind="stable")[:5])
+            np.testing.assert_allclose(got["logps"][i], lp[got["ids"][i]], atol=2.0 ** -16, rtol=0)
+    assert worst <= (2.0 ** -16 if kv != 8 else 0.5), worst
+    assert np.isnan(got["logp"][-1, 0])
+    assert np.isfinite(got["logps"]).all() and (np.diff(got["logps"], axis=1) <= 0).all()
+
+
+def test_scores_with_outlier_channels():
+    fields = dict(FIELDS, outliers=[3, 17, 40])
+    eng, one = opened(fields, 0)[0], opened(fields, 0)[0]
+    ids = tokens(20)
+    got = eng.score(ids, 0, given=[[5, 6]] * 20)
+    for i, t in enumerate(ids):
+        one.forward(t, i)
+        x = one.logits().astype(np.float64)
+        lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+        np.testing.assert_allclose(got["logp"][i], lp[[5, 6]], atol=2.0 ** -16, rtol=0)
+
+
+def test_log_probabilities_of_the_last_step():
+    eng = opened(FIELDS, 0)[0]
+    with pytest.raises(package().HipError):
+        eng.logprobs(given=[3])  # no step with logits has run
+    eng.forwardMany(tokens(10), 0)
+    ids = eng.generateMany(5, 10, tokens(10) + [5], 11, 7, 0.0, 0.9, 1.3, [], [])
+    x = eng.logits().astype(np.float64)
+    lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+    got = eng.logprobs(given=[ids[-1], 0], top=32)
+    np.testing.assert_allclose(got["logp"], lp[[ids[-1], 0]], atol=2.0 ** -16, rtol=0)
+    assert got["ids"][0] == ids[-1]
+    np.testing.assert_array_equal(got["ids"], np.argsort(-x, kind="stable")[:32])
+    assert abs(got["entropy"] + (np.exp(lp) * lp).sum()) < 1e-4
+    assert eng.logprobs()["logp"].size == 0
+
+
+def test_scores_that_are_refused():
+    pk = package()
+    eng, cfg = opened(FIELDS, 8)[:2]
+    lib, f = pk.library(), np.zeros(64, dtype=np.float32)
+    i = np.array([5, 6], dtype=np.int32)
+    ip, fp = ctypes.c_void_p(i.ctypes.data), ctypes.c_void_p(f.ctypes.data)
+    E = pk.hip_engine
+    for args, code in (((None, 2, 0, ip, 1, 0, fp, fp, None, None), E.HE_E_ARG),
+                       ((ip, 0, 0, ip, 1, 0, fp, fp, None, None), E.HE_E_ARG),
+                       ((ip, 65, 0, ip, 1, 0, fp, fp, None, None), E.HE_E_ARG),
+                       ((ip, 2, 299, ip, 1, 0, fp, fp, None, None), E.HE_E_STATE),
+                       ((ip, 2, -1, ip, 1, 0, fp, fp, None, None), E.HE_E_STATE),
+                       ((ip, 2, 0, None, 1, 0, fp, fp, None, None), E.HE_E_ARG),
+                       ((ip, 2, 0, ip, -1, 0, fp, fp, None, None), E.HE_E_ARG),
+                       ((ip, 2, 0, ip, 1, 33, fp, fp, ip, fp), E.HE_E_ARG),
+                       ((ip, 2, 0, ip, 1, 2, fp, fp, None, fp), E.HE_E_ARG),
+                       ((ip, 2, 0, None, 0, 0, None, None, None, None), E.HE_E_ARG)):
+        assert lib.he_score(eng._h, *args) == code
+    i[0] = 320
+    assert lib.he_score(eng._h, ip, 2, 0, ip, 1, 0, fp, fp, None, None) == E.HE_E_ARG
+    assert lib.he_score(None, ip, 2, 0, ip, 1, 0, fp, fp, None, None) == E.HE_E_ARG
+    assert lib.he_logprobs(None, ip, 1, 0, fp, fp, None, None) == E.HE_E_ARG
+
+
+@pytest.mark.skipif(shutil.which("node") is None, reason="no node here")
+def test_the_node_host_gives_the_same(tmp_path):
+    """forward_hip.mjs with eightBitCache, score() and logprobs(): the Python host's numbers to the bit"""
+    eng, cfg, tensors, ck, cos, sin = opened(FIELDS, 8)
+    ids = tokens(90)
+    ck.tofile(tmp_path / "checkpoint.bin")
+    np.asarray(cos, np.float32).tofile(tmp_path / "cos.bin")
+    np.asarray(sin, np.float32).tofile(tmp_path / "sin.bin")
+    job = {"size": int(ck.size), "plan": {**plan_of(cfg, tensors), "half_kv": True}, "tokens": ids, "steps": 20}
+    (tmp_path / "job.json").write_text(json.dumps(job))
+    proc = subprocess.run(["node", os.path.join(REPO, "tests", "node", "score_engine.mjs"), str(tmp_path / "job.json")],
+                          stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=120)
+    assert proc.returncode == 0, proc.stderr[-3000:]
+    out = json.loads(proc.stdout.strip().splitlines()[-1])
+    got = eng.score(ids, 0, top=3)
+    steps = eng.generateMany(7, 90, [], 0, 16, 0.0, 0.9, 1.0, [], [])
+    last = eng.logprobs(given=[steps[-1], 3], top=2)
+    assert out["steps"] == steps
+    for name in ("entropy", "ids", "logps"):
+        np.testing.assert_array_equal(np.array(out["score"][name], dtype=np.float32),
+                                      got[name].reshape(-1).astype(np.float32))
+    np.testing.assert_array_equal(np.array(out["score"]["logp"][:-1], dtype=np.float32), got["logp"][:-1, 0])
+    assert out["score"]["logp"][-1] is None  # (NaN)
+    np.testing.assert_array_equal(np.array(out["last"]["logp"], dtype=np.float32), last["logp"])
+    np.testing.assert_array_equal(out["last"]["ids"], last["ids"])
+    assert out["threw"] == [True] * 4
+    assert out["footprint"] + ck.size >= out["memoryBytes"]
