@@ -13,8 +13,8 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LOWEST = -3.402823466e38f;
-constexpr int THREADS = 256, QUADS = 4, BATCH = 4 * QUADS;  // logits a thread takes at once
-constexpr int LIST = 1024;  // candidates a workgroup holds: a batch adds at most 16 x 32 behind its threshold
+constexpr int THREADS = 256, WAVES = THREADS / 64, QUADS = 4, BATCH = 4 * QUADS;  // logits a thread takes at once
+constexpr int HELD = 256;  // candidates a wave holds
 
 // What a workgroup's part of a row comes to. A logit's key orders logits by value, the lower index first among equals; 0:
 // none (a logit of minus infinity has no key).
@@ -46,89 +46,84 @@ __device__ __forceinline__ void join(T &m, T &z, T &h, T m2, T z2, T h2) {
 }
 
 struct Shared {
-  uint64_t list[LIST];
-  uint64_t tops[THREADS];
-  uint64_t threshold;
-  int count;
-  Part parts[THREADS / 64];
+  uint64_t held[WAVES][HELD];  // the waves' candidates
+  uint64_t list[WAVES * HELD];
+  uint64_t best[WAVES];
+  uint32_t bars[WAVES];
+  int counts[WAVES], count;
+  Part parts[WAVES];
 };
 
-// the k-th largest of the workgroup's threads' keys (k <= THREADS): no fewer than k keys of the workgroup reach it. By
-// counting, for each key, those before it (equal ones, which are 0, by thread).
-__device__ __forceinline__ uint64_t kth_of_threads(Shared &s, uint64_t key, int k) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-  s.tops[tid] = key;
-  __syncthreads();
-  int before = 0;
-  for (int i = 0; i < THREADS; i += 2) {
-    const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&s.tops[i]);
-    before += (o.x > key || (o.x == key && i < tid)) + (o.y > key || (o.y == key && i + 1 < tid));
+__device__ __forceinline__ uint32_t ordered_of(float x) { return (uint32_t)(key_of(x, 0) >> 32); }
+
+// a value that at least k (at most 64) of the wave's lanes reach, the largest of 20 leading bits (in ordered_of's bits; 0
+// where fewer lanes hold one): a bit at a time, by counting lanes
+__device__ __forceinline__ uint32_t reached_by(uint32_t mine, int k) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 12; --bit) {
+    const uint32_t more = t | 1u << bit;
+    if (__popcll(__ballot(mine >= more)) >= k) t = more;
   }
-  if (before == k - 1) s.threshold = key;
-  __syncthreads();
-  return s.threshold;
+  return t;
 }
 
-// the k largest keys of the list, in order, to its front; the list then holds at most k
-__device__ __forceinline__ void tighten(Shared &s, int k) {
-  const int tid = threadIdx.x, n = s.count;
-  uint64_t mine[LIST / THREADS];
-  int place[LIST / THREADS];
+__device__ __forceinline__ uint64_t wave_most(uint64_t x) {
 #pragma unroll
-  for (int j = 0; j < LIST / THREADS; ++j) {
-    const int i = tid + THREADS * j;
-    mine[j] = i < n ? s.list[i] : 0;
+  for (int o = 32; o; o >>= 1) {
+    const uint64_t y = __shfl_xor(x, o);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+// the k largest of a wave's n candidates to the front, in order, one at a time (where they pass HELD: rows of ties)
+__device__ __forceinline__ int wave_tighten(uint64_t *held, int n, int k) {
+  const int lane = threadIdx.x % 64;
+  uint64_t mine[HELD / 64];
+#pragma unroll
+  for (int j = 0; j < HELD / 64; ++j) mine[j] = lane + 64 * j < n ? held[lane + 64 * j] : 0;
+  wave_sync_lds();
+  const int kept = min(n, k);
+  for (int i = 0; i < kept; ++i) {
+    uint64_t top = 0;
+#pragma unroll
+    for (int j = 0; j < HELD / 64; ++j) top = mine[j] > top ? mine[j] : top;
+    top = wave_most(top);
+    if (lane == 0) held[i] = top;
+#pragma unroll
+    for (int j = 0; j < HELD / 64; ++j) mine[j] = mine[j] == top ? 0 : mine[j];
+  }
+  wave_sync_lds();
+  return kept;
+}
+
+// the k largest of the list's n keys to its front, in order: each key's place is the number of keys before it
+__device__ __forceinline__ void sort_list(Shared &s, int n, int k) {
+  const int tid = threadIdx.x;
+  constexpr int EACH = WAVES * HELD / THREADS;
+  uint64_t mine[EACH];
+  int place[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    mine[j] = tid + THREADS * j < n ? s.list[tid + THREADS * j] : 0;
     place[j] = 0;
   }
-  if (tid + 1 == THREADS && n % 2) s.list[n] = 0;  // (n < LIST)
-  __syncthreads();
-  for (int i = 0; i < n; i += 2) {
-    const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&s.list[i]);
+  if (n <= THREADS) {
+    for (int i = 0; i < n; ++i) place[0] += s.list[i] > mine[0];
+  } else {
+    for (int i = 0; i < n; ++i) {
+      const uint64_t o = s.list[i];
 #pragma unroll
-    for (int j = 0; j < LIST / THREADS; ++j) place[j] += (o.x > mine[j]) + (o.y > mine[j]);
+      for (int j = 0; j < EACH; ++j) place[j] += o > mine[j];
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < LIST / THREADS; ++j)
+  for (int j = 0; j < EACH; ++j)
     if (mine[j] && place[j] < k) s.list[place[j]] = mine[j];
   if (tid == 0) s.count = min(n, k);
   __syncthreads();
-}
-
-// up to BATCH keys a thread into the list, those that reach the threshold (which grows where they are too many)
-template <int N>
-__device__ __forceinline__ void take(Shared &s, const uint64_t (&key)[N], uint64_t &threshold, int k) {
-  const int tid = threadIdx.x;
-  int n = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) n += key[j] >= threshold;
-  if (!__syncthreads_or(n)) return;
-  const int held = s.count;
-  int at = n ? atomicAdd(&s.count, n) : 0;
-  __syncthreads();
-  if (s.count >= LIST) {  // (the same in the whole workgroup)
-    __syncthreads();
-    if (tid == 0) s.count = held;
-    uint64_t top = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) top = key[j] > top ? key[j] : top;
-    const uint64_t t = kth_of_threads(s, top, k);  // at most k threads' keys reach it: N k in all
-    threshold = t > threshold ? t : threshold;
-    if (held + N * k >= LIST) {
-      tighten(s, k);
-      if (s.count == k && s.list[k - 1] > threshold) threshold = s.list[k - 1];
-    }
-    n = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += key[j] >= threshold;
-    __syncthreads();
-    at = n ? atomicAdd(&s.count, n) : 0;
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (key[j] >= threshold) s.list[at++] = key[j];
 }
 
 // the row's results from its joined part and its sorted alternatives
@@ -151,19 +146,23 @@ __device__ __forceinline__ void finish(const LogprobArgs &a, int64_t row, double
 }
 
 // Workgroup (part, row): `quads` aligned quads of the row's logits from part * quads on. ALONE: the row's only part.
+// Every wave picks its own candidates for the largest: a logit that reaches a bar which at least `top` of the wave's lanes
+// have reached so far. The bar is found again where many lanes reach it; at the end the highest of the waves' bars leaves a
+// few dozen candidates to sort.
 template <bool ALONE, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, int quads) {
   __shared__ Shared s;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
   const int64_t row = blockIdx.y;
   const float *x = a.logits + row * a.stride;
   const int ahead = (int)(reinterpret_cast<uintptr_t>(x) % 16 / 4);  // floats between an aligned address and the row
   const float *base = x - ahead;
   const int all = (int)(((int64_t)ahead + a.n + 3) / 4), from = blockIdx.x * quads, to = min(all, from + quads);
-  if (TOP && tid == 0) s.count = 0;
   float m = LOWEST, z = 0.0f, h = 0.0f;
-  uint64_t threshold = 0;
-  float bar = -__builtin_inff();
+  float bar = LOWEST;
+  uint64_t least = 0;  // a key that candidates are above, once ties have filled the wave's list
+  uint32_t reached = 0;
+  int held = 0;
   for (int q0 = from; q0 < to; q0 += THREADS * QUADS) {
     float v[BATCH];
 #pragma unroll
@@ -203,31 +202,58 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
     z += zs;
     h += hs;
     if (TOP) {
-      if (q0 == from || __syncthreads_or(most >= bar)) {
-        uint64_t key[BATCH], best = 0;
+      const int lanes = __popcll(__ballot(most >= bar));
+      if (lanes) {
+        if (q0 == from || lanes >= 8) {
+          reached = reached_by(m > LOWEST ? ordered_of(m) : 0, a.top);
+          if (reached) bar = __builtin_fmaxf(bar, value_of((uint64_t)reached << 32));
+        }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          key[j] = key_of(v[j], (uint32_t)((q0 + THREADS * (j / 4) + tid) * 4 - ahead + j % 4));
-          best = key[j] > best ? key[j] : best;
+          const uint64_t key = key_of(v[j], (uint32_t)((q0 + THREADS * (j / 4) + tid) * 4 - ahead + j % 4));
+          uint64_t takes = __ballot(v[j] >= bar && key > least);
+          if (!takes) continue;
+          if (held + __popcll(takes) > HELD) {
+            held = wave_tighten(s.held[wave], held, a.top);
+            if (held == a.top) {
+              least = s.held[wave][held - 1];
+              bar = __builtin_fmaxf(bar, value_of(least));
+            }
+            takes = __ballot(v[j] >= bar && key > least);
+          }
+          if (v[j] >= bar && key > least)
+            s.held[wave][held + __builtin_amdgcn_mbcnt_hi((uint32_t)(takes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takes, 0))] = key;
+          held += __popcll(takes);
         }
-        if (q0 == from) {  // the first threshold: the k-th of the threads' largest
-          const uint64_t t = kth_of_threads(s, best, a.top);
-          threshold = t > 1 ? t : 1;
-        }
-        take(s, key, threshold, a.top);
-        bar = value_of(threshold);
       }
     }
   }
   // the workgroup's part: across the lanes, then the waves
 #pragma unroll
   for (int o = 32; o; o >>= 1) join(m, z, h, __shfl_xor(m, o), __shfl_xor(z, o), __shfl_xor(h, o));
-  if (tid % 64 == 0) s.parts[tid / 64] = Part{m, z, h, 0};
+  if (lane == 0) {
+    s.parts[wave] = Part{m, z, h, 0};
+    if (TOP) {
+      s.bars[wave] = reached;
+      s.counts[wave] = held;
+    }
+  }
+  if (TOP && tid == 0) s.count = 0;
   __syncthreads();
-  if (TOP) tighten(s, a.top);
+  if (TOP) {
+    uint32_t high = s.bars[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) high = s.bars[w] > high ? s.bars[w] : high;
+    for (int i = lane; i < held; i += 64) {
+      const uint64_t key = s.held[wave][i];
+      if ((uint32_t)(key >> 32) >= high) s.list[atomicAdd(&s.count, 1)] = key;
+    }
+    __syncthreads();
+    sort_list(s, s.count, a.top);
+  }
   double dm = s.parts[0].m, dz = s.parts[0].z, dh = s.parts[0].h;
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w)
+  for (int w = 1; w < WAVES; ++w)
     join(dm, dz, dh, (double)s.parts[w].m, (double)s.parts[w].z, (double)s.parts[w].h);
   if (ALONE) {
     finish(a, row, dm, dz, dh, s.list, TOP ? s.count : 0);
@@ -244,47 +270,68 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
 template <bool TOP>
 __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArgs a, int parts) {
   __shared__ Shared s;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
   const int64_t row = blockIdx.x;
   const Part *p = reinterpret_cast<const Part *>(a.workspace) + row * parts;
-  if (TOP && tid == 0) s.count = 0;
+  const uint64_t *keys = reinterpret_cast<const uint64_t *>(a.workspace + sizeof(Part) * parts * (int64_t)gridDim.x) +
+                         row * parts * a.top;
+  const int n = TOP ? parts * a.top : 0;
+  uint64_t best = 0;
+  for (int i = tid; i < n; i += THREADS) best = keys[i] > best ? keys[i] : best;
   float m = LOWEST, z = 0.0f, h = 0.0f;
   for (int i = tid; i < parts; i += THREADS) join(m, z, h, p[i].m, p[i].z, p[i].h);
 #pragma unroll
   for (int o = 32; o; o >>= 1) join(m, z, h, __shfl_xor(m, o), __shfl_xor(z, o), __shfl_xor(h, o));
-  if (tid % 64 == 0) s.parts[tid / 64] = Part{m, z, h, 0};
+  const uint32_t reached = TOP ? reached_by((uint32_t)(best >> 32), a.top) : 0;
+  if (lane == 0) {
+    s.parts[wave] = Part{m, z, h, 0};
+    s.bars[wave] = reached;
+  }
+  if (tid == 0) s.count = 0;
   __syncthreads();
   if (TOP) {
-    const uint64_t *keys = reinterpret_cast<const uint64_t *>(a.workspace + sizeof(Part) * parts * (int64_t)gridDim.x) +
-                           row * parts * a.top;
-    uint64_t threshold = 1;
-    for (int at = 0; at < parts * a.top; at += THREADS * BATCH) {
-      uint64_t key[BATCH], best = 0;
+    uint32_t high = s.bars[0];
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int i = at + THREADS * j + tid;
-        key[j] = i < parts * a.top ? keys[i] : 0;
-        best = key[j] > best ? key[j] : best;
+    for (int w = 1; w < WAVES; ++w) high = s.bars[w] > high ? s.bars[w] : high;
+    const uint64_t least = high ? (uint64_t)high << 32 : 1;
+    for (int i = tid; i < n; i += THREADS)
+      if (keys[i] >= least) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < WAVES * HELD) s.list[at] = keys[i];
       }
-      if (at == 0) {
-        const uint64_t t = kth_of_threads(s, best, a.top);
-        threshold = t > 1 ? t : 1;
-      }
-      take(s, key, threshold, a.top);
-    }
     __syncthreads();
-    tighten(s, a.top);
+    const int count = s.count;
+    __syncthreads();
+    if (count <= WAVES * HELD) {
+      sort_list(s, count, a.top);
+    } else {  // ties by the thousand: the largest one at a time
+      uint64_t last = ~0ull;
+      for (int k = 0; k < a.top; ++k) {
+        best = 0;
+        for (int i = tid; i < n; i += THREADS) best = keys[i] < last && keys[i] > best ? keys[i] : best;
+        best = wave_most(best);
+        if (lane == 0) s.best[wave] = best;
+        __syncthreads();
+        last = s.best[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) last = s.best[w] > last ? s.best[w] : last;
+        if (tid == 0) s.list[k] = last;
+        __syncthreads();
+      }
+      if (tid == 0) s.count = a.top;
+      __syncthreads();
+    }
   }
   double dm = s.parts[0].m, dz = s.parts[0].z, dh = s.parts[0].h;
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w)
+  for (int w = 1; w < WAVES; ++w)
     join(dm, dz, dh, (double)s.parts[w].m, (double)s.parts[w].z, (double)s.parts[w].h);
   finish(a, row, dm, dz, dh, s.list, TOP ? s.count : 0);
 }
 
-// a row's parts: enough workgroups for the card, each with at least a thousand logits
+// a row's parts: enough workgroups for the card, each with a batch of its threads at least
 int parts_of(int32_t m, int32_t n) {
-  const int64_t most = ((int64_t)n + 1023) / 1024, wanted = (1024 + (int64_t)m - 1) / m;
+  const int64_t most = ((int64_t)n + THREADS * BATCH - 1) / (THREADS * BATCH), wanted = (1024 + (int64_t)m - 1) / m;
   return (int)(wanted < most ? wanted : most);
 }
 
