@@ -4,6 +4,8 @@
 // exp(x - m) (x - m). One pass over the logits: every thread keeps its m, Z and H (rescaled when m grows), and the largest
 // are picked out on the way by a threshold that only ever grows. Bound by reading the logits once; a few rows are split
 // over many workgroups, whose parts a second launch joins.
+#include <algorithm>
+
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -11,7 +13,7 @@ namespace ple {
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 constexpr float LOWEST = -3.402823466e38f;
 constexpr int THREADS = 256, WAVES = THREADS / 64, QUADS = 4, BATCH = 4 * QUADS;  // logits a thread takes at once
 constexpr int HELD = 256;  // candidates a wave holds
@@ -33,12 +35,12 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
 }
 
-// m, Z, H of two parts together (z 0: an empty part, whatever its m)
+// m, Z, H (in nats) of two parts together (z 0: an empty part, whatever its m)
 template <class T>
 __device__ __forceinline__ void join(T &m, T &z, T &h, T m2, T z2, T h2) {
   const T top = m2 > m || m2 != m2 ? m2 : m;  // (a NaN stays)
-  // (a part's m may lie 2^128 below: its factor is 0, its difference kept finite)
-  const T d1 = m - top < (T)-1e30 ? (T)-1e30 : m - top, d2 = m2 - top < (T)-1e30 ? (T)-1e30 : m2 - top;
+  // (a part's m may lie 2^128 below, or be minus infinity: its factor is 0, its difference kept finite)
+  const T d1 = m - top > (T)-1e30 ? m - top : (T)-1e30, d2 = m2 - top > (T)-1e30 ? m2 - top : (T)-1e30;
   const T f1 = (T)__builtin_amdgcn_exp2f((float)(d1 * (T)LOG2E)), f2 = (T)__builtin_amdgcn_exp2f((float)(d2 * (T)LOG2E));
   h = (h + z * d1) * f1 + (h2 + z2 * d2) * f2;
   z = z * f1 + z2 * f2;
@@ -47,25 +49,81 @@ __device__ __forceinline__ void join(T &m, T &z, T &h, T m2, T z2, T h2) {
 
 struct Shared {
   uint64_t held[WAVES][HELD];  // the waves' candidates
-  uint64_t list[WAVES * HELD];
+  uint64_t list[WAVES * HELD + 8];
   uint64_t best[WAVES];
-  uint32_t bars[WAVES];
-  int counts[WAVES], count;
+  uint32_t bars[WAVES][2];
+  int count;
   Part parts[WAVES];
 };
 
 __device__ __forceinline__ uint32_t ordered_of(float x) { return (uint32_t)(key_of(x, 0) >> 32); }
 
-// a value that at least k (at most 64) of the wave's lanes reach, the largest of 20 leading bits (in ordered_of's bits; 0
-// where fewer lanes hold one): a bit at a time, by counting lanes
+// a value that at least k (at most 64) of the wave's lanes reach, the largest of 16 leading bits (in ordered_of's bits; 0
+// where fewer lanes hold one): two bits at a time, by counting lanes
 __device__ __forceinline__ uint32_t reached_by(uint32_t mine, int k) {
   uint32_t t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 12; --bit) {
-    const uint32_t more = t | 1u << bit;
-    if (__popcll(__ballot(mine >= more)) >= k) t = more;
+  for (int bit = 30; bit >= 16; bit -= 2) {
+    const uint32_t one = t | 1u << bit, two = t | 2u << bit, three = t | 3u << bit;
+    const int a = __popcll(__ballot(mine >= one)), b = __popcll(__ballot(mine >= two)), c = __popcll(__ballot(mine >= three));
+    t = c >= k ? three : b >= k ? two : a >= k ? one : t;
   }
   return t;
+}
+
+// the wave's sum, and its largest (a NaN stays), in every lane: by DPP within rows of 16, their last lanes broadcast on
+template <class F>
+__device__ __forceinline__ float wave_all(float x, F f) {
+#define STEP(from, rows) \
+  f(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), from, rows, 0xF, false)))
+  x = STEP(0xB1, 0xF);   // lane ^ 1
+  x = STEP(0x4E, 0xF);   // lane ^ 2
+  x = STEP(0x141, 0xF);  // 8 lanes mirrored
+  x = STEP(0x140, 0xF);  // 16 mirrored: every lane holds its row's
+#undef STEP
+  const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 0)),
+              b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16)),
+              c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 32)),
+              d = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 48));
+  return f(f(a, b), f(c, d));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return wave_all(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_top(float x) {
+  return wave_all(x, [](float a, float b) { return wmax(a, b); });
+}
+// the parts of the wave's lanes as one (z 0: an empty part, whatever its m)
+__device__ __forceinline__ void join_lanes(float &m, float &z, float &h) {
+  const float top = wave_top(m), d = z > 0.0f ? __builtin_fmaxf(m - top, -1e30f) : 0.0f;
+  const float f = __builtin_amdgcn_exp2f(d * LOG2E);
+  h = wave_sum(__builtin_fmaf(d, z, h) * f);
+  z = wave_sum(z * f);
+  m = top;
+}
+
+// a bar that at least k of the workgroup's threads reach: one that k of some wave's lanes reach (`alone`), or each wave's
+// share of k
+__device__ __forceinline__ void raise_bars(Shared &s, uint32_t alone, uint32_t mine, int k) {
+  const uint32_t share = reached_by(mine, (k + WAVES - 1) / WAVES);
+  if (threadIdx.x % 64 == 0) {
+    s.bars[threadIdx.x / 64][0] = alone;
+    s.bars[threadIdx.x / 64][1] = share;
+  }
+}
+__device__ __forceinline__ uint32_t highest_bar(const Shared &s) {
+  uint32_t alone = s.bars[0][0], share = s.bars[0][1];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    alone = s.bars[w][0] > alone ? s.bars[w][0] : alone;
+    share = s.bars[w][1] < share ? s.bars[w][1] : share;
+  }
+  return share > alone ? share : alone;
+}
+
+// the lanes of a mask before this one
+__device__ __forceinline__ int before_me(uint64_t lanes) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
 }
 
 __device__ __forceinline__ uint64_t wave_most(uint64_t x) {
@@ -85,6 +143,7 @@ __device__ __forceinline__ int wave_tighten(uint64_t *held, int n, int k) {
   for (int j = 0; j < HELD / 64; ++j) mine[j] = lane + 64 * j < n ? held[lane + 64 * j] : 0;
   wave_sync_lds();
   const int kept = min(n, k);
+#pragma unroll 1
   for (int i = 0; i < kept; ++i) {
     uint64_t top = 0;
 #pragma unroll
@@ -98,20 +157,31 @@ __device__ __forceinline__ int wave_tighten(uint64_t *held, int n, int k) {
   return kept;
 }
 
-// the k largest of the list's n keys to its front, in order: each key's place is the number of keys before it
+// the k largest of the list's n keys to its front, in order: each key's place is the number of keys before it. (The list
+// holds zeros for eight places from n on.)
 __device__ __forceinline__ void sort_list(Shared &s, int n, int k) {
   const int tid = threadIdx.x;
   constexpr int EACH = WAVES * HELD / THREADS;
   uint64_t mine[EACH];
   int place[EACH];
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    mine[j] = tid + THREADS * j < n ? s.list[tid + THREADS * j] : 0;
-    place[j] = 0;
-  }
+  for (int j = 0; j < EACH; ++j) mine[j] = place[j] = 0;
   if (n <= THREADS) {
-    for (int i = 0; i < n; ++i) place[0] += s.list[i] > mine[0];
+    if (tid < n) {
+      mine[0] = s.list[tid];
+#pragma unroll 1
+      for (int i = 0; i < n; i += 8) {
+        uint64_t o[8];  // (eight reads in flight)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) o[u] = s.list[i + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) place[0] += o[u] > mine[0];
+      }
+    }
   } else {
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) mine[j] = tid + THREADS * j < n ? s.list[tid + THREADS * j] : 0;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const uint64_t o = s.list[i];
 #pragma unroll
@@ -131,7 +201,7 @@ __device__ __forceinline__ void finish(const LogprobArgs &a, int64_t row, double
                                        int held) {
   const float *x = a.logits + row * a.stride;
   const bool fine = z > 0.0 && m > (double)-__builtin_inff() && m < (double)__builtin_inff();
-  const double nan = __builtin_nan(""), logz = log(z);
+  const double nan = __builtin_nan(""), logz = logf((float)z);
   if (threadIdx.x == 0 && a.entropy) a.entropy[row] = (float)(fine ? logz - h / z : nan);
   for (int g = threadIdx.x; g < a.n_given; g += THREADS) {
     const int t = a.given[row * a.n_given + g];
@@ -157,11 +227,21 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
   const float *x = a.logits + row * a.stride;
   const int ahead = (int)(reinterpret_cast<uintptr_t>(x) % 16 / 4);  // floats between an aligned address and the row
   const float *base = x - ahead;
-  const int all = (int)(((int64_t)ahead + a.n + 3) / 4), from = blockIdx.x * quads, to = min(all, from + quads);
-  float m = LOWEST, z = 0.0f, h = 0.0f;
+  const int all = (int)(((int64_t)ahead + a.n + 3) / 4), from = blockIdx.x * quads, to = blockIdx.x + 1 == gridDim.x ? all : min(all, from + quads);
+  // the thread's largest logit m, and against a reference of m: Z = sum 2^t, H = sum 2^t t, t = x log2(e) - up, up the next
+  // whole number above m log2(e): a multiply-add an exponential's argument, every rescaling exact. (Logits past 2^20, where
+  // that loses t, are taken against m itself: t = (x - m) log2(e).)
+  float m = -__builtin_inff(), up = 0.0f, z = 0.0f, h = 0.0f;
+  bool plain = false;  // (the same in the whole wave)
+  auto to_plain = [&] {  // Z and H against m itself
+    const float g = plain ? 0.0f : z > 0.0f ? __builtin_fmaf(-m, LOG2E, up) : 0.0f;
+    h = __builtin_fmaf(g, z, h);
+    const float f = __builtin_amdgcn_exp2f(g);
+    z *= f;
+    h *= f;
+  };
   float bar = LOWEST;
   uint64_t least = 0;  // a key that candidates are above, once ties have filled the wave's list
-  uint32_t reached = 0;
   int held = 0;
   for (int q0 = from; q0 < to; q0 += THREADS * QUADS) {
     float v[BATCH];
@@ -188,16 +268,38 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
     float most = v[0];
 #pragma unroll
     for (int j = 1; j < BATCH; ++j) most = wmax(most, v[j]);
-    const float top = wmax(m, most), d = __builtin_fmaxf(m - top, -1e30f), f = __builtin_amdgcn_exp2f(d * LOG2E);
-    h = (h + z * d) * f;
-    z = z * f;
-    m = top;
+    const float top = wmax(m, most);
+    if (!plain && __any(!(__builtin_fabsf(top) <= 0x1p20f) && top != -__builtin_inff())) {
+      to_plain();
+      plain = true;
+      up = m > -__builtin_inff() ? m : 0.0f;
+    }
     float zs = 0.0f, hs = 0.0f;
+    m = top;
+    if (!plain) {
+      const float next = m > -__builtin_inff() ? __builtin_ceilf(m * LOG2E) : 0.0f;
+      const float f = z > 0.0f ? __builtin_amdgcn_exp2f(up - next) : 0.0f;
+      h = __builtin_fmaf(up - next, z, h) * f;
+      z = z * f;
+      up = next;
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const float t = __builtin_fmaxf(v[j] - m, -150.0f), e = __builtin_amdgcn_exp2f(t * LOG2E);
-      zs += e;
-      hs = __builtin_fmaf(e, t, hs);
+      for (int j = 0; j < BATCH; ++j) {
+        const float t = __builtin_fmaxf(__builtin_fmaf(v[j], LOG2E, -up), -150.0f), e = __builtin_amdgcn_exp2f(t);
+        zs += e;
+        hs = __builtin_fmaf(e, t, hs);
+      }
+    } else {
+      const float next = m > -__builtin_inff() ? m : 0.0f;
+      const float d = z > 0.0f ? __builtin_fmaxf((up - next) * LOG2E, -1e30f) : 0.0f, f = __builtin_amdgcn_exp2f(d);
+      h = __builtin_fmaf(d, z, h) * f;
+      z = z * f;
+      up = next;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const float t = __builtin_fmaxf((v[j] - up) * LOG2E, -150.0f), e = __builtin_amdgcn_exp2f(t);
+        zs += e;
+        hs = __builtin_fmaf(e, t, hs);
+      }
     }
     z += zs;
     h += hs;
@@ -205,51 +307,73 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
       const int lanes = __popcll(__ballot(most >= bar));
       if (lanes) {
         if (q0 == from || lanes >= 8) {
-          reached = reached_by(m > LOWEST ? ordered_of(m) : 0, a.top);
+          const uint32_t reached = reached_by(ordered_of(m), a.top);
           if (reached) bar = __builtin_fmaxf(bar, value_of((uint64_t)reached << 32));
         }
+        uint64_t takes[BATCH];
+        int all = 0;
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          const uint64_t key = key_of(v[j], (uint32_t)((q0 + THREADS * (j / 4) + tid) * 4 - ahead + j % 4));
-          uint64_t takes = __ballot(v[j] >= bar && key > least);
+          takes[j] = __ballot(v[j] >= bar);
+          all += __popcll(takes[j]);
+        }
+        const uint32_t first = (uint32_t)((q0 + tid) * 4 - ahead);  // the lane's first logit
+        if (!least && held + all <= HELD) {
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j) {
+            if (!takes[j]) continue;
+            if (v[j] >= bar)
+              s.held[wave][held + before_me(takes[j])] = key_of(v[j], first + (uint32_t)(THREADS * (j / 4) * 4 + j % 4));
+            held += __popcll(takes[j]);
+          }
+          continue;
+        }
+        // ties or an ascending row: a value a lane at a time, the list tightened where it is full
+#pragma unroll 1
+        for (int j = 0; j < BATCH; ++j) {
+          const float x = v[0];
+#pragma unroll
+          for (int i = 1; i < BATCH; ++i) v[i - 1] = v[i];
+          uint64_t takes = __ballot(x >= bar);
           if (!takes) continue;
+          const uint64_t key = key_of(x, first + (uint32_t)(THREADS * (j / 4) * 4 + j % 4));
+          bool mine = x >= bar && key > least;
+          takes = __ballot(mine);
           if (held + __popcll(takes) > HELD) {
             held = wave_tighten(s.held[wave], held, a.top);
             if (held == a.top) {
               least = s.held[wave][held - 1];
               bar = __builtin_fmaxf(bar, value_of(least));
             }
-            takes = __ballot(v[j] >= bar && key > least);
+            mine = x >= bar && key > least;
+            takes = __ballot(mine);
           }
-          if (v[j] >= bar && key > least)
-            s.held[wave][held + __builtin_amdgcn_mbcnt_hi((uint32_t)(takes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)takes, 0))] = key;
+          if (mine)
+            s.held[wave][held + before_me(takes)] = key;
           held += __popcll(takes);
         }
       }
     }
   }
-  // the workgroup's part: across the lanes, then the waves
-#pragma unroll
-  for (int o = 32; o; o >>= 1) join(m, z, h, __shfl_xor(m, o), __shfl_xor(z, o), __shfl_xor(h, o));
-  if (lane == 0) {
-    s.parts[wave] = Part{m, z, h, 0};
-    if (TOP) {
-      s.bars[wave] = reached;
-      s.counts[wave] = held;
-    }
-  }
+  // the workgroup's part: across the lanes, then the waves (H by whole exponentials' arguments: in nats)
+  to_plain();
+  h *= LN2;
+  if (TOP) raise_bars(s, bar > LOWEST ? ordered_of(bar) : 0, ordered_of(m), a.top);
+  join_lanes(m, z, h);
+  if (lane == 0) s.parts[wave] = Part{m, z, h, 0};
   if (TOP && tid == 0) s.count = 0;
   __syncthreads();
   if (TOP) {
-    uint32_t high = s.bars[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) high = s.bars[w] > high ? s.bars[w] : high;
+    const uint32_t high = highest_bar(s);
     for (int i = lane; i < held; i += 64) {
       const uint64_t key = s.held[wave][i];
       if ((uint32_t)(key >> 32) >= high) s.list[atomicAdd(&s.count, 1)] = key;
     }
     __syncthreads();
-    sort_list(s, s.count, a.top);
+    const int count = s.count;
+    if (tid < 8) s.list[count + tid] = 0;
+    __syncthreads();
+    sort_list(s, count, a.top);
   }
   double dm = s.parts[0].m, dz = s.parts[0].z, dh = s.parts[0].h;
 #pragma unroll
@@ -280,19 +404,13 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
   for (int i = tid; i < n; i += THREADS) best = keys[i] > best ? keys[i] : best;
   float m = LOWEST, z = 0.0f, h = 0.0f;
   for (int i = tid; i < parts; i += THREADS) join(m, z, h, p[i].m, p[i].z, p[i].h);
-#pragma unroll
-  for (int o = 32; o; o >>= 1) join(m, z, h, __shfl_xor(m, o), __shfl_xor(z, o), __shfl_xor(h, o));
-  const uint32_t reached = TOP ? reached_by((uint32_t)(best >> 32), a.top) : 0;
-  if (lane == 0) {
-    s.parts[wave] = Part{m, z, h, 0};
-    s.bars[wave] = reached;
-  }
+  join_lanes(m, z, h);
+  if (TOP) raise_bars(s, reached_by((uint32_t)(best >> 32), a.top), (uint32_t)(best >> 32), a.top);
+  if (lane == 0) s.parts[wave] = Part{m, z, h, 0};
   if (tid == 0) s.count = 0;
   __syncthreads();
   if (TOP) {
-    uint32_t high = s.bars[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) high = s.bars[w] > high ? s.bars[w] : high;
+    const uint32_t high = highest_bar(s);
     const uint64_t least = high ? (uint64_t)high << 32 : 1;
     for (int i = tid; i < n; i += THREADS)
       if (keys[i] >= least) {
@@ -301,6 +419,7 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
       }
     __syncthreads();
     const int count = s.count;
+    if (tid < 8 && count <= WAVES * HELD) s.list[count + tid] = 0;
     __syncthreads();
     if (count <= WAVES * HELD) {
       sort_list(s, count, a.top);
@@ -329,10 +448,11 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
   finish(a, row, dm, dz, dh, s.list, TOP ? s.count : 0);
 }
 
-// a row's parts: enough workgroups for the card, each with a batch of its threads at least
+// a row's parts, of whole batches of a workgroup: enough workgroups to fill the card
 int parts_of(int32_t m, int32_t n) {
-  const int64_t most = ((int64_t)n + THREADS * BATCH - 1) / (THREADS * BATCH), wanted = (1024 + (int64_t)m - 1) / m;
-  return (int)(wanted < most ? wanted : most);
+  const int64_t batches = ((int64_t)n + THREADS * BATCH - 1) / (THREADS * BATCH);
+  const int64_t each = std::max<int64_t>(1, batches * m / 1024);
+  return (int)((batches + each - 1) / each);
 }
 
 }  // namespace
@@ -344,8 +464,9 @@ int64_t logprobs_workspace(int32_t m, int32_t n, int32_t top) {
 
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {
   const int parts = parts_of(a.m, a.n);
-  // (three floats more than n where a row starts behind an aligned address)
-  const int quads = (int)((((int64_t)a.n + 6) / 4 + parts - 1) / parts);
+  // (three floats more than n where a row starts behind an aligned address: the last part takes them)
+  const int64_t batches = ((int64_t)a.n + THREADS * BATCH - 1) / (THREADS * BATCH);
+  const int quads = (int)((batches + parts - 1) / parts) * THREADS * QUADS;
   for (int32_t row = 0; row < a.m; row += 65535) {
     LogprobArgs b = a;
     b.m = a.m - row < 65535 ? a.m - row : 65535;

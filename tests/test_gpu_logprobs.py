@@ -130,6 +130,20 @@ def test_flat_and_peaked_rows():
     assert ids[1, 0] == 7 and ids[2, 0] == 9 and list(ids[0]) == [0, 1]
 
 
+@pytest.mark.parametrize("size", [1.0, 1e3, 1.04e6, 1.05e6, 1e7, 1e30, 3.4028234e38])
+def test_logits_of_any_size(size):
+    """the two ways a thread's sums are taken (past 2^20 against the largest logit itself), a row that crosses from one to the
+    other on the way, rows of the type's lowest value"""
+    rng = np.random.default_rng(8)
+    x = (rng.standard_normal((5, 20011)) * 2).astype(np.float32)
+    x[0] += np.float32(size)
+    x[1] -= np.float32(size)
+    x[2, 10000:] += np.float32(size)
+    x[3] = -np.float32(size)
+    x[4, :3] = -np.float32(size)
+    agree(x, rng.integers(0, 20011, (5, 3)), 9)
+
+
 def test_rows_without_probabilities():
     """a NaN, an infinity, nothing but minus infinity: NaN and -1 in that row, the others as without it"""
     rng = np.random.default_rng(4)
