@@ -47,6 +47,9 @@ __device__ __forceinline__ void join(T &m, T &z, T &h, T m2, T z2, T h2) {
   m = top;
 }
 
+// the candidates a part passes on: what is left of them behind its bar, as a rule
+__host__ __device__ constexpr int slots_of(int top) { return top ? 2 * top + 8 : 0; }
+
 struct Shared {
   uint64_t held[WAVES][HELD];  // the waves' candidates
   uint64_t list[WAVES * HELD + 8];
@@ -243,8 +246,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
   float bar = LOWEST;
   uint64_t least = 0;  // a key that candidates are above, once ties have filled the wave's list
   int held = 0;
-  for (int q0 = from; q0 < to; q0 += THREADS * QUADS) {
-    float v[BATCH];
+  float4 next[QUADS];  // a batch is read while the one before it is worked on
+  auto read = [&](int q0) {
 #pragma unroll
     for (int j = 0; j < QUADS; ++j) {
       const int q = q0 + THREADS * j + tid;
@@ -260,11 +263,20 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
           if (e + 3 >= 0 && e + 3 < a.n) w.w = x[e + 3];
         }
       }
-      v[4 * j] = w.x;
-      v[4 * j + 1] = w.y;
-      v[4 * j + 2] = w.z;
-      v[4 * j + 3] = w.w;
+      next[j] = w;
     }
+  };
+  read(from);
+  for (int q0 = from; q0 < to; q0 += THREADS * QUADS) {
+    float v[BATCH];
+#pragma unroll
+    for (int j = 0; j < QUADS; ++j) {
+      v[4 * j] = next[j].x;
+      v[4 * j + 1] = next[j].y;
+      v[4 * j + 2] = next[j].z;
+      v[4 * j + 3] = next[j].w;
+    }
+    if (q0 + THREADS * QUADS < to) read(q0 + THREADS * QUADS);
     float most = v[0];
 #pragma unroll
     for (int j = 1; j < BATCH; ++j) most = wmax(most, v[j]);
@@ -277,11 +289,11 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
     float zs = 0.0f, hs = 0.0f;
     m = top;
     if (!plain) {
-      const float next = m > -__builtin_inff() ? __builtin_ceilf(m * LOG2E) : 0.0f;
-      const float f = z > 0.0f ? __builtin_amdgcn_exp2f(up - next) : 0.0f;
-      h = __builtin_fmaf(up - next, z, h) * f;
+      const float to_up = m > -__builtin_inff() ? __builtin_ceilf(m * LOG2E) : 0.0f;
+      const float f = z > 0.0f ? __builtin_amdgcn_exp2f(up - to_up) : 0.0f;
+      h = __builtin_fmaf(up - to_up, z, h) * f;
       z = z * f;
-      up = next;
+      up = to_up;
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         const float t = __builtin_fmaxf(__builtin_fmaf(v[j], LOG2E, -up), -150.0f), e = __builtin_amdgcn_exp2f(t);
@@ -289,11 +301,11 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
         hs = __builtin_fmaf(e, t, hs);
       }
     } else {
-      const float next = m > -__builtin_inff() ? m : 0.0f;
-      const float d = z > 0.0f ? __builtin_fmaxf((up - next) * LOG2E, -1e30f) : 0.0f, f = __builtin_amdgcn_exp2f(d);
+      const float to_up = m > -__builtin_inff() ? m : 0.0f;
+      const float d = z > 0.0f ? __builtin_fmaxf((up - to_up) * LOG2E, -1e30f) : 0.0f, f = __builtin_amdgcn_exp2f(d);
       h = __builtin_fmaf(d, z, h) * f;
       z = z * f;
-      up = next;
+      up = to_up;
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         const float t = __builtin_fmaxf((v[j] - up) * LOG2E, -150.0f), e = __builtin_amdgcn_exp2f(t);
@@ -371,9 +383,12 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
     }
     __syncthreads();
     const int count = s.count;
-    if (tid < 8) s.list[count + tid] = 0;
-    __syncthreads();
-    sort_list(s, count, a.top);
+    // (a part's candidates are sorted only where they are more than its slots)
+    if (ALONE || count > slots_of(a.top)) {
+      if (tid < 8) s.list[count + tid] = 0;
+      __syncthreads();
+      sort_list(s, count, a.top);
+    }
   }
   double dm = s.parts[0].m, dz = s.parts[0].z, dh = s.parts[0].h;
 #pragma unroll
@@ -385,8 +400,8 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
   }
   const int64_t part = row * gridDim.x + blockIdx.x;
   if (tid == 0) reinterpret_cast<Part *>(a.workspace)[part] = Part{(float)dm, (float)dz, (float)dh, 0};
-  if (TOP && tid < a.top)
-    reinterpret_cast<uint64_t *>(a.workspace + sizeof(Part) * gridDim.x * gridDim.y)[part * a.top + tid] =
+  if (TOP && tid < slots_of(a.top))
+    reinterpret_cast<uint64_t *>(a.workspace + sizeof(Part) * gridDim.x * gridDim.y)[part * slots_of(a.top) + tid] =
         tid < s.count ? s.list[tid] : 0;
 }
 
@@ -398,10 +413,15 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
   const int64_t row = blockIdx.x;
   const Part *p = reinterpret_cast<const Part *>(a.workspace) + row * parts;
   const uint64_t *keys = reinterpret_cast<const uint64_t *>(a.workspace + sizeof(Part) * parts * (int64_t)gridDim.x) +
-                         row * parts * a.top;
-  const int n = TOP ? parts * a.top : 0;
-  uint64_t best = 0;
-  for (int i = tid; i < n; i += THREADS) best = keys[i] > best ? keys[i] : best;
+                         row * parts * slots_of(a.top);
+  const int n = TOP ? parts * slots_of(a.top) : 0;
+  uint64_t mine[8], best = 0;  // (the first 2048 are read once)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    mine[j] = tid + THREADS * j < n ? keys[tid + THREADS * j] : 0;
+    best = mine[j] > best ? mine[j] : best;
+  }
+  for (int i = tid + THREADS * 8; i < n; i += THREADS) best = keys[i] > best ? keys[i] : best;
   float m = LOWEST, z = 0.0f, h = 0.0f;
   for (int i = tid; i < parts; i += THREADS) join(m, z, h, p[i].m, p[i].z, p[i].h);
   join_lanes(m, z, h);
@@ -412,11 +432,14 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
   if (TOP) {
     const uint32_t high = highest_bar(s);
     const uint64_t least = high ? (uint64_t)high << 32 : 1;
-    for (int i = tid; i < n; i += THREADS)
-      if (keys[i] >= least) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < WAVES * HELD) s.list[at] = keys[i];
-      }
+    auto take = [&](uint64_t key) {
+      if (key < least) return;
+      const int at = atomicAdd(&s.count, 1);
+      if (at < WAVES * HELD) s.list[at] = key;
+    };
+#pragma unroll
+    for (int j = 0; j < 8; ++j) take(mine[j]);
+    for (int i = tid + THREADS * 8; i < n; i += THREADS) take(keys[i]);
     __syncthreads();
     const int count = s.count;
     if (tid < 8 && count <= WAVES * HELD) s.list[count + tid] = 0;
@@ -459,7 +482,7 @@ int parts_of(int32_t m, int32_t n) {
 
 int64_t logprobs_workspace(int32_t m, int32_t n, int32_t top) {
   const int64_t parts = parts_of(m, n);
-  return parts == 1 ? 0 : parts * m * ((int64_t)sizeof(Part) + 8 * top);
+  return parts == 1 ? 0 : parts * m * ((int64_t)sizeof(Part) + 8 * slots_of(top));
 }
 
 hipError_t launch_logprobs(const LogprobArgs &a, hipStream_t s) {
