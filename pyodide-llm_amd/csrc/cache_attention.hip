@@ -5,7 +5,7 @@
 // A wave takes 32 rows (tokens x query heads of one kv head) of one block of positions and goes over the cache's blocks
 // once, with a running maximum and sum. The rows are the columns of every product, so that a row's statistics live in its
 // lane (and the lane 32 past it):
-//   S^T = K Q^T on i8 MFMA: a query in three signed base-256 digits, x = round(q * 8355000 / max|q|) = 65536 d0 + 256 d1 +
+//   S^T = K Q^T on i8 MFMA: a query in three signed base-256 digits, x = round(q * 4160000 / max|q|) = 65536 d0 + 256 d1 +
 //     d2: float32's precision (2^-23 of the row's largest), the keys' bytes as they lie, the int32 sums exact;
 //   O^T = V^T P^T on f16 MFMA: the values' bytes are exact in f16, a probability goes in two halves (22 bits).
 // Maxima are rounded up to whole powers of two, so that every rescaling is exact; the products' scale (2^mw - 14) follows
@@ -27,25 +27,24 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr float DIGITS = 4160000.0f;  // a query's largest value in digits (below 2^22 - 0x8080)
 constexpr float NONE = -1e30f;  // no maximum yet (finite: its differences stay numbers)
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
-// a query's 16 values as three words of digits each four: round(x * m) = 65536 d0 + 256 d1 + d2
+// four of a query's values as three words of digits: round(x m) = 65536 d0 + 256 d1 + d2, below 2^22. Added to 1.5 * 2^23
+// + 0x8080, the sum's low three bytes are d0 + 64, d1 + 128 and d2 + 128; they are gathered by value and taken back.
+// (16 instructions; with conversions, shifts and masks 72)
 __device__ __forceinline__ void digits(const float4 x, float m, int32_t &d0, int32_t &d1, int32_t &d2) {
-  const float in[4] = {x.x, x.y, x.z, x.w};
-  uint32_t w0 = 0, w1 = 0, w2 = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int32_t n = (int32_t)__builtin_rintf(in[j] * m);
-    const int32_t low = (int32_t)(int8_t)n, rest = (n - low) >> 8, mid = (int32_t)(int8_t)rest, high = (rest - mid) >> 8;
-    w0 |= (uint32_t)(high & 255) << (8 * j);
-    w1 |= (uint32_t)(mid & 255) << (8 * j);
-    w2 |= (uint32_t)(low & 255) << (8 * j);
-  }
-  d0 = (int32_t)w0;
-  d1 = (int32_t)w1;
-  d2 = (int32_t)w2;
+  constexpr float BIAS = 12582912.0f + 32896.0f;
+  const uint32_t a = __float_as_uint(__builtin_fmaf(x.x, m, BIAS)), b = __float_as_uint(__builtin_fmaf(x.y, m, BIAS)),
+                 c = __float_as_uint(__builtin_fmaf(x.z, m, BIAS)), d = __float_as_uint(__builtin_fmaf(x.w, m, BIAS));
+  const uint32_t low = __builtin_amdgcn_perm(b, a, 0x05010400u), high = __builtin_amdgcn_perm(d, c, 0x05010400u);
+  d2 = (int32_t)(__builtin_amdgcn_perm(high, low, 0x05040100u) ^ 0x80808080u);
+  d1 = (int32_t)(__builtin_amdgcn_perm(high, low, 0x07060302u) ^ 0x80808080u);
+  const uint32_t top = __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0602u), __builtin_amdgcn_perm(b, a, 0x0c0c0602u),
+                                             0x05040100u);
+  d0 = (int32_t)(((top | 0x80808080u) - 0x40404040u) ^ 0x80808080u);  // (no byte borrows from the next)
 }
 
 // four value bytes (value + 128) as two pairs of halves: 0x6400 | byte is 1024 + byte
@@ -96,9 +95,10 @@ struct Tile {
     first_token = ((pos >> tokens_log2) + index) << tokens_log2;
     last_token = min(end, first_token + (1 << tokens_log2)) - 1;
     own = first_token / CACHE_BLOCK;  // the tile's tokens lie in one block
-    token = first_token + col / group;
-    row = col / group < (1 << tokens_log2) && token >= pos && token < end;
-    qhead = head * group + col % group;
+    const int mine = (int)(((float)col + 0.5f) * __builtin_amdgcn_rcpf((float)group));  // col / group
+    token = first_token + mine;
+    row = mine < (1 << tokens_log2) && token >= pos && token < end;
+    qhead = head * group + col - mine * group;
     q = a.q + (int64_t)(row ? token - pos : 0) * a.q_stride + qhead * HS;
     unit = LOG2E / __builtin_sqrtf((float)HS);
     run = {NONE, 0.0f, NONE};
@@ -106,33 +106,37 @@ struct Tile {
     for (int t = 0; t < TILES; ++t) o[t] = (f32x16)(0.0f);
   }
 
-  // the queries' digits: lane (row, half) holds channels 32 s + 16 half .. + 15 of step s
+  // the queries' digits: lane (row, half) holds channels 32 s + 16 half .. + 15 of step s. (Every load first, none behind a
+  // branch: one after the other they took 6 us.)
   __device__ __forceinline__ void read_queries() {
+    float4 x[STEPS][4];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int d = 32 * s + 16 * half;
+      const float4 *from = reinterpret_cast<const float4 *>(q + (HS % 32 == 0 || d < HS ? d : 0));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[s][j] = from[j];
+    }
     float largest = 0.0f;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int d = 32 * s + 16 * half + 4 * j;
-        if (!row || d >= HS) continue;
-        const float4 x = *reinterpret_cast<const float4 *>(q + d);
-        largest = wmax(largest, wmax(wmax(__builtin_fabsf(x.x), __builtin_fabsf(x.y)),
-                                     wmax(__builtin_fabsf(x.z), __builtin_fabsf(x.w))));
+        if (!row || (HS % 32 && 32 * s + 16 * half >= HS)) x[s][j] = make_float4(0, 0, 0, 0);
+        largest = wmax(largest, wmax(wmax(__builtin_fabsf(x[s][j].x), __builtin_fabsf(x[s][j].y)),
+                                     wmax(__builtin_fabsf(x[s][j].z), __builtin_fabsf(x[s][j].w))));
       }
     largest = wmax(largest, other_half(largest));
     // (below 2^-100 a query is taken as zero; one that is not finite makes its row's scores not a number)
-    const bool finite = largest < __builtin_inff(), some = finite && largest > 0x1p-100f;
-    const float to_digits = some ? 8355000.0f / largest : 0.0f;
-    from_digits = finite ? largest / 8355000.0f * unit : __builtin_nanf("");
+    const bool finite = largest < __builtin_inff();
+    const float to_digits = finite && largest > 0x1p-100f ? DIGITS / largest : 0.0f;
+    from_digits = finite ? largest / DIGITS * unit : __builtin_nanf("");
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int d = 32 * s + 16 * half + 4 * j;
-        float4 x = make_float4(0, 0, 0, 0);
-        if (row && d < HS && some) x = *reinterpret_cast<const float4 *>(q + d);
         int32_t d0, d1, d2;
-        digits(x, to_digits, d0, d1, d2);
+        digits(x[s][j], to_digits, d0, d1, d2);
         q0[s][j] = d0;
         q1[s][j] = d1;
         q2[s][j] = d2;
@@ -240,6 +244,19 @@ struct Tile {
       if (p >= pos) return x + (int64_t)(p - pos) * a.rows.x_stride + head * HS;
       return recent + ((int64_t)(a.rows.displaced ? CACHE_RECENT + p % CACHE_BLOCK : p % CACHE_RECENT) * c.nkv + head) * HS;
     };
+    // (a shared block's values are asked for first: they come while its scores are made)
+    constexpr int MINE = PARTS > 1 ? (TILES + PARTS - 1) / PARTS : 1;
+    float x[MINE][16];
+    auto values = [&](int t, float (&to)[16]) {
+      const int d = HS % 32 == 0 || 32 * t + col < HS ? 32 * t + col : 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        to[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token))[d];
+    };
+    if (PARTS > 1) {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) values(min(i * PARTS + part, TILES - 1), x[i]);
+    }
     const bool key = p0 + col <= last_token;
     const float *k = source(a.rows.k, c.recent_keys, key ? p0 + col : last_token) + half * (HS / 2);
     const float *qh = q + half * (HS / 2);
@@ -248,11 +265,11 @@ struct Tile {
     for (int n = 0; n < (HS / 8 + PARTS - 1) / PARTS; ++n) {
       const int i = 4 * (n * PARTS + part);
       if (HS / 8 % PARTS && i >= HS / 2) break;  // (the same in the whole wave)
-      const float4 x = *reinterpret_cast<const float4 *>(k + i), y = *reinterpret_cast<const float4 *>(qh + i);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, s, 0, 0, 0);
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, s, 0, 0, 0);
+      const float4 kk = *reinterpret_cast<const float4 *>(k + i), y = *reinterpret_cast<const float4 *>(qh + i);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.x, y.x, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.y, y.y, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.z, y.z, s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.w, y.w, s, 0, 0, 0);
     }
     if (PARTS > 1) {
 #pragma unroll
@@ -274,30 +291,38 @@ struct Tile {
     }
     top = __builtin_fmaxf(top, other_half(top));
     const float factor = advance(top, 1.0f);
-    float bad = 0.0f, sum = 0.0f;
+    float sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int j = p0 + 8 * (r / 4) + 4 * half + r % 4;
-      const bool there = j <= last_token;
-      const float *v = source(a.rows.v, c.recent_values, there ? j : last_token);
-      const float e = j <= token ? __builtin_amdgcn_exp2f(p[r] - run.m) : 0.0f;
+      const float e = __builtin_amdgcn_exp2f(p[r] - run.m);  // (0 behind the token)
       sum += e;
-      const float w = e * factor;
-      bool strange = false;
+      p[r] = e * factor;
+    }
+    // a value that is not finite is left out of the product (which would carry it to rows that do not see it) and makes the
+    // rows that see it not a number
+    uint32_t strange = 0;  // bit r: this lane's value of its position r is not finite
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if (PARTS > 1 && t % PARTS != part) continue;  // (the same in the whole wave)
-        float x = 0.0f;
-        if (there && (HS % 32 == 0 || 32 * t + col < HS)) x = v[32 * t + col];
-        const bool fine = __builtin_fabsf(x) < __builtin_inff();
-        strange |= !fine;
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(fine ? x : 0.0f, w, o[t], 0, 0, 0);
+    for (int t = 0; t < TILES; ++t) {
+      if (PARTS > 1 && t % PARTS != part) continue;  // (the same in the whole wave)
+      float(&v)[16] = x[PARTS > 1 ? t / PARTS : 0];
+      if (PARTS == 1) values(t, v);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = p0 + 8 * (r / 4) + 4 * half + r % 4;
+        if (j > last_token || (HS % 32 && 32 * t + col >= HS)) v[r] = 0.0f;
+        const bool fine = __builtin_fabsf(v[r]) < __builtin_inff();
+        strange |= fine ? 0u : 1u << r;
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(fine ? v[r] : 0.0f, p[r], o[t], 0, 0, 0);
       }
-      // a value that is not finite is left out of the product (which would carry it to rows that do not see it) and makes
-      // the rows that see it not a number
-      const uint64_t any = __ballot(strange);
-      const int j0 = p0 + 8 * (r / 4) + r % 4;
-      if (((uint32_t)any && j0 <= token) || ((uint32_t)(any >> 32) && j0 + 4 <= token)) bad = __builtin_nanf("");
+    }
+    float bad = 0.0f;
+    if (__any(strange != 0)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint64_t any = __ballot(strange >> r & 1);
+        const int j0 = p0 + 8 * (r / 4) + r % 4;
+        if (((uint32_t)any && j0 <= token) || ((uint32_t)(any >> 32) && j0 + 4 <= token)) bad = __builtin_nanf("");
+      }
     }
     run.l = (PARTS > 1 && part ? 0.0f : run.l + sum) + bad;
   }
@@ -414,63 +439,72 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
 template <int HS>
 __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int tokens_log2, int rows, int most, int stride) {
   constexpr int QUADS = HS / 4, GROUPS = 256 / QUADS;
+  constexpr int AHEAD = 8;  // parts a thread reads before it knows their weights
   __shared__ float4 sums[GROUPS * QUADS];
-  __shared__ float scales[256];
-  __shared__ float tops[2][4], total[4];
-  const int tid = threadIdx.x, r = blockIdx.x, head = blockIdx.y, tile = blockIdx.z;
+  __shared__ float scales[4][256];
+  const int tid = threadIdx.x, lane = tid % 64, r = blockIdx.x, head = blockIdx.y, tile = blockIdx.z;
   const int pos = a.rows.dpos ? *a.rows.dpos : a.rows.pos, group = a.nh / a.rows.c.nkv;
-  const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + r / group;
+  const int mine = (int)(((float)r + 0.5f) * __builtin_amdgcn_rcpf((float)group));  // r / group
+  const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + mine;
   if (token < pos || token >= pos + a.rows.count) return;  // (the whole workgroup)
   const int parts = parts_of(token / CACHE_BLOCK, most) + 1;
   const int64_t at = ((int64_t)tile * gridDim.y + head) * stride;
-  const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (at * rows + r) * QUADS;
+  const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (at * rows + r) * QUADS + tid % QUADS;
   const float4 *stats = reinterpret_cast<const float4 *>(a.workspace) + (int64_t)stride * gridDim.y * gridDim.z * rows * QUADS +
                         at * rows + r;
-  const float4 mine = tid < parts ? stats[(int64_t)tid * rows] : make_float4(NONE, 0.0f, NONE, 0.0f);
-  float m = mine.x, mw = mine.z;
+  float4 stat[4], x[AHEAD];
 #pragma unroll
-  for (int x = 32; x; x >>= 1) {
-    m = __builtin_fmaxf(m, __shfl_xor(m, x));
-    mw = __builtin_fmaxf(mw, __shfl_xor(mw, x));
+  for (int j = 0; j < 4; ++j) {
+    stat[j] = make_float4(NONE, 0.0f, NONE, 0.0f);
+    if (lane + 64 * j < parts) stat[j] = stats[(int64_t)(lane + 64 * j) * rows];
   }
-  if (tid % 64 == 0) {
-    tops[0][tid / 64] = m;
-    tops[1][tid / 64] = mw;
-  }
-  __syncthreads();
-  m = __builtin_fmaxf(__builtin_fmaxf(tops[0][0], tops[0][1]), __builtin_fmaxf(tops[0][2], tops[0][3]));
-  mw = __builtin_fmaxf(__builtin_fmaxf(tops[1][0], tops[1][1]), __builtin_fmaxf(tops[1][2], tops[1][3]));
-  float l = mine.y * __builtin_amdgcn_exp2f(mine.x - m);
 #pragma unroll
-  for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
-  if (tid % 64 == 0) total[tid / 64] = l;
-  scales[tid] = __builtin_amdgcn_exp2f(mine.z - mw);
-  __syncthreads();
-  l = (total[0] + total[1]) + (total[2] + total[3]);
+  for (int i = 0; i < AHEAD; ++i)
+    x[i] = o[(int64_t)min(tid / QUADS + i * GROUPS, parts - 1) * rows * QUADS];
+  // (every wave for itself: no barrier before the sums)
+  float m = NONE, mw = NONE, l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    m = __builtin_fmaxf(m, stat[j].x);
+    mw = __builtin_fmaxf(mw, stat[j].z);
+  }
+  m = wave_top(m);
+  mw = wave_top(mw);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    l += stat[j].y * __builtin_amdgcn_exp2f(stat[j].x - m);
+    scales[tid / 64][lane + 64 * j] = __builtin_amdgcn_exp2f(stat[j].z - mw);
+  }
+  l = wave_sum(l);
+  wave_sync_lds();
   if (tid < GROUPS * QUADS) {
     float4 y = make_float4(0, 0, 0, 0);
-    for (int p = tid / QUADS; p < parts; p += GROUPS) {
-      const float4 x = o[(int64_t)p * rows * QUADS + tid % QUADS];
-      const float f = scales[p];
-      y.x = __builtin_fmaf(x.x, f, y.x);
-      y.y = __builtin_fmaf(x.y, f, y.y);
-      y.z = __builtin_fmaf(x.z, f, y.z);
-      y.w = __builtin_fmaf(x.w, f, y.w);
-    }
+    auto add = [&](const float4 &v, int p) {
+      const float f = scales[tid / 64][p];
+      y.x = __builtin_fmaf(v.x, f, y.x);
+      y.y = __builtin_fmaf(v.y, f, y.y);
+      y.z = __builtin_fmaf(v.z, f, y.z);
+      y.w = __builtin_fmaf(v.w, f, y.w);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (tid / QUADS + i * GROUPS < parts) add(x[i], tid / QUADS + i * GROUPS);
+    for (int p = tid / QUADS + AHEAD * GROUPS; p < parts; p += GROUPS) add(o[(int64_t)p * rows * QUADS], p);
     sums[tid] = y;
   }
   __syncthreads();
   if (tid >= QUADS) return;
   float4 y = sums[tid];
+#pragma unroll
   for (int g = 1; g < GROUPS; ++g) {
-    const float4 x = sums[g * QUADS + tid];
-    y.x += x.x;
-    y.y += x.y;
-    y.z += x.z;
-    y.w += x.w;
+    const float4 z = sums[g * QUADS + tid];
+    y.x += z.x;
+    y.y += z.y;
+    y.z += z.z;
+    y.w += z.w;
   }
   const float scale = __builtin_amdgcn_exp2f(mw - m - 14.0f) / l;
-  float *out = a.out + (int64_t)(token - pos) * a.out_stride + (head * group + r % group) * HS + 4 * tid;
+  float *out = a.out + (int64_t)(token - pos) * a.out_stride + (head * group + r - mine * group) * HS + 4 * tid;
   *reinterpret_cast<float4 *>(out) = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
 }
 

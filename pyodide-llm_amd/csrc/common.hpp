@@ -138,6 +138,29 @@ __device__ __forceinline__ float wave_max32(float v) {
   return v;
 }
 
+// the wave's sum, and its largest (a NaN stays), in every lane: by DPP within rows of 16, their last lanes broadcast on
+template <class F>
+__device__ __forceinline__ float wave_all(float x, F f) {
+#define STEP(from, rows) \
+  f(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), from, rows, 0xF, false)))
+  x = STEP(0xB1, 0xF);   // lane ^ 1
+  x = STEP(0x4E, 0xF);   // lane ^ 2
+  x = STEP(0x141, 0xF);  // 8 lanes mirrored
+  x = STEP(0x140, 0xF);  // 16 mirrored: every lane holds its row's
+#undef STEP
+  const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 0)),
+              b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 16)),
+              c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 32)),
+              d = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 48));
+  return f(f(a, b), f(c, d));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return wave_all(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_top(float x) {
+  return wave_all(x, [](float a, float b) { return wmax(a, b); });
+}
+
 __device__ __forceinline__ float add32(float acc, const float4 v[8]) {
 #pragma unroll
   for (int u = 0; u < 8; ++u) {

@@ -61,8 +61,8 @@ class Model:
     def attention(self, q, pos, nh):
         """(out, bound) [count][nh][hs]: the attention in float64, and how far a float32 result may lie from it.
 
-        The bound, of a row with scores s and probabilities p: a query's digits are off by 1.5 / 8355000 of its largest
-        value (the rounding and the float32 product before it), float32 products and sums by 2^-23 each, so a score by
+        The bound, of a row with scores s and probabilities p: a query's digits are off by 0.5 / 4160000 of its largest
+        value (rounded once), float32 products and sums by 2^-23 each, so a score by
         ds <= 2^-22 max|q| max_j sum|k_j| / sqrt(hs) + 2^-21 max|s| (nats: combined, scaled, the maximum taken off); a
         probability by 2 ds + 2^-21 (the exponential, two halves of 11 bits); and the float32 sums of n terms, 16 a
         product, by (n / 16 + 32) 2^-24: all of it at most that part of max|v|, three times over for the division by
