@@ -107,22 +107,29 @@ struct Tile {
   }
 
   // the queries' digits: lane (row, half) holds channels 32 s + 16 half .. + 15 of step s. (Every load first, none behind a
-  // branch: one after the other they took 6 us.)
-  __device__ __forceinline__ void read_queries() {
+  // branch: one after the other they took 6 us. The first block's bytes are asked for right behind them.)
+  __device__ __forceinline__ void read_queries(const CacheView &c, int first) {
     float4 x[STEPS][4];
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int d = 32 * s + 16 * half;
-      const float4 *from = reinterpret_cast<const float4 *>(q + (HS % 32 == 0 || d < HS ? d : 0));
+    for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[s][j] = from[j];
+      for (int j = 0; j < 4; ++j) x[s][j] = make_float4(0, 0, 0, 0);
+    if (row) {  // (a column without a row asks for nothing: a wave's 1 KiB load takes 16 cycles of the CU's one port)
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        const int d = 32 * s + 16 * half;
+        if (HS % 32 && d >= HS) continue;
+        const float4 *from = reinterpret_cast<const float4 *>(q + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[s][j] = from[j];
+      }
     }
+    start(c, first);
     float largest = 0.0f;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (!row || (HS % 32 && 32 * s + 16 * half >= HS)) x[s][j] = make_float4(0, 0, 0, 0);
         largest = wmax(largest, wmax(wmax(__builtin_fabsf(x[s][j].x), __builtin_fabsf(x[s][j].y)),
                                      wmax(__builtin_fabsf(x[s][j].z), __builtin_fabsf(x[s][j].w))));
       }
@@ -158,31 +165,42 @@ struct Tile {
     return __builtin_amdgcn_exp2f(__builtin_fminf(m - mw + 14.0f, 126.0f));
   }
 
-  // blocks first, first + step, .. below to, by their 8-bit values
-  __device__ __forceinline__ void blocks(const CacheView &c, int first, int to, int step) {
-    if (first >= to) return;
+  // the bytes and scales of a block
+  i32x4 k[STEPS], v[TILES];
+  const int8_t *kp;
+  const uint8_t *vp;
+  const float2 *sp;
+  __device__ __forceinline__ void load_keys(int b) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      k[s] = (i32x4)(0);
+      if (HS % 32 == 0 || 32 * s + 16 * half < HS)
+        k[s] = *reinterpret_cast<const i32x4 *>(kp + (int64_t)b * (CACHE_BLOCK * HS) + s * (CACHE_BLOCK * 32));
+    }
+  }
+  __device__ __forceinline__ void load_values(int b) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      v[t] = (i32x4)(0);
+      if (HS % 32 == 0 || 32 * t + col < HS)
+        v[t] = *reinterpret_cast<const i32x4 *>(vp + (int64_t)b * (CACHE_BLOCK * HS) + t * (32 * CACHE_BLOCK));
+    }
+  }
+  // asks for the first block
+  __device__ __forceinline__ void start(const CacheView &c, int first) {
     const int64_t at = (int64_t)head * c.blocks;
-    const int8_t *kp = c.keys + at * (CACHE_BLOCK * HS) + half * (CACHE_BLOCK * 16) + col * 16;
-    const uint8_t *vp = c.values + at * (CACHE_BLOCK * HS) + col * CACHE_BLOCK + half * 16;
-    const float2 *sp = reinterpret_cast<const float2 *>(c.scales) + at;
-    // keys are read a block ahead (once the products have taken this block's), values while this block's scores are made
-    i32x4 k[STEPS], v[TILES];
-    auto load_keys = [&](int b) {
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        k[s] = (i32x4)(0);
-        if (HS % 32 == 0 || 32 * s + 16 * half < HS)
-          k[s] = *reinterpret_cast<const i32x4 *>(kp + (int64_t)b * (CACHE_BLOCK * HS) + s * (CACHE_BLOCK * 32));
-      }
-    };
+    kp = c.keys + at * (CACHE_BLOCK * HS) + half * (CACHE_BLOCK * 16) + col * 16;
+    vp = c.values + at * (CACHE_BLOCK * HS) + col * CACHE_BLOCK + half * 16;
+    sp = reinterpret_cast<const float2 *>(c.scales) + at;
     load_keys(first);
+    load_values(first);
+  }
+
+  // blocks first, first + step, .. below to, by their 8-bit values, once start(first) has run: each one's bytes are asked for
+  // once the products have taken those of the block before it
+  __device__ __forceinline__ void blocks(int first, int to, int step) {
     for (int b = first; b < to; b += step) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        v[t] = (i32x4)(0);
-        if (HS % 32 == 0 || 32 * t + col < HS)
-          v[t] = *reinterpret_cast<const i32x4 *>(vp + (int64_t)b * (CACHE_BLOCK * HS) + t * (32 * CACHE_BLOCK));
-      }
+      const int next = b + step < to ? b + step : b;  // (the last one again: no use of it)
       const float2 scale = sp[b];
       i32x16 s0 = (i32x16)(0), s1 = (i32x16)(0), s2 = (i32x16)(0);
 #pragma unroll
@@ -192,7 +210,7 @@ struct Tile {
         s2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q2[s], s2, 0, 0, 0);
       }
       const float ks = scale.x, vs = scale.y;
-      load_keys(b + step < to ? b + step : b);  // (the last one again: no use of it)
+      load_keys(next);
       const float each = from_digits * ks;
       float p[16], top = -__builtin_inff();
 #pragma unroll
@@ -230,6 +248,7 @@ struct Tile {
           o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, lo[s], o[t], 0, 0, 0);
         }
       }
+      load_values(next);
     }
   }
 
@@ -335,8 +354,10 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const Ca
   tile.head = blockIdx.y;
   tile.place(a, blockIdx.x * 4 + threadIdx.x / 64, tokens_log2);
   if (tile.first_token > tile.last_token) return;
-  tile.read_queries();
-  tile.blocks(a.rows.c, 0, tile.own, 1);
+  if (tile.own) {
+    tile.read_queries(a.rows.c, 0);
+    tile.blocks(0, tile.own, 1);
+  }
   tile.template own_block<1>(a, 0, nullptr);
   const Running &run = tile.run;
   const float sum = run.l + other_half(run.l);
@@ -380,8 +401,8 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
   } else {
     const int from = (int)((int64_t)tile.own * (part - 1) / splits), to = (int)((int64_t)tile.own * part / splits);
     if (from + wave < to) {
-      tile.read_queries();
-      tile.blocks(a.rows.c, from + wave, to, 4);
+      tile.read_queries(a.rows.c, from + wave);
+      tile.blocks(from + wave, to, 4);
     }
   }
   const Running &run = tile.run;
