@@ -54,15 +54,18 @@ __device__ __forceinline__ void widen(uint32_t w, f16x2 &a, f16x2 &b) {
   b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - bias;
 }
 
-// w in two halves, hi + lo = w to 22 bits, of two values at once. (The halves pass through a register that the compiler
-// does not see into: it would otherwise form the one for the product and the one that is taken off w by different
-// instructions, the product e * factor rounded once or twice, and leave an f16 step between them.)
+// w in two halves, hi + lo = w to 22 bits, of two values at once. (What is left of w is taken from the very register that
+// goes to the product: formed from w anew, by an instruction that rounds the exponential's product once or twice, the half
+// taken off could be an f16 step from the one kept.)
 __device__ __forceinline__ void split(float w0, float w1, f16x2 &hi, f16x2 &lo) {
   const f16x2 h = {(_Float16)w0, (_Float16)w1};
   uint32_t bits = __builtin_bit_cast(uint32_t, h);
+  float r0, r1;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(bits), "v"(w0));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(bits), "v"(w1));
   asm volatile("" : "+v"(bits));
   hi = __builtin_bit_cast(f16x2, bits);
-  lo = f16x2{(_Float16)(w0 - (float)hi[0]), (_Float16)(w1 - (float)hi[1])};
+  lo = f16x2{(_Float16)r0, (_Float16)r1};
 }
 
 // a row's running statistics: scores are in powers of two
@@ -150,9 +153,8 @@ struct Tile {
       }
   }
 
-  // the statistics after positions whose largest score is `top`, of values up to 2^bits: the factor of a probability in
-  // the products
-  __device__ __forceinline__ float advance(float top, float bits) {
+  // the statistics after positions whose largest score is `top`, of values up to 2^bits
+  __device__ __forceinline__ void advance(float top, float bits) {
     const float up = __builtin_ceilf(top), m = __builtin_fmaxf(run.m, up), mw = __builtin_fmaxf(run.mw, up + bits);
     run.l *= __builtin_amdgcn_exp2f(run.m - m);
     const float gamma = __builtin_amdgcn_exp2f(run.mw - mw);
@@ -162,7 +164,6 @@ struct Tile {
     }
     run.m = m;
     run.mw = mw;
-    return __builtin_amdgcn_exp2f(__builtin_fminf(m - mw + 14.0f, 126.0f));
   }
 
   // the bytes and scales of a block
@@ -202,39 +203,57 @@ struct Tile {
     for (int b = first; b < to; b += step) {
       const int next = b + step < to ? b + step : b;  // (the last one again: no use of it)
       const float2 scale = sp[b];
-      i32x16 s0 = (i32x16)(0), s1 = (i32x16)(0), s2 = (i32x16)(0);
+      // 256 (K d0) + K d1 in one accumulator, K d2 in another that starts at 1.5 * 2^23's bits and is read as a float
+      constexpr float MAGIC = 12582912.0f;
+      i32x16 s0 = (i32x16)(0), s2 = (i32x16)(0x4B400000);
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q0[s], s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q1[s], s1, 0, 0, 0);
-        s2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q2[s], s2, 0, 0, 0);
-      }
+      for (int s = 0; s < STEPS; ++s) s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q0[s], s0, 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) s2 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q2[s], s2, 0, 0, 0);
+      s0 <<= 8;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q1[s], s0, 0, 0, 0);
       const float ks = scale.x, vs = scale.y;
       load_keys(next);
+      // a score (in powers of two): each (p - MAGIC)
       const float each = from_digits * ks;
       float p[16], top = -__builtin_inff();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_fmaf((float)s0[r], 65536.0f, __builtin_fmaf((float)s1[r], 256.0f, (float)s2[r])) * each;
+        p[r] = __builtin_fmaf((float)s0[r], 256.0f, __int_as_float(s2[r]));
         top = __builtin_fmaxf(top, p[r]);
       }
       top = __builtin_fmaxf(top, other_half(top));
-      const float bits = vs > 0.0f ? (float)((int)(__float_as_uint(vs) >> 23) - 126) : -200.0f;
-      const float factor = advance(top, bits) * vs;
+      advance((top - MAGIC) * each, vs > 0.0f ? (float)((int)(__float_as_uint(vs) >> 23) - 126) : -200.0f);
+      // a probability comes with its block's value scale, 2^(score + log2 vs + 14 - mw), and goes to l with that taken back.
+      // Where the block's values lie 2^100 below the reference (or are zero) they are left out, and l takes 2^(score - m)
+      const float log_vs = __builtin_amdgcn_logf(vs), below = run.m - run.mw;
+      const bool tiny = log_vs + below < -100.0f;
+      const float scaled = tiny ? -below : log_vs, c = __builtin_fmaf(-MAGIC, each, scaled + 14.0f - run.mw);
       f16x8 hi[2], lo[2];
       float sum = 0.0f;
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(p[r] - run.m), e1 = __builtin_amdgcn_exp2f(p[r + 1] - run.m);
-        sum += e0 + e1;
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], each, c)),
+                    w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r + 1], each, c));
+        sum += w0;
+        sum += w1;
         f16x2 h, l;
-        split(e0 * factor, e1 * factor, h, l);
+        split(w0, w1, h, l);
         hi[r / 8][r % 8] = h[0];
         hi[r / 8][r % 8 + 1] = h[1];
         lo[r / 8][r % 8] = l[0];
         lo[r / 8][r % 8 + 1] = l[1];
       }
-      run.l += sum;
+      run.l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(-14.0f - scaled - below), run.l);
+      if (__any(tiny)) {
+        const f16x8 zero = (f16x8)((_Float16)0.0f);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          hi[s] = tiny ? zero : hi[s];
+          lo[s] = tiny ? zero : lo[s];
+        }
+      }
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         f16x2 h[8];
@@ -259,36 +278,54 @@ struct Tile {
   __device__ __forceinline__ void own_block(const CacheAttn &a, int part, float *shared) {
     const CacheView &c = a.rows.c;
     const int p0 = own * CACHE_BLOCK;
+    // the row of position p (this kv head's), for one that is not past the tile's last token
     auto source = [&](const float *x, const float *recent, int p) {
-      if (p >= pos) return x + (int64_t)(p - pos) * a.rows.x_stride + head * HS;
-      return recent + ((int64_t)(a.rows.displaced ? CACHE_RECENT + p % CACHE_BLOCK : p % CACHE_RECENT) * c.nkv + head) * HS;
+      const int kept = a.rows.displaced ? CACHE_RECENT + p % CACHE_BLOCK : p % CACHE_RECENT;
+      const int64_t at = p >= pos ? (int64_t)(p - pos) * a.rows.x_stride : (int64_t)(kept * c.nkv) * HS;
+      return (p >= pos ? x : recent) + at + head * HS;
     };
-    // (a shared block's values are asked for first: they come while its scores are made)
-    constexpr int MINE = PARTS > 1 ? (TILES + PARTS - 1) / PARTS : 1;
-    float x[MINE][16];
-    auto values = [&](int t, float (&to)[16]) {
-      const int d = HS % 32 == 0 || 32 * t + col < HS ? 32 * t + col : 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        to[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token))[d];
-    };
-    if (PARTS > 1) {
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) values(min(i * PARTS + part, TILES - 1), x[i]);
-    }
+    // every load first: the keys and queries, and a shared block's values, which come while its scores are made
+    constexpr int MINE = PARTS > 1 ? (TILES + PARTS - 1) / PARTS : 1, QUADS = (HS / 8 + PARTS - 1) / PARTS;
     const bool key = p0 + col <= last_token;
     const float *k = source(a.rows.k, c.recent_keys, key ? p0 + col : last_token) + half * (HS / 2);
     const float *qh = q + half * (HS / 2);
+    float x[MINE][16];
+    const float *from[16];
+    auto values = [&](int t, float (&to)[16]) {
+      const int d = HS % 32 == 0 || 32 * t + col < HS ? 32 * t + col : 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) to[r] = from[r][d];
+    };
     f32x16 s = (f32x16)(0.0f);
-#pragma unroll 4
-    for (int n = 0; n < (HS / 8 + PARTS - 1) / PARTS; ++n) {
-      const int i = 4 * (n * PARTS + part);
-      if (HS / 8 % PARTS && i >= HS / 2) break;  // (the same in the whole wave)
-      const float4 kk = *reinterpret_cast<const float4 *>(k + i), y = *reinterpret_cast<const float4 *>(qh + i);
+    auto scores = [&](const float4 &kk, const float4 &y) {
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.x, y.x, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.y, y.y, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.z, y.z, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.w, y.w, s, 0, 0, 0);
+    };
+    if (PARTS > 1) {
+      float4 kk[QUADS], y[QUADS];
+#pragma unroll
+      for (int n = 0; n < QUADS; ++n) {
+        const int i = 4 * min(n * PARTS + part, HS / 8 - 1);
+        kk[n] = *reinterpret_cast<const float4 *>(k + i);
+        y[n] = *reinterpret_cast<const float4 *>(qh + i);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        from[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token));
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) values(min(i * PARTS + part, TILES - 1), x[i]);
+#pragma unroll
+      for (int n = 0; n < QUADS; ++n)
+        if (HS / 8 % PARTS == 0 || n * PARTS + part < HS / 8) scores(kk[n], y[n]);  // (the same in the whole wave)
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < HS / 2; i += 4)
+        scores(*reinterpret_cast<const float4 *>(k + i), *reinterpret_cast<const float4 *>(qh + i));
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        from[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token));
     }
     if (PARTS > 1) {
 #pragma unroll
@@ -309,7 +346,8 @@ struct Tile {
       top = __builtin_fmaxf(top, p[r]);
     }
     top = __builtin_fmaxf(top, other_half(top));
-    const float factor = advance(top, 1.0f);
+    advance(top, 1.0f);
+    const float factor = __builtin_amdgcn_exp2f(__builtin_fminf(run.m - run.mw + 14.0f, 126.0f));
     float sum = 0.0f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -347,12 +385,17 @@ struct Tile {
   }
 };
 
-// Many tiles: one a wave, over all its blocks
+// Many tiles: one a wave, over all its blocks; a workgroup takes four in a row of one kv head (`fours` such workgroups a head). The
+// workgroups come by their length, longest first, in rounds of 256 that run to and fro, so that the two that a CU starts
+// with are a long one and a short one (taken by head and position, a 2048-token prompt's longest shared CUs: 138 us, now
+// 96).
 template <int HS>
-__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const CacheAttn a, int tokens_log2) {
+__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const CacheAttn a, int tokens_log2, int fours) {
   Tile<HS> tile;
-  tile.head = blockIdx.y;
-  tile.place(a, blockIdx.x * 4 + threadIdx.x / 64, tokens_log2);
+  const int round = blockIdx.x / 256, last = min(256, (int)gridDim.x - round * 256) - 1, at = blockIdx.x % 256;
+  const int rank = round * 256 + (round % 2 ? last - at : at);
+  tile.head = rank % a.rows.c.nkv;
+  tile.place(a, (fours - 1 - rank / a.rows.c.nkv) * 4 + threadIdx.x / 64, tokens_log2);
   if (tile.first_token > tile.last_token) return;
   if (tile.own) {
     tile.read_queries(a.rows.c, 0);
@@ -558,7 +601,8 @@ template <int HS>
 hipError_t launch(const CacheAttn &a, hipStream_t s) {
   const Layout l = layout_of(a);
   if (!l.most) {
-    hipLaunchKernelGGL(attend_kernel<HS>, dim3((l.tiles + 3) / 4, a.rows.c.nkv), dim3(256), 0, s, a, l.log2);
+    const int fours = (l.tiles + 3) / 4;
+    hipLaunchKernelGGL(attend_kernel<HS>, dim3(fours * a.rows.c.nkv), dim3(256), 0, s, a, l.log2, fours);
     return hipGetLastError();
   }
   const size_t bytes = std::max<size_t>(4 * l.rows * (HS + 4), 4 * 16 * 64) * sizeof(float);
