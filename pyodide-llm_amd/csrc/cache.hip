@@ -27,65 +27,89 @@ __device__ __forceinline__ int nearest_quotient(float x, float s) {
   return max(-127, min(127, (int)n));  // (past it only where the scale is a denormal of few bits)
 }
 
-// One (block, kv head, keys or values) a workgroup: the block's rows read once, kept in registers; a complete block's
-// largest magnitude gives its scale, its bytes go through LDS into the cache's order; the call's rows among the latest
-// 128 positions are copied. Bound by memory: each float32 value is read once, each byte written once.
+// where a block's bytes lie in LDS on their way into (and out of) the cache's order: a chunk of 16 channels of keys takes
+// 512 + 16 bytes, a channel of values 32 + 4, so that the lanes of a row, four channels apart, meet few others' banks
+__device__ __forceinline__ constexpr int key_at(int t, int d) { return d / 16 * 528 + t * 16 + d % 16; }
+__device__ __forceinline__ constexpr int value_at(int byte, int d) { return d * 36 + byte; }
+template <int HS>
+constexpr int lds_bytes() { return HS * 36; }
+
+// One (block, kv head, keys or values) a workgroup; a thread takes four positions of four channels, so that keys leave it as
+// a word a position and values as a word a channel. The block's rows are read once and kept in registers; a complete
+// block's largest magnitude gives its scale, its bytes go through LDS into the cache's order; the call's rows among the
+// latest 128 positions are copied. Bound by memory: each float32 value is read once, each byte written once.
 template <int HS>
 __global__ __launch_bounds__(256) void append_kernel(const CacheRows a) {
-  constexpr int QUADS = CACHE_BLOCK * HS / 4, EACH = (QUADS + 255) / 256;
+  constexpr int UNITS = CACHE_BLOCK / 4 * (HS / 4), EACH = (UNITS + 255) / 256;
   const int pos = a.dpos ? *a.dpos : a.pos, end = pos + a.count;
   const int block = pos / CACHE_BLOCK + blockIdx.x, head = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
   const int p0 = block * CACHE_BLOCK;
   const float *x = which ? a.v : a.k;
   float *recent = which ? a.c.recent_values : a.c.recent_keys;
   const bool whole = p0 + CACHE_BLOCK <= end;
-  float4 v[EACH];
+  float4 v[EACH][4];
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int f = tid + 256 * i, t = f / (HS / 4), d = f % (HS / 4) * 4, p = p0 + t;
-    v[i] = make_float4(0, 0, 0, 0);
-    if (QUADS % 256 && f >= QUADS) continue;
-    if (p < end && (whole || p >= pos))
-      v[i] = *reinterpret_cast<const float4 *>(row_of(a, x, recent, p, pos, head) + d);
-    top = wmax(top, wmax(wmax(__builtin_fabsf(v[i].x), __builtin_fabsf(v[i].y)),
-                         wmax(__builtin_fabsf(v[i].z), __builtin_fabsf(v[i].w))));
-  }
-  __shared__ float tops[4];
-  __shared__ alignas(16) uint8_t bytes[CACHE_BLOCK * HS];
-  if (whole) {  // (the same in the whole workgroup)
+    const int u = tid + 256 * i, t = u / (HS / 4) * 4, d = u % (HS / 4) * 4;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = wmax(top, __shfl_xor(top, o));
+    for (int r = 0; r < 4; ++r) {
+      const int p = p0 + t + r;
+      v[i][r] = make_float4(0, 0, 0, 0);
+      if ((UNITS % 256 == 0 || u < UNITS) && p < end && (whole || p >= pos))
+        v[i][r] = *reinterpret_cast<const float4 *>(row_of(a, x, recent, p, pos, head) + d);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      top = wmax(top, wmax(wmax(__builtin_fabsf(v[i][r].x), __builtin_fabsf(v[i][r].y)),
+                           wmax(__builtin_fabsf(v[i][r].z), __builtin_fabsf(v[i][r].w))));
+  __shared__ float tops[4];
+  __shared__ alignas(16) uint8_t bytes[lds_bytes<HS>()];
+  if (whole) {  // (the same in the whole workgroup)
+    top = wave_top(top);
     if (tid % 64 == 0) tops[tid / 64] = top;
     __syncthreads();
     const float s = wmax(wmax(tops[0], tops[1]), wmax(tops[2], tops[3])) * (1.0f / 127.0f);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      const int f = tid + 256 * i, t = f / (HS / 4), d = f % (HS / 4) * 4;
-      if (QUADS % 256 && f >= QUADS) continue;
-      const float in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      uint32_t packed = 0;
+      const int u = tid + 256 * i, t = u / (HS / 4) * 4, d = u % (HS / 4) * 4;
+      if (UNITS % 256 && u >= UNITS) continue;
+      uint32_t q[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int q = nearest_quotient(in[j], s);
-        if (which) bytes[(d + j) * CACHE_BLOCK + value_byte(t)] = (uint8_t)(q + 128);
-        else packed |= (uint32_t)(uint8_t)(int8_t)q << (8 * j);
+      for (int r = 0; r < 4; ++r) {
+        const float in[4] = {v[i][r].x, v[i][r].y, v[i][r].z, v[i][r].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[r][j] = (uint32_t)(nearest_quotient(in[j], s) + (which ? 128 : 0)) & 255u;
       }
-      if (!which) *reinterpret_cast<uint32_t *>(bytes + (d / 16 * CACHE_BLOCK + t) * 16 + d % 16) = packed;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<uint32_t *>(bytes + (which ? value_at(value_byte(t), d + r) : key_at(t + r, d))) =
+            which ? q[0][r] | q[1][r] << 8 | q[2][r] << 16 | q[3][r] << 24
+                  : q[r][0] | q[r][1] << 8 | q[r][2] << 16 | q[r][3] << 24;
     }
     __syncthreads();
     const int64_t at = (int64_t)head * a.c.blocks + block;
     uint8_t *out = (which ? a.c.values : reinterpret_cast<uint8_t *>(a.c.keys)) + at * (CACHE_BLOCK * HS);
-    for (int i = tid; i < CACHE_BLOCK * HS / 16; i += 256)
-      reinterpret_cast<uint4 *>(out)[i] = reinterpret_cast<const uint4 *>(bytes)[i];
+    for (int i = tid; i < CACHE_BLOCK * HS / 16; i += 256) {
+      const uint32_t *from = reinterpret_cast<const uint32_t *>(
+          bytes + (which ? value_at(i % 2 * 16, i / 2) : key_at(i % CACHE_BLOCK, i / CACHE_BLOCK * 16)));
+      reinterpret_cast<uint4 *>(out)[i] = make_uint4(from[0], from[1], from[2], from[3]);
+    }
     if (tid == 0) a.c.scales[at * 2 + which] = s;
   }
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int f = tid + 256 * i, t = f / (HS / 4), d = f % (HS / 4) * 4, p = p0 + t;
-    if (QUADS % 256 && f >= QUADS) continue;
-    if (p >= pos && p < end && p >= end - CACHE_RECENT)
-      *reinterpret_cast<float4 *>(recent + ((int64_t)(p % CACHE_RECENT) * a.c.nkv + head) * HS + d) = v[i];
+    const int u = tid + 256 * i, t = u / (HS / 4) * 4, d = u % (HS / 4) * 4;
+    if (UNITS % 256 && u >= UNITS) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = p0 + t + r;
+      if (p >= pos && p < end && p >= end - CACHE_RECENT)
+        *reinterpret_cast<float4 *>(recent + ((int64_t)(p % CACHE_RECENT) * a.c.nkv + head) * HS + d) = v[i][r];
+    }
   }
 }
 
@@ -99,35 +123,62 @@ __global__ __launch_bounds__(256) void set_apart_kernel(const CacheView c, int f
   }
 }
 
-// positions from.. as float32 rows: by their 8-bit values, those of block `recent_block` from the recent rows; into
-// k / v [count][n_kv * hs], or (k null) into the recent rows
-__global__ __launch_bounds__(256) void read_kernel(const CacheView c, float *k, float *v, int from, int recent_block) {
-  const int p = from + blockIdx.x, width = c.nkv * c.hs, block = p / CACHE_BLOCK, t = p % CACHE_BLOCK;
-  const int64_t recent = (int64_t)(p % CACHE_RECENT) * width;
-  for (int i = threadIdx.x; i < width; i += 256) {
-    const int head = i / c.hs, d = i % c.hs;
-    float kv, vv;
-    if (block != recent_block) {
-      const int64_t at = (int64_t)head * c.blocks + block, base = at * CACHE_BLOCK * c.hs;
-      kv = (float)c.keys[base + (d / 16 * CACHE_BLOCK + t) * 16 + d % 16] * c.scales[at * 2];
-      vv = (float)((int)c.values[base + (int64_t)d * CACHE_BLOCK + value_byte(t)] - 128) * c.scales[at * 2 + 1];
-    } else {
-      kv = c.recent_keys[recent + i];
-      vv = c.recent_values[recent + i];
+// One (block, kv head, keys or values) a workgroup: positions from..to - 1 of it as float32 rows, by their 8-bit values (read
+// in the cache's order, turned through LDS), those of block `recent_block` from the recent rows; into k / v
+// [to - from][n_kv * hs], or (null) into the recent rows
+template <int HS>
+__global__ __launch_bounds__(256) void read_kernel(const CacheView c, float *k, float *v, int from, int to,
+                                                   int recent_block) {
+  const int block = from / CACHE_BLOCK + blockIdx.x, head = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+  const int p0 = block * CACHE_BLOCK;
+  float *recent = which ? c.recent_values : c.recent_keys, *out = which ? v : k;
+  const bool eight = block != recent_block;
+  __shared__ alignas(16) uint8_t bytes[lds_bytes<HS>()];
+  float s = 0.0f;
+  if (eight) {  // (the same in the whole workgroup)
+    const int64_t at = (int64_t)head * c.blocks + block;
+    const uint8_t *in = (which ? c.values : reinterpret_cast<const uint8_t *>(c.keys)) + at * (CACHE_BLOCK * HS);
+    s = c.scales[at * 2 + which];
+    for (int i = tid; i < CACHE_BLOCK * HS / 16; i += 256) {
+      const uint4 w = reinterpret_cast<const uint4 *>(in)[i];
+      uint32_t *to_lds = reinterpret_cast<uint32_t *>(
+          bytes + (which ? value_at(i % 2 * 16, i / 2) : key_at(i % CACHE_BLOCK, i / CACHE_BLOCK * 16)));
+      to_lds[0] = w.x;
+      to_lds[1] = w.y;
+      to_lds[2] = w.z;
+      to_lds[3] = w.w;
     }
-    if (k) {
-      k[(int64_t)blockIdx.x * width + i] = kv;
-      v[(int64_t)blockIdx.x * width + i] = vv;
+    __syncthreads();
+  }
+  for (int f = tid; f < CACHE_BLOCK * (HS / 4); f += 256) {
+    const int t = f / (HS / 4), d = f % (HS / 4) * 4, p = p0 + t;
+    if (p < from || p >= to) continue;
+    float *kept = recent + ((int64_t)(p % CACHE_RECENT) * c.nkv + head) * HS + d;
+    float4 y;
+    if (!eight) {
+      y = *reinterpret_cast<const float4 *>(kept);
+    } else if (which) {
+      const uint8_t *b = bytes + value_at(value_byte(t), d);
+      y = make_float4((float)((int)b[0] - 128) * s, (float)((int)b[36] - 128) * s, (float)((int)b[72] - 128) * s,
+                      (float)((int)b[108] - 128) * s);
     } else {
-      c.recent_keys[recent + i] = kv;
-      c.recent_values[recent + i] = vv;
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(bytes + key_at(t, d));
+      y = make_float4((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s,
+                      (float)(int8_t)(w >> 24) * s);
     }
+    float *to_row = out ? out + ((int64_t)(p - from) * c.nkv + head) * HS + d : kept;
+    *reinterpret_cast<float4 *>(to_row) = y;
   }
 }
 
 template <int HS>
 void launch_append(const CacheRows &a, int blocks, hipStream_t s) {
   hipLaunchKernelGGL(append_kernel<HS>, dim3(blocks, a.c.nkv, 2), dim3(256), 0, s, a);
+}
+template <int HS>
+void launch_read(const CacheView &c, float *k, float *v, int from, int to, int recent, hipStream_t s) {
+  hipLaunchKernelGGL(read_kernel<HS>, dim3((to - 1) / CACHE_BLOCK - from / CACHE_BLOCK + 1, c.nkv, 2), dim3(256), 0, s, c, k,
+                     v, from, to, recent);
 }
 
 }  // namespace
@@ -154,7 +205,17 @@ hipError_t launch_cache_append(const CacheRows &rows, hipStream_t s) {
 
 hipError_t launch_cache_read(const CacheView &c, float *keys, float *values, int32_t from, int32_t count, int32_t recent,
                              hipStream_t s) {
-  hipLaunchKernelGGL(read_kernel, dim3(count), dim3(256), 0, s, c, keys, values, from, recent);
+  const int to = from + count;
+  switch (c.hs) {
+    case 16: launch_read<16>(c, keys, values, from, to, recent, s); break;
+    case 32: launch_read<32>(c, keys, values, from, to, recent, s); break;
+    case 48: launch_read<48>(c, keys, values, from, to, recent, s); break;
+    case 64: launch_read<64>(c, keys, values, from, to, recent, s); break;
+    case 96: launch_read<96>(c, keys, values, from, to, recent, s); break;
+    case 128: launch_read<128>(c, keys, values, from, to, recent, s); break;
+    case 256: launch_read<256>(c, keys, values, from, to, recent, s); break;
+    default: return hipErrorInvalidValue;
+  }
   return hipGetLastError();
 }
 

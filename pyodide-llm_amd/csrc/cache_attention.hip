@@ -201,7 +201,7 @@ struct Tile {
   // once the products have taken those of the block before it
   __device__ __forceinline__ void blocks(int first, int to, int step) {
     for (int b = first; b < to; b += step) {
-      const int next = b + step < to ? b + step : b;  // (the last one again: no use of it)
+      const int next = b + step < to ? b + step : b;  // (the last one again, unused: a branch around the reads cost 10%)
       const float2 scale = sp[b];
       // 256 (K d0) + K d1 in one accumulator, K d2 in another that starts at 1.5 * 2^23's bits and is read as a float
       constexpr float MAGIC = 12582912.0f;
@@ -385,28 +385,44 @@ struct Tile {
   }
 };
 
-// Many tiles: one a wave, over all its blocks; a workgroup takes four in a row of one kv head (`fours` such workgroups a head). The
-// workgroups come by their length, longest first, in rounds of 256 that run to and fro, so that the two that a CU starts
-// with are a long one and a short one (taken by head and position, a 2048-token prompt's longest shared CUs: 138 us, now
-// 96).
+// Many tiles: one a wave. A workgroup of eight waves (four where a head's 256 values take twice the registers) takes half as
+// many tiles in a row and as many as far from the end as these are from the start (`halves` such rows a kv head), so that
+// every workgroup, and every SIMD, has as many blocks to go over as the others: a tile's blocks grow with its position. With parts > 1 a workgroup takes one part in `parts` of its tiles'
+// blocks (the last the own block too) and leaves statistics and outputs in the workspace, as attend_part_kernel does.
+// Workgroups that the eight XCDs take in turn are of different kv heads, so that an XCD's L2 holds few heads' blocks.
 template <int HS>
-__global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const CacheAttn a, int tokens_log2, int fours) {
+constexpr int half_waves() { return HS <= 128 ? 4 : 2; }
+template <int HS>
+__global__ __launch_bounds__(128 * half_waves<HS>(), HS <= 128 ? 2 : 1) void attend_kernel(
+    const CacheAttn a, int tokens_log2, int rows, int tiles, int halves, int parts) {
+  constexpr int HALF = half_waves<HS>();
   Tile<HS> tile;
-  const int round = blockIdx.x / 256, last = min(256, (int)gridDim.x - round * 256) - 1, at = blockIdx.x % 256;
-  const int rank = round * 256 + (round % 2 ? last - at : at);
-  tile.head = rank % a.rows.c.nkv;
-  tile.place(a, (fours - 1 - rank / a.rows.c.nkv) * 4 + threadIdx.x / 64, tokens_log2);
-  if (tile.first_token > tile.last_token) return;
-  if (tile.own) {
-    tile.read_queries(a.rows.c, 0);
-    tile.blocks(0, tile.own, 1);
+  const int wave = threadIdx.x / 64, nkv = a.rows.c.nkv;
+  const int pair = blockIdx.x / nkv / parts, part = blockIdx.x / nkv % parts;
+  const int half = wave < HALF ? pair : halves - 1 - pair, index = half * HALF + wave % HALF;
+  if ((wave >= HALF && half == pair) || index >= tiles) return;  // (the middle row once; the last one's missing tiles)
+  tile.head = blockIdx.x % nkv;
+  tile.place(a, index, tokens_log2);
+  const int from = (int)((int64_t)tile.own * part / parts), to = (int)((int64_t)tile.own * (part + 1) / parts);
+  if (from < to) {
+    tile.read_queries(a.rows.c, from);
+    tile.blocks(from, to, 1);
   }
-  tile.template own_block<1>(a, 0, nullptr);
+  if (part == parts - 1) tile.template own_block<1>(a, 0, nullptr);
   const Running &run = tile.run;
   const float sum = run.l + other_half(run.l);
-  const float scale = __builtin_amdgcn_exp2f(run.mw - run.m - 14.0f) / sum;
-  if (!tile.row) return;
-  float *out = a.out + (int64_t)(tile.token - tile.pos) * a.out_stride + tile.qhead * HS;
+  if (tile.col >= rows || (parts == 1 && !tile.row)) return;
+  float scale = 1.0f, *out;
+  if (parts == 1) {
+    scale = __builtin_amdgcn_exp2f(run.mw - run.m - 14.0f) / sum;
+    out = a.out + (int64_t)(tile.token - tile.pos) * a.out_stride + tile.qhead * HS;
+  } else {
+    const int64_t at = (((int64_t)index * nkv + tile.head) * parts + part) * rows + tile.col;
+    out = a.workspace + at * HS;
+    if (tile.half == 0)
+      reinterpret_cast<float4 *>(a.workspace + (int64_t)tiles * nkv * parts * rows * HS)[at] =
+          make_float4(run.m, sum, run.mw, 0.0f);
+  }
 #pragma unroll
   for (int t = 0; t < Tile<HS>::TILES; ++t)
 #pragma unroll
@@ -417,6 +433,37 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_kernel(const Ca
         *reinterpret_cast<float4 *>(out + d) =
             make_float4(o[r] * scale, o[r + 1] * scale, o[r + 2] * scale, o[r + 3] * scale);
     }
+}
+
+// The few parts of many rows together: four values of a (tile row, kv head, tile) a thread
+template <int HS>
+__global__ __launch_bounds__(256) void attend_join_rows_kernel(const CacheAttn a, int tokens_log2, int rows, int tiles,
+                                                               int parts) {
+  constexpr int QUADS = HS / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, at = i / QUADS;  // (tile, kv head, row)
+  const int nkv = a.rows.c.nkv, quad = (int)(i % QUADS), r = (int)(at % rows), group = a.nh / nkv;
+  if (at >= (int64_t)tiles * nkv * rows) return;
+  const int64_t unit = at / rows;
+  const int tile = (int)(unit / nkv), head = (int)(unit % nkv), pos = a.rows.pos, mine = r / group;
+  const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + mine;
+  if (token < pos || token >= pos + a.rows.count) return;
+  const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (unit * parts * rows + r) * QUADS + quad;
+  const float4 *stats = reinterpret_cast<const float4 *>(a.workspace + (int64_t)tiles * nkv * parts * rows * HS) +
+                        unit * parts * rows + r;
+  float m = NONE, l = 0.0f, mw = NONE;
+  float4 y = make_float4(0, 0, 0, 0);
+  for (int p = 0; p < parts; ++p) {
+    const float4 x = o[(int64_t)p * rows * QUADS], s = stats[(int64_t)p * rows];
+    const float top = __builtin_fmaxf(m, s.x), high = __builtin_fmaxf(mw, s.z);
+    l = l * __builtin_amdgcn_exp2f(m - top) + s.y * __builtin_amdgcn_exp2f(s.x - top);
+    const float f = __builtin_amdgcn_exp2f(mw - high), g = __builtin_amdgcn_exp2f(s.z - high);
+    y = make_float4(y.x * f + x.x * g, y.y * f + x.y * g, y.z * f + x.z * g, y.w * f + x.w * g);
+    m = top;
+    mw = high;
+  }
+  const float scale = __builtin_amdgcn_exp2f(mw - m - 14.0f) / l;
+  float *out = a.out + (int64_t)(token - pos) * a.out_stride + (head * group + r - mine * group) * HS + 4 * quad;
+  *reinterpret_cast<float4 *>(out) = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
 }
 
 // the parts a tile's `own` earlier blocks are split into, of `most` at most: a block for each of a part's four waves at
@@ -448,6 +495,7 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
       tile.blocks(from + wave, to, 4);
     }
   }
+  // the four waves' outputs and statistics through LDS, put on one reference by the threads that add them
   const Running &run = tile.run;
   const float sum = run.l + other_half(run.l);
   if (tile.half == 0) {
@@ -455,17 +503,6 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
     stats[wave][tile.col][1] = sum;
     stats[wave][tile.col][2] = run.mw;
   }
-  __syncthreads();
-  // the four waves' statistics as one, and each wave's outputs on it
-  float m = NONE, l = 0.0f, mw = NONE;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    m = __builtin_fmaxf(m, stats[w][tile.col][0]);
-    mw = __builtin_fmaxf(mw, stats[w][tile.col][2]);
-  }
-#pragma unroll
-  for (int w = 0; w < 4; ++w) l += stats[w][tile.col][1] * __builtin_amdgcn_exp2f(stats[w][tile.col][0] - m);
-  const float scale = __builtin_amdgcn_exp2f(run.mw - mw);
   if (tile.col < rows) {
 #pragma unroll
     for (int t = 0; t < Tile<HS>::TILES; ++t)
@@ -475,25 +512,38 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
         const f32x16 &o = tile.o[t];
         if (HS % 32 == 0 || d < HS)
           *reinterpret_cast<float4 *>(shared + (wave * rows + tile.col) * STRIDE + d) =
-              make_float4(o[r] * scale, o[r + 1] * scale, o[r + 2] * scale, o[r + 3] * scale);
+              make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
       }
   }
   __syncthreads();
   const int64_t at = ((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * gridDim.x + part;
   float4 *const out = reinterpret_cast<float4 *>(a.workspace) + at * rows * (HS / 4);
   for (int i = threadIdx.x; i < rows * (HS / 4); i += 256) {
-    const float *x = shared + i / (HS / 4) * STRIDE + i % (HS / 4) * 4;
-    float4 y = *reinterpret_cast<const float4 *>(x);
+    const int row = i / (HS / 4);
+    const float *x = shared + row * STRIDE + i % (HS / 4) * 4;
+    float mw = NONE;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
+    for (int w = 0; w < 4; ++w) mw = __builtin_fmaxf(mw, stats[w][row][2]);
+    float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
       const float4 z = *reinterpret_cast<const float4 *>(x + w * rows * STRIDE);
-      y.x += z.x;
-      y.y += z.y;
-      y.z += z.z;
-      y.w += z.w;
+      const float f = __builtin_amdgcn_exp2f(stats[w][row][2] - mw);
+      y.x = __builtin_fmaf(z.x, f, y.x);
+      y.y = __builtin_fmaf(z.y, f, y.y);
+      y.z = __builtin_fmaf(z.z, f, y.z);
+      y.w = __builtin_fmaf(z.w, f, y.w);
     }
     out[i] = y;
   }
+  float m = NONE, l = 0.0f, mw = NONE;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    m = __builtin_fmaxf(m, stats[w][tile.col][0]);
+    mw = __builtin_fmaxf(mw, stats[w][tile.col][2]);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) l += stats[w][tile.col][1] * __builtin_amdgcn_exp2f(stats[w][tile.col][0] - m);
   if (threadIdx.x < rows)  // (wave 0: lane = column)
     (reinterpret_cast<float4 *>(a.workspace) + (int64_t)gridDim.x * gridDim.y * gridDim.z * rows * (HS / 4))[
         at * rows + tile.col] = make_float4(m, l, mw, 0.0f);
@@ -573,27 +623,33 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
 }
 
 // How a call is laid out: the tokens a tile takes (2^log2: the largest power of two whose rows, token and query head, are at
-// most 32, so that tiles, which start at its multiples, never straddle two blocks), and the most parts a tile's blocks are
-// split into where there are too few tiles for the card's 1024 SIMDs (0: one wave a tile)
+// most 32, so that tiles, which start at its multiples, never straddle two blocks); with many tiles (at least FEW waves of
+// them) one a wave, their blocks in `parts`; with few, each tile's blocks in at most `most` parts
 struct Layout {
-  int log2, rows, tiles, most;
+  int log2, rows, tiles, most, parts;
 };
 constexpr int PARTS_MOST = 255;  // parts that attend_join_kernel takes, less the own block's
+constexpr int FEW = 192;
 int tokens_log2(int group) {
   int log2 = 0;
   while (log2 < 5 && (2 << log2) * group <= 32) ++log2;
   return log2;
 }
-int most_parts(int64_t waves) {
-  return waves >= 2048 ? 0 : (int)std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves);
+int most_parts(int64_t waves) { return (int)std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves); }
+// parts that fill the card's SIMDs with two waves (one where a head's 256 values take twice the registers), of two blocks at
+// least
+int tile_parts(int64_t waves, int hs, int blocks) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({16, (hs <= 128 ? 2048 : 1024) / waves, blocks / 2}));
 }
 Layout layout_of(const CacheAttn &a) {
   Layout l;
-  const int group = a.nh / a.rows.c.nkv;
+  const int group = a.nh / a.rows.c.nkv, last = a.rows.pos + a.rows.count - 1;
   l.log2 = tokens_log2(group);
   l.rows = group << l.log2;
-  l.tiles = ((a.rows.pos + a.rows.count - 1) >> l.log2) - (a.rows.pos >> l.log2) + 1;
-  l.most = most_parts((int64_t)l.tiles * a.rows.c.nkv);
+  l.tiles = (last >> l.log2) - (a.rows.pos >> l.log2) + 1;
+  const int64_t waves = (int64_t)l.tiles * a.rows.c.nkv;
+  l.most = waves < FEW ? most_parts(waves) : 0;
+  l.parts = tile_parts(waves, a.rows.c.hs, last / CACHE_BLOCK);
   return l;
 }
 
@@ -601,8 +657,14 @@ template <int HS>
 hipError_t launch(const CacheAttn &a, hipStream_t s) {
   const Layout l = layout_of(a);
   if (!l.most) {
-    const int fours = (l.tiles + 3) / 4;
-    hipLaunchKernelGGL(attend_kernel<HS>, dim3(fours * a.rows.c.nkv), dim3(256), 0, s, a, l.log2, fours);
+    const int halves = (l.tiles + half_waves<HS>() - 1) / half_waves<HS>();
+    hipLaunchKernelGGL(attend_kernel<HS>, dim3((halves + 1) / 2 * a.rows.c.nkv * l.parts), dim3(128 * half_waves<HS>()), 0, s,
+                       a, l.log2, l.rows, l.tiles, halves, l.parts);
+    if (l.parts > 1) {
+      const int64_t threads = (int64_t)l.tiles * a.rows.c.nkv * l.rows * (HS / 4);
+      hipLaunchKernelGGL(attend_join_rows_kernel<HS>, dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, a, l.log2,
+                         l.rows, l.tiles, l.parts);
+    }
     return hipGetLastError();
   }
   const size_t bytes = std::max<size_t>(4 * l.rows * (HS + 4), 4 * 16 * 64) * sizeof(float);
@@ -621,12 +683,17 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
 
 }  // namespace
 
-// (the most over the positions: the fewest tiles that count tokens make give the most parts, the most tiles the most rows)
+// (the most over the positions: count tokens make one tile more where they start inside one; the fewest make the most parts)
 int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count) {
   const int log2 = tokens_log2(nh / c.nkv);
-  const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2;
-  const int most = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4);
-  return most ? (fewest + 1) * c.nkv * (most + 1) * rows * (c.hs + 4) * (int64_t)sizeof(float) : 0;
+  const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2, most = fewest + 1;
+  int64_t parts = 0;
+  if (fewest * c.nkv < FEW) parts = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4) + 1;
+  if (most * c.nkv >= FEW) {
+    const int p = tile_parts(std::max<int64_t>(FEW, fewest * c.nkv), c.hs, c.blocks);
+    parts = std::max<int64_t>(parts, p > 1 ? p : 0);
+  }
+  return most * c.nkv * parts * rows * (c.hs + 4) * (int64_t)sizeof(float);
 }
 
 hipError_t launch_cache_attention(const CacheAttn &args, hipStream_t s) {
