@@ -14,18 +14,28 @@ __device__ __forceinline__ const float *row_of(const CacheRows &a, const float *
   return recent + ((int64_t)row * a.c.nkv + head) * a.c.hs;
 }
 
-// q = x / s rounded to the nearest integer, ties to even, exactly: the float32 quotient is off by half a step of its own
-// at most, so its nearest integer n is the answer or next to it, and x - n s is exact in one fma (n s has 31 bits and
-// lies within s of x), so that comparing twice it with s decides
-__device__ __forceinline__ int nearest_quotient(float x, float s) {
-  if (!(s > 0.0f) || !(s < __builtin_inff())) return 0;  // (a scale that is not finite stands for what is not a number)
-  float n = __builtin_rintf(x / s);
-  const float over = __builtin_fmaf(-n, s, x), twice = over + over;
-  const bool odd = ((int)n & 1) != 0;
-  if (twice > s || (twice == s && odd)) n += 1.0f;
-  else if (-twice > s || (-twice == s && odd)) n -= 1.0f;
-  return max(-127, min(127, (int)n));  // (past it only where the scale is a denormal of few bits)
-}
+// x / s rounded to the nearest integer, ties to even, exactly: x times 1 / s is off by 2^-22 of itself at most, so its nearest
+// integer n is the answer or next to it, and x - n s is exact in one fma (n s has 31 bits and lies within s of x), so that
+// comparing twice it with s decides. A scale that is next to nothing is taken up by 2^64 first, and x with it. (A
+// division for every value: 15.3 us for 2048 tokens of 8 heads of 128 in and out again; so 14.2.)
+struct Quotient {
+  float s, inverse, up;
+  bool none;
+  __device__ __forceinline__ explicit Quotient(float scale) {
+    none = !(scale > 0.0f) || !(scale < __builtin_inff());  // (a scale that is not finite stands for what is not a number)
+    up = scale < 0x1p-60f ? 0x1p64f : 1.0f;
+    s = scale * up;
+    inverse = 1.0f / s;
+  }
+  __device__ __forceinline__ int operator()(float x) const {
+    x *= up;
+    const float n = __builtin_rintf(x * inverse), over = __builtin_fmaf(-n, s, x), twice = over + over;
+    int q = (int)n;
+    const int odd = q & 1;
+    q += (twice > s) + (odd & (twice == s)) - (-twice > s) - (odd & (-twice == s));
+    return none ? 0 : max(-127, min(127, q));  // (past it only where the scale is a denormal of few bits)
+  }
+};
 
 // where a block's bytes lie in LDS on their way into (and out of) the cache's order: a chunk of 16 channels of keys takes
 // 512 + 16 bytes, a channel of values 32 + 4, so that the lanes of a row, four channels apart, meet few others' banks
@@ -73,6 +83,7 @@ __global__ __launch_bounds__(256) void append_kernel(const CacheRows a) {
     if (tid % 64 == 0) tops[tid / 64] = top;
     __syncthreads();
     const float s = wmax(wmax(tops[0], tops[1]), wmax(tops[2], tops[3])) * (1.0f / 127.0f);
+    const Quotient quotient(s);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int u = tid + 256 * i, t = u / (HS / 4) * 4, d = u % (HS / 4) * 4;
@@ -82,7 +93,7 @@ __global__ __launch_bounds__(256) void append_kernel(const CacheRows a) {
       for (int r = 0; r < 4; ++r) {
         const float in[4] = {v[i][r].x, v[i][r].y, v[i][r].z, v[i][r].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[r][j] = (uint32_t)(nearest_quotient(in[j], s) + (which ? 128 : 0)) & 255u;
+        for (int j = 0; j < 4; ++j) q[r][j] = (uint32_t)(quotient(in[j]) + (which ? 128 : 0)) & 255u;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
