@@ -340,7 +340,7 @@ int64_t hk_cache_workspace(const hk_cache *cache, int32_t n_heads, int32_t count
 
 /* Positions from..from + count - 1 as a token at position end (from + count <= end) would read them: those before end's
  * block by their 8-bit values, that block's by their float32 rows; keys and values float32
- * [count][n_kv_heads * head_size]. */
+ * [count][n_kv_heads * head_size], 16-byte aligned. */
 int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t from, int32_t count, int32_t end,
                       void *stream);
 

@@ -127,7 +127,8 @@ int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t f
   int32_t rc = view_of("hk_cache_read", cache, v);
   if (!rc) rc = buffers_of("hk_cache_read", v);
   if (rc) return rc;
-  if (!keys || !values) return failed(HE_E_ARG, "hk_cache_read: a required pointer is null");
+  if (!keys || !values || !aligned(keys) || !aligned(values))
+    return failed(HE_E_ARG, "hk_cache_read: keys or values is null or not 16-byte aligned");
   if (from < 0 || count < 0 || (int64_t)from + count > end || end > cache->seq_len)
     return failed(HE_E_ARG, "hk_cache_read: positions out of range");
   if (count == 0) return HE_OK;

@@ -95,3 +95,10 @@ def test_log_probabilities_that_are_refused(change, text):
                 n_given=1, m=2, n=100, top=3, workspace=1 << 26, size=1 << 30)
     args.update(change)
     refused(package().library().hk_logprobs(*args.values(), None), text=text)
+
+
+@pytest.mark.parametrize("change", [dict(keys=(1 << 20) + 4), dict(values=(1 << 21) + 8)])
+def test_reads_into_rows_that_are_not_aligned(change):
+    to = dict(keys=1 << 20, values=1 << 21)
+    to.update(change)
+    refused(package().library().hk_cache_read(to["keys"], to["values"], ctypes.byref(cache()), 0, 4, 8, None), text=b"16-byte")
