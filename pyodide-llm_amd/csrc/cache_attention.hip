@@ -271,32 +271,40 @@ struct Tile {
     }
   }
 
-  // the tile's own block by its float32 rows, up to the tile's last token, on float32 MFMA. PARTS waves share it (wave
+  // The tile's own block by its float32 rows, up to the tile's last token, on float32 MFMA. PARTS waves share it (wave
   // `part`): each takes its share of the channels of the products of keys and queries, whose parts are added through
-  // `shared` (PARTS x 64 x 16 floats), and of the output's; the sums of probabilities count with part 0
+  // `shared` (PARTS x 64 x 16 floats; a barrier between own_scores and own_values), and of the output's; the sums of
+  // probabilities count with part 0
   template <int PARTS>
-  __device__ __forceinline__ void own_block(const CacheAttn &a, int part, float *shared) {
-    const CacheView &c = a.rows.c;
-    const int p0 = own * CACHE_BLOCK;
-    // the row of position p (this kv head's), for one that is not past the tile's last token
-    auto source = [&](const float *x, const float *recent, int p) {
-      const int kept = a.rows.displaced ? CACHE_RECENT + p % CACHE_BLOCK : p % CACHE_RECENT;
-      const int64_t at = p >= pos ? (int64_t)(p - pos) * a.rows.x_stride : (int64_t)(kept * c.nkv) * HS;
-      return (p >= pos ? x : recent) + at + head * HS;
-    };
-    // every load first: the keys and queries, and a shared block's values, which come while its scores are made
-    constexpr int MINE = PARTS > 1 ? (TILES + PARTS - 1) / PARTS : 1, QUADS = (HS / 8 + PARTS - 1) / PARTS;
-    const bool key = p0 + col <= last_token;
-    const float *k = source(a.rows.k, c.recent_keys, key ? p0 + col : last_token) + half * (HS / 2);
-    const float *qh = q + half * (HS / 2);
-    float x[MINE][16];
-    const float *from[16];
-    auto values = [&](int t, float (&to)[16]) {
-      const int d = HS % 32 == 0 || 32 * t + col < HS ? 32 * t + col : 0;
+  static constexpr int mine() {
+    return PARTS > 1 ? (TILES + PARTS - 1) / PARTS : 1;
+  }
+  // the row of position p (this kv head's), for one that is not past the tile's last token
+  __device__ __forceinline__ const float *source(const CacheAttn &a, const float *x, const float *recent, int p) const {
+    const int kept = a.rows.displaced ? CACHE_RECENT + p % CACHE_BLOCK : p % CACHE_RECENT;
+    const int64_t at = p >= pos ? (int64_t)(p - pos) * a.rows.x_stride : (int64_t)(kept * a.rows.c.nkv) * HS;
+    return (p >= pos ? x : recent) + at + head * HS;
+  }
+  __device__ __forceinline__ void value_rows(const CacheAttn &a, const float *(&from)[16]) const {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) to[r] = from[r][d];
-    };
-    f32x16 s = (f32x16)(0.0f);
+    for (int r = 0; r < 16; ++r)
+      from[r] = source(a, a.rows.v, a.rows.c.recent_values,
+                       min(own * CACHE_BLOCK + 8 * (r / 4) + 4 * half + r % 4, last_token));
+  }
+  __device__ __forceinline__ void values(int t, const float *const (&from)[16], float (&to)[16]) const {
+    const int d = HS % 32 == 0 || 32 * t + col < HS ? 32 * t + col : 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) to[r] = from[r][d];
+  }
+  template <int PARTS>
+  __device__ __forceinline__ void own_scores(const CacheAttn &a, int part, float *shared, float (&x)[mine<PARTS>()][16],
+                                             f32x16 &s) const {
+    // every load first: the keys and queries, and a shared block's values, which come while its scores are made
+    constexpr int QUADS = (HS / 8 + PARTS - 1) / PARTS;
+    const int key = min(own * CACHE_BLOCK + col, last_token);
+    const float *k = source(a, a.rows.k, a.rows.c.recent_keys, key) + half * (HS / 2);
+    const float *qh = q + half * (HS / 2);
+    s = (f32x16)(0.0f);
     auto scores = [&](const float4 &kk, const float4 &y) {
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.x, y.x, s, 0, 0, 0);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(kk.y, y.y, s, 0, 0, 0);
@@ -311,26 +319,26 @@ struct Tile {
         kk[n] = *reinterpret_cast<const float4 *>(k + i);
         y[n] = *reinterpret_cast<const float4 *>(qh + i);
       }
+      const float *from[16];
+      value_rows(a, from);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        from[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token));
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) values(min(i * PARTS + part, TILES - 1), x[i]);
+      for (int i = 0; i < mine<PARTS>(); ++i) values(min(i * PARTS + part, TILES - 1), from, x[i]);
 #pragma unroll
       for (int n = 0; n < QUADS; ++n)
         if (HS / 8 % PARTS == 0 || n * PARTS + part < HS / 8) scores(kk[n], y[n]);  // (the same in the whole wave)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) shared[(part * 16 + r) * 64 + lane] = s[r];
     } else {
 #pragma unroll 4
       for (int i = 0; i < HS / 2; i += 4)
         scores(*reinterpret_cast<const float4 *>(k + i), *reinterpret_cast<const float4 *>(qh + i));
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        from[r] = source(a.rows.v, c.recent_values, min(p0 + 8 * (r / 4) + 4 * half + r % 4, last_token));
     }
+  }
+  template <int PARTS>
+  __device__ __forceinline__ void own_values(const CacheAttn &a, int part, const float *shared,
+                                             float (&x)[mine<PARTS>()][16], f32x16 &s) {
+    const int p0 = own * CACHE_BLOCK;
     if (PARTS > 1) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) shared[(part * 16 + r) * 64 + lane] = s[r];
-      __syncthreads();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[r] = shared[r * 64 + lane];
@@ -358,11 +366,13 @@ struct Tile {
     // a value that is not finite is left out of the product (which would carry it to rows that do not see it) and makes the
     // rows that see it not a number
     uint32_t strange = 0;  // bit r: this lane's value of its position r is not finite
+    const float *from[16];
+    if (PARTS == 1) value_rows(a, from);
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       if (PARTS > 1 && t % PARTS != part) continue;  // (the same in the whole wave)
       float(&v)[16] = x[PARTS > 1 ? t / PARTS : 0];
-      if (PARTS == 1) values(t, v);
+      if (PARTS == 1) values(t, from, v);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = p0 + 8 * (r / 4) + 4 * half + r % 4;
@@ -387,8 +397,9 @@ struct Tile {
 
 // Many tiles: one a wave. A workgroup of eight waves (four where a head's 256 values take twice the registers) takes half as
 // many tiles in a row and as many as far from the end as these are from the start (`halves` such rows a kv head), so that
-// every workgroup, and every SIMD, has as many blocks to go over as the others: a tile's blocks grow with its position. With parts > 1 a workgroup takes one part in `parts` of its tiles'
-// blocks (the last the own block too) and leaves statistics and outputs in the workspace, as attend_part_kernel does.
+// every workgroup, and every SIMD, has as many blocks to go over as the others: a tile's blocks grow with its position. With
+// parts > 1 a workgroup takes one part in `parts` of its tiles' blocks (the last the own block too) and leaves statistics and
+// outputs in the workspace, as attend_part_kernel does.
 // Workgroups that the eight XCDs take in turn are of different kv heads, so that an XCD's L2 holds few heads' blocks.
 template <int HS>
 constexpr int half_waves() { return HS <= 128 ? 4 : 2; }
@@ -408,7 +419,12 @@ __global__ __launch_bounds__(128 * half_waves<HS>(), HS <= 128 ? 2 : 1) void att
     tile.read_queries(a.rows.c, from);
     tile.blocks(from, to, 1);
   }
-  if (part == parts - 1) tile.template own_block<1>(a, 0, nullptr);
+  if (part == parts - 1) {
+    float x[1][16];
+    f32x16 scores;
+    tile.template own_scores<1>(a, 0, nullptr, x, scores);
+    tile.template own_values<1>(a, 0, nullptr, x, scores);
+  }
   const Running &run = tile.run;
   const float sum = run.l + other_half(run.l);
   if (tile.col >= rows || (parts == 1 && !tile.row)) return;
@@ -486,7 +502,11 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
   const int splits = parts_of(tile.own, most);
   if (part > splits) return;  // (the whole workgroup)
   if (part == 0) {
-    tile.template own_block<4>(a, wave, shared);
+    float x[Tile<HS>::template mine<4>()][16];
+    f32x16 scores;
+    tile.template own_scores<4>(a, wave, shared, x, scores);
+    __syncthreads();
+    tile.template own_values<4>(a, wave, shared, x, scores);
     __syncthreads();  // (shared holds the outputs next)
   } else {
     const int from = (int)((int64_t)tile.own * (part - 1) / splits), to = (int)((int64_t)tile.own * part / splits);
@@ -547,6 +567,78 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
   if (threadIdx.x < rows)  // (wave 0: lane = column)
     (reinterpret_cast<float4 *>(a.workspace) + (int64_t)gridDim.x * gridDim.y * gridDim.z * rows * (HS / 4))[
         at * rows + tile.col] = make_float4(m, l, mw, 0.0f);
+}
+
+// One token over a short cache (short_cache): a workgroup of eight waves a kv head, four for the token's own block and four
+// for the earlier ones, whose outputs are put together through LDS: one launch in place of the parts and their join. By the
+// cache's size, not the token's position, which a launch may not know. At the end of a cache of 256, 512, 1024 positions, one
+// launch against the parts: 6 kv heads of 48 7.4, 9.0, 11.9 us against 8.8; 8 of 64 7.2, 8.5, 11.2 against 8.6; 8 of 128 9.1,
+// 10.9, 14.5 against 9.1.
+constexpr bool short_cache(int blocks, int hs) { return blocks <= 16 && blocks * hs <= 1024; }
+template <int HS>
+__global__ __launch_bounds__(512, HS <= 128 ? 2 : 1) void attend_short_kernel(const CacheAttn a, int rows) {
+  extern __shared__ float4 lds[];
+  constexpr int STRIDE = HS + 4;
+  float *const shared = reinterpret_cast<float *>(lds), *const outputs = shared + 4 * 16 * 64;
+  __shared__ float stats[8][32][3];
+  const int wave = threadIdx.x / 64;
+  Tile<HS> tile;
+  tile.head = blockIdx.x;
+  tile.place(a, 0, 0);
+  float x[Tile<HS>::template mine<4>()][16];
+  f32x16 scores;
+  if (wave < 4) {
+    tile.template own_scores<4>(a, wave, shared, x, scores);
+  } else if (wave - 4 < tile.own) {
+    tile.read_queries(a.rows.c, wave - 4);
+    tile.blocks(wave - 4, tile.own, 4);
+  }
+  __syncthreads();
+  if (wave < 4) tile.template own_values<4>(a, wave, shared, x, scores);
+  const Running &run = tile.run;
+  const float sum = run.l + other_half(run.l);
+  if (tile.half == 0) {
+    stats[wave][tile.col][0] = run.m;
+    stats[wave][tile.col][1] = sum;
+    stats[wave][tile.col][2] = run.mw;
+  }
+  if (tile.col < rows) {
+#pragma unroll
+    for (int t = 0; t < Tile<HS>::TILES; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * t + 8 * (r / 4) + 4 * tile.half;
+        const f32x16 &o = tile.o[t];
+        if (HS % 32 == 0 || d < HS)
+          *reinterpret_cast<float4 *>(outputs + (wave * rows + tile.col) * STRIDE + d) =
+              make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (HS / 4); i += 512) {
+    const int row = i / (HS / 4);
+    const float *from = outputs + row * STRIDE + i % (HS / 4) * 4;
+    float m = NONE, mw = NONE, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      m = __builtin_fmaxf(m, stats[w][row][0]);
+      mw = __builtin_fmaxf(mw, stats[w][row][2]);
+    }
+    float4 y = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float4 z = *reinterpret_cast<const float4 *>(from + w * rows * STRIDE);
+      const float f = __builtin_amdgcn_exp2f(stats[w][row][2] - mw);
+      l += stats[w][row][1] * __builtin_amdgcn_exp2f(stats[w][row][0] - m);
+      y.x = __builtin_fmaf(z.x, f, y.x);
+      y.y = __builtin_fmaf(z.y, f, y.y);
+      y.z = __builtin_fmaf(z.z, f, y.z);
+      y.w = __builtin_fmaf(z.w, f, y.w);
+    }
+    const float scale = __builtin_amdgcn_exp2f(mw - m - 14.0f) / l;
+    float *out = a.out + ((int)blockIdx.x * rows + row) * HS + i % (HS / 4) * 4;
+    *reinterpret_cast<float4 *>(out) = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
+  }
 }
 
 // A row's parts together: one (tile row, kv head, tile) a workgroup
@@ -623,16 +715,17 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
 }
 
 // How a call is laid out: the tokens a tile takes (2^log2: the largest power of two whose rows, token and query head, are at
-// most 32, so that tiles, which start at its multiples, never straddle two blocks); with many tiles (at least FEW waves of
-// them) one a wave, their blocks in `parts`; with few, each tile's blocks in at most `most` parts
+// most 32, and no larger than the call needs; tiles start at its multiples, so that none straddles two blocks); with many tiles
+// (at least FEW waves of them) one a wave, their blocks in `parts`; with few, and for a single token, whose position the launch
+// may not know, each tile's blocks in at most `most` parts
 struct Layout {
   int log2, rows, tiles, most, parts;
 };
 constexpr int PARTS_MOST = 255;  // parts that attend_join_kernel takes, less the own block's
 constexpr int FEW = 192;
-int tokens_log2(int group) {
+int tokens_log2(int group, int count) {
   int log2 = 0;
-  while (log2 < 5 && (2 << log2) * group <= 32) ++log2;
+  while (log2 < 5 && (2 << log2) * group <= 32 && 1 << log2 < count) ++log2;
   return log2;
 }
 int most_parts(int64_t waves) { return (int)std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves); }
@@ -644,11 +737,11 @@ int tile_parts(int64_t waves, int hs, int blocks) {
 Layout layout_of(const CacheAttn &a) {
   Layout l;
   const int group = a.nh / a.rows.c.nkv, last = a.rows.pos + a.rows.count - 1;
-  l.log2 = tokens_log2(group);
+  l.log2 = tokens_log2(group, a.rows.count);
   l.rows = group << l.log2;
   l.tiles = (last >> l.log2) - (a.rows.pos >> l.log2) + 1;
   const int64_t waves = (int64_t)l.tiles * a.rows.c.nkv;
-  l.most = waves < FEW ? most_parts(waves) : 0;
+  l.most = waves < FEW || a.rows.count == 1 ? most_parts(waves) : 0;
   l.parts = tile_parts(waves, a.rows.c.hs, last / CACHE_BLOCK);
   return l;
 }
@@ -656,6 +749,14 @@ Layout layout_of(const CacheAttn &a) {
 template <int HS>
 hipError_t launch(const CacheAttn &a, hipStream_t s) {
   const Layout l = layout_of(a);
+  const int last = (a.rows.pos + a.rows.count - 1) / CACHE_BLOCK;
+  if constexpr (HS <= 128) {
+    const size_t bytes = (4 * 16 * 64 + 8 * l.rows * (HS + 4)) * sizeof(float);
+    if (a.rows.count == 1 && short_cache(a.rows.c.blocks, HS) && bytes <= 65536 - 4096) {  // (and `stats`)
+      hipLaunchKernelGGL(attend_short_kernel<HS>, dim3(a.rows.c.nkv), dim3(512), bytes, s, a, l.rows);
+      return hipGetLastError();
+    }
+  }
   if (!l.most) {
     const int halves = (l.tiles + half_waves<HS>() - 1) / half_waves<HS>();
     hipLaunchKernelGGL(attend_kernel<HS>, dim3((halves + 1) / 2 * a.rows.c.nkv * l.parts), dim3(128 * half_waves<HS>()), 0, s,
@@ -673,7 +774,7 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (err != hipSuccess) return err;
   }
-  const int last = (a.rows.pos + a.rows.count - 1) / CACHE_BLOCK, stride = std::max(1, std::min(l.most, (last + 3) / 4)) + 1;
+  const int stride = std::max(1, std::min(l.most, (last + 3) / 4)) + 1;
   hipLaunchKernelGGL(attend_part_kernel<HS>, dim3(stride, l.tiles, a.rows.c.nkv), dim3(256), bytes, s, a, l.log2, l.rows,
                      l.most);
   hipLaunchKernelGGL(attend_join_kernel<HS>, dim3(l.rows, a.rows.c.nkv, l.tiles), dim3(256), 0, s, a, l.log2, l.rows,
@@ -685,11 +786,12 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
 
 // (the most over the positions: count tokens make one tile more where they start inside one; the fewest make the most parts)
 int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count) {
-  const int log2 = tokens_log2(nh / c.nkv);
-  const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2, most = fewest + 1;
+  const int log2 = tokens_log2(nh / c.nkv, count);
+  const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2;
+  const int64_t most = fewest + (count > 1);
   int64_t parts = 0;
-  if (fewest * c.nkv < FEW) parts = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4) + 1;
-  if (most * c.nkv >= FEW) {
+  if (fewest * c.nkv < FEW || count == 1) parts = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4) + 1;
+  if (most * c.nkv >= FEW && count > 1) {
     const int p = tile_parts(std::max<int64_t>(FEW, fewest * c.nkv), c.hs, c.blocks);
     parts = std::max<int64_t>(parts, p > 1 ? p : 0);
   }

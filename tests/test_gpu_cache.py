@@ -369,3 +369,16 @@ def test_a_conversation_with_its_probabilities():
         np.testing.assert_array_equal(ids.numpy()[:, 0], out.reshape(c, -1).argmax(-1))
         np.testing.assert_allclose(logps.numpy()[:, 0], x.max(-1) - lse, atol=1e-4, rtol=0)  # (the bound of `within`)
         pos += c
+
+
+@pytest.mark.parametrize("nh, nkv, hs", [(200, 200, 16), (400, 200, 32)])
+@pytest.mark.parametrize("pos, count", [(700, 1), (690, 2), (500, 9)])
+def test_attention_of_few_tokens_with_many_kv_heads(nh, nkv, hs, pos, count):
+    """as many tiles as waves fill the card with, from one token on"""
+    rng = np.random.default_rng(pos + nh)
+    cache, model = Cache(nkv, hs, pos + count), Model(nkv, hs, pos + count)
+    k, v = rows(rng, pos + count, nkv, hs)
+    cache.append(k, v, 0)
+    model.append(k, v, 0)
+    q = rng.standard_normal((count, nh * hs)).astype(np.float32)
+    within(cache.attention(q, k[pos:], v[pos:], pos, nh), model, q, pos, nh)
