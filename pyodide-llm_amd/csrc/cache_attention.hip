@@ -482,9 +482,18 @@ __global__ __launch_bounds__(256) void attend_join_rows_kernel(const CacheAttn a
   *reinterpret_cast<float4 *>(out) = make_float4(y.x * scale, y.y * scale, y.z * scale, y.w * scale);
 }
 
-// the parts a tile's `own` earlier blocks are split into, of `most` at most: a block for each of a part's four waves at
-// least. (By the tile alone, not by the launch, which may not know its position: the same sums either way.)
-__device__ __forceinline__ int parts_of(int own, int most) { return max(1, min(most, (own + 3) / 4)); }
+// The parts a tile's `own` earlier blocks are split into: a block for each of a part's four waves at least, and as many that
+// the launch is one workgroup a CU (`most`, most_parts; 257 workgroups take 3 us more than 256), or two where that leaves
+// waves more than eight blocks and the registers allow it. (By the tile alone, not by the launch, which may not know its
+// position: the same sums either way.) 8 kv heads of 128, a token behind 16k, 32k, 64k, 128k positions: one a CU 13.9, 18.3,
+// 34.6, 60.9 us, two 14.2, 18.7, 34.1, 57.7; of 256 values behind 32k, 64k: 35.7, 60.2, two 41.0, 66.5.
+constexpr int PARTS_MOST = 255;  // (attend_join_kernel takes one more, the own block's)
+template <int HS>
+__host__ __device__ inline int parts_of(int own, int most) {
+  if (HS <= 128 && own > 8 * 4 * most) most = most < PARTS_MOST / 2 ? 2 * most + 1 : PARTS_MOST;
+  const int parts = (own + 3) / 4;
+  return parts < 1 ? 1 : parts < most ? parts : most;
+}
 
 // Few tiles: the blocks of a tile in parts, one a workgroup, whose four waves take them in turn, and one part more for the
 // tile's own block (the first, which takes the longest). A part's statistics (m, l, mw) and outputs go to the
@@ -499,7 +508,7 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
   Tile<HS> tile;
   tile.head = blockIdx.z;
   tile.place(a, blockIdx.y, tokens_log2);
-  const int splits = parts_of(tile.own, most);
+  const int splits = parts_of<HS>(tile.own, most);
   if (part > splits) return;  // (the whole workgroup)
   if (part == 0) {
     float x[Tile<HS>::template mine<4>()][16];
@@ -653,7 +662,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
   const int mine = (int)(((float)r + 0.5f) * __builtin_amdgcn_rcpf((float)group));  // r / group
   const int token = (((pos >> tokens_log2) + tile) << tokens_log2) + mine;
   if (token < pos || token >= pos + a.rows.count) return;  // (the whole workgroup)
-  const int parts = parts_of(token / CACHE_BLOCK, most) + 1;
+  const int parts = parts_of<HS>(token / CACHE_BLOCK, most) + 1;
   const int64_t at = ((int64_t)tile * gridDim.y + head) * stride;
   const float4 *o = reinterpret_cast<const float4 *>(a.workspace) + (at * rows + r) * QUADS + tid % QUADS;
   const float4 *stats = reinterpret_cast<const float4 *>(a.workspace) + (int64_t)stride * gridDim.y * gridDim.z * rows * QUADS +
@@ -721,14 +730,14 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
 struct Layout {
   int log2, rows, tiles, most, parts;
 };
-constexpr int PARTS_MOST = 255;  // parts that attend_join_kernel takes, less the own block's
 constexpr int FEW = 192;
 int tokens_log2(int group, int count) {
   int log2 = 0;
   while (log2 < 5 && (2 << log2) * group <= 32 && 1 << log2 < count) ++log2;
   return log2;
 }
-int most_parts(int64_t waves) { return (int)std::min<int64_t>(PARTS_MOST, (2048 / 4 + waves - 1) / waves); }
+// (each tile's own block is a part more)
+int most_parts(int64_t waves) { return (int)std::min<int64_t>(PARTS_MOST, std::max<int64_t>(1, 256 / waves - 1)); }
 // parts that fill the card's SIMDs with two waves (one where a head's 256 values take twice the registers), of two blocks at
 // least
 int tile_parts(int64_t waves, int hs, int blocks) {
@@ -774,7 +783,7 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (err != hipSuccess) return err;
   }
-  const int stride = std::max(1, std::min(l.most, (last + 3) / 4)) + 1;
+  const int stride = parts_of<HS>(last, l.most) + 1;
   hipLaunchKernelGGL(attend_part_kernel<HS>, dim3(stride, l.tiles, a.rows.c.nkv), dim3(256), bytes, s, a, l.log2, l.rows,
                      l.most);
   hipLaunchKernelGGL(attend_join_kernel<HS>, dim3(l.rows, a.rows.c.nkv, l.tiles), dim3(256), 0, s, a, l.log2, l.rows,
@@ -784,18 +793,23 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
 
 }  // namespace
 
-// (the most over the positions: count tokens make one tile more where they start inside one; the fewest make the most parts)
+// (the most over the positions: count tokens make one tile more where they start inside one)
 int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count) {
   const int log2 = tokens_log2(nh / c.nkv, count);
   const int64_t rows = nh / c.nkv << log2, fewest = ((int64_t)count + (1 << log2) - 1) >> log2;
-  const int64_t most = fewest + (count > 1);
-  int64_t parts = 0;
-  if (fewest * c.nkv < FEW || count == 1) parts = std::min(most_parts(fewest * c.nkv), (c.blocks + 3) / 4) + 1;
-  if (most * c.nkv >= FEW && count > 1) {
-    const int p = tile_parts(std::max<int64_t>(FEW, fewest * c.nkv), c.hs, c.blocks);
-    parts = std::max<int64_t>(parts, p > 1 ? p : 0);
+  int64_t most = 0;
+  for (int64_t tiles = fewest; tiles <= fewest + (count > 1); ++tiles) {
+    const int64_t waves = tiles * c.nkv;
+    int64_t parts;
+    if (waves < FEW || count == 1) {
+      parts = (c.hs <= 128 ? parts_of<16> : parts_of<256>)(c.blocks, most_parts(waves)) + 1;
+    } else {
+      parts = tile_parts(waves, c.hs, c.blocks);
+      if (parts == 1) parts = 0;  // (nothing to join)
+    }
+    most = std::max(most, waves * parts * rows * (c.hs + 4) * (int64_t)sizeof(float));
   }
-  return most * c.nkv * parts * rows * (c.hs + 4) * (int64_t)sizeof(float);
+  return most;
 }
 
 hipError_t launch_cache_attention(const CacheAttn &args, hipStream_t s) {

@@ -382,3 +382,18 @@ def test_attention_of_few_tokens_with_many_kv_heads(nh, nkv, hs, pos, count):
     model.append(k, v, 0)
     q = rng.standard_normal((count, nh * hs)).astype(np.float32)
     within(cache.attention(q, k[pos:], v[pos:], pos, nh), model, q, pos, nh)
+
+
+@pytest.mark.parametrize("nh, nkv, hs", [(22, 2, 64), (8, 8, 128), (32, 1, 16), (10, 5, 32), (4, 2, 256), (200, 200, 16)])
+@pytest.mark.parametrize("pos, count", [(0, 1), (5003, 1), (5001, 6), (4999, 37), (90, 300), (3000, 1000)])
+def test_nothing_is_written_behind_the_workspace(nh, nkv, hs, pos, count):
+    lib, seq = package().library(), pos + count
+    cache = Cache(nkv, hs, seq)
+    q, k = Dev((count, nh * hs), np.float32), Dev((count, nkv * hs), np.float32)
+    out = Dev((count, nh * hs), np.float32)
+    need = lib.hk_cache_workspace(cache.ref, nh, count)
+    assert need >= 0
+    space = Dev(need + 65536, np.uint8, np.full(need + 65536, 0xA5))
+    check(lib.hk_cache_attention(out.ptr, q.ptr, k.ptr, k.ptr, cache.ref, nh, nh * hs, nkv * hs, nh * hs, count, pos,
+                                 space.ptr, need, None))
+    assert (space.numpy()[need:] == 0xA5).all()
