@@ -449,8 +449,10 @@ __global__ __launch_bounds__(THREADS) void logprobs_join_kernel(const LogprobArg
   finish(a, row, dm, dz, dh, s.list, TOP ? s.count : 0);
 }
 
-// a row's parts, of whole batches of a workgroup: enough workgroups to fill the card
+// A row's parts, of whole batches of a workgroup: enough workgroups to fill the card. Many rows are not split: 1000 rows of
+// 32000 take 31 us, in two parts each 37.6; but 512 of 128256 57 in two parts, 61 unsplit.
 int parts_of(int32_t m, int32_t n) {
+  if (m >= 640) return 1;
   const int64_t batches = ((int64_t)n + THREADS * BATCH - 1) / (THREADS * BATCH);
   const int64_t each = std::max<int64_t>(1, batches * m / 1024);
   return (int)((batches + each - 1) / each);
