@@ -344,8 +344,10 @@ int64_t hk_cache_workspace(const hk_cache *cache, int32_t n_heads, int32_t count
 int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t from, int32_t count, int32_t end,
                       void *stream);
 
-/* Goes back to position pos (any before where the last call ended), where its block's earlier float32 rows are no longer
- * held: they are taken from the block's 8-bit values. The next hk_cache_append is at pos. */
+/* Goes back to position pos, further than the latest HK_CACHE_RECENT - HK_CACHE_BLOCK: its block is complete and its earlier
+ * float32 rows are no longer held, so they are taken from the block's 8-bit values. The next hk_cache_append is at pos.
+ * (Within the latest positions no call is needed, and none may be made in a block that has not been complete: it has no
+ * 8-bit values, and its float32 rows would be lost.) */
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
 
 /* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats apart

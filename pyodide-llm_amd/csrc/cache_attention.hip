@@ -350,7 +350,8 @@ struct Tile {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = p0 + 8 * (r / 4) + 4 * half + r % 4;
-      p[r] = j <= token ? s[r] * unit : -__builtin_inff();
+      // (an infinite score, of a key that is not finite: not a number, whichever its sign)
+      p[r] = j <= token ? __builtin_fmaf(s[r], 0.0f, s[r] * unit) : -__builtin_inff();
       top = __builtin_fmaxf(top, p[r]);
     }
     top = __builtin_fmaxf(top, other_half(top));

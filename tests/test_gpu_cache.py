@@ -397,3 +397,23 @@ def test_nothing_is_written_behind_the_workspace(nh, nkv, hs, pos, count):
     check(lib.hk_cache_attention(out.ptr, q.ptr, k.ptr, k.ptr, cache.ref, nh, nh * hs, nkv * hs, nh * hs, count, pos,
                                  space.ptr, need, None))
     assert (space.numpy()[need:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_an_infinite_key_reaches_every_row_that_sees_it(sign):
+    """also those whose score it takes to minus infinity: in its own block, and once that is in 8 bits"""
+    nh, nkv, hs, n, at = 4, 2, 64, 100, 41
+    rng = np.random.default_rng(17)
+    k, v = rows(rng, n, nkv, hs)
+    q = rng.standard_normal((n, nh * hs)).astype(np.float32)
+    k[at, hs + 3] = sign * np.inf
+    cache = Cache(nkv, hs, n)
+    cache.append(k, v, 0)
+    got = cache.attention(q, k, v, 0, nh)
+    assert np.isnan(got[at:, 2:]).any(-1).all()
+    assert np.isfinite(got[:at]).all() and np.isfinite(got[:, :2]).all()
+    few = Cache(nkv, hs, n)
+    few.append(k[:50], v[:50], 0)
+    for p in (40, 41, 49):
+        one = few.attention(q[p:p + 1], k[p:p + 1], v[p:p + 1], p, nh)
+        assert np.isfinite(one[0, :2]).all() and np.isnan(one[0, 2:]).any(-1).all() == (p >= at)
