@@ -47,7 +47,8 @@ constexpr int lds_bytes() { return HS * 36; }
 // One (block, kv head, keys or values) a workgroup; a thread takes four positions of four channels, so that keys leave it as
 // a word a position and values as a word a channel. The block's rows are read once and kept in registers; a complete
 // block's largest magnitude gives its scale, its bytes go through LDS into the cache's order; the call's rows among the
-// latest 128 positions are copied. Bound by memory: each float32 value is read once, each byte written once.
+// latest 128 positions are copied. Bound by memory: each float32 value is read once, each byte written once (2048 tokens of 8
+// heads of 128: 7.4 us, 21 MB; out again by read_kernel 5.9). A token's call is latency, 3 us.
 template <int HS>
 __global__ __launch_bounds__(256) void append_kernel(const CacheRows a) {
   constexpr int UNITS = CACHE_BLOCK / 4 * (HS / 4), EACH = (UNITS + 255) / 256;
