@@ -206,12 +206,14 @@ struct Tile {
   // blocks first, first + step, .. below to, by their 8-bit values, once start(first) has run: each one's bytes are asked for
   // once the products have taken those of the block before it
   __device__ __forceinline__ void blocks(int first, int to, int step) {
+    i32x16 magic = (i32x16)(0x4B400000);  // (kept in registers where they suffice: made anew, it took 23 instructions a block)
+    if (HS <= 128) asm volatile("" : "+v"(magic));
     for (int b = first; b < to; b += step) {
       const int next = b + step < to ? b + step : b;  // (the last one again, unused: a branch around the reads cost 10%)
       const float2 scale = sp[b];
       // 256 (K d0) + K d1 in one accumulator, K d2 in another that starts at 1.5 * 2^23's bits and is read as a float
       constexpr float MAGIC = 12582912.0f;
-      i32x16 s0 = (i32x16)(0), s2 = (i32x16)(0x4B400000);
+      i32x16 s0 = (i32x16)(0), s2 = magic;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) s0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(k[s], q0[s], s0, 0, 0, 0);
 #pragma unroll
