@@ -6,7 +6,7 @@
 // second launch joins.
 //
 // 512 rows of 128256 with 5 alternatives take 56 us, 4.7 TB/s (a plain streaming read 41): the VALU issues in 0.78 of the
-// cycles, an exponential, a maximum and four other operations a logit and the candidates' ballots. One row takes 11.4, a chain of
+// cycles, an exponential, a maximum and four other operations a logit and the candidates' ballots. One row takes 11.0, a chain of
 // latencies: the read, the bar, the join's reads and its ordering.
 #include <algorithm>
 
@@ -229,8 +229,16 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(const LogprobArgs a, 
   int reached_since = 0;  // lanes that have reached the bar since it was found
   uint64_t least = 0;  // a key that candidates are above, once ties have filled the wave's list
   int held = 0;
+  const int inside = min(to, (int)(((int64_t)ahead + a.n) / 4));  // quads from here on are not whole, or another part's
   float4 next[QUADS];  // a batch is read while the one before it is worked on
   auto read = [&](int q0) {
+    // (the same in the whole workgroup: a batch that lies inside the row and the part)
+    if (q0 * 4 >= ahead && q0 + THREADS * QUADS <= inside) {
+      const float4 *from = reinterpret_cast<const float4 *>(base) + q0 + tid;
+#pragma unroll
+      for (int j = 0; j < QUADS; ++j) next[j] = from[THREADS * j];
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < QUADS; ++j) {
       const int q = q0 + THREADS * j + tid;
