@@ -12,9 +12,9 @@
 // the largest probability times its block's value scale, so that halves neither overflow nor lose bits where the blocks'
 // scales differ.
 //
-// What bounds it: 32 rows by 32 positions of 128 channels take 28 MFMAs (890 cycles) and about 320 VALU instructions (1300),
-// and the two add up, whichever wave of a SIMD they are of: 2048 tokens of 32 / 8 heads of 128 from the start take 97 us, 1001
-// of 28 / 4 at 20,003 580 to 610 (500 TFLOP/s of the attention's 4 hs a score). One token over 131,077 positions, 268 MB,
+// What bounds it: 32 rows by 32 positions of 128 channels take 28 MFMAs (890 cycles) and about 290 VALU instructions (1200),
+// and the two add up, whichever wave of a SIMD they are of: 2048 tokens of 32 / 8 heads of 128 from the start take 93 us, 1001
+// of 28 / 4 at 20,003 570 to 610 (500 TFLOP/s of the attention's 4 hs a score). One token over 131,077 positions, 268 MB,
 // takes 54 to 58 us (4.7 TB/s; a plain streaming read of as much 44); over 4077 9.6, which is latency: a chain of loads,
 // products and two barriers for the token's own block, a second launch that joins the parts.
 #include <algorithm>

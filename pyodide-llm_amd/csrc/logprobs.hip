@@ -5,7 +5,7 @@
 // are picked out on the way by a threshold that only ever grows. A few rows are split over many workgroups, whose parts a
 // second launch joins.
 //
-// 512 rows of 128256 with 5 alternatives take 56 us, 4.7 TB/s (a plain streaming read 41): the VALU issues in 0.78 of the
+// 512 rows of 128256 with 5 alternatives take 56 us, 4.7 TB/s (a plain streaming read 41): the VALU issues in 0.6 of the
 // cycles, an exponential, a maximum and four other operations a logit and the candidates' ballots. One row takes 11.0, a chain of
 // latencies: the read, the bar, the join's reads and its ordering.
 #include <algorithm>
