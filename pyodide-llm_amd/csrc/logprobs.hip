@@ -6,7 +6,7 @@
 // second launch joins.
 //
 // 512 rows of 128256 with 5 alternatives take 56 us, 4.7 TB/s (a plain streaming read 41): the VALU issues in 0.6 of the
-// cycles, an exponential, a maximum and four other operations a logit and the candidates' ballots. One row takes 11.0, a chain of
+// cycles, an exponential, a maximum and four other operations a logit and the candidates' ballots. One row takes 10.5, a chain of
 // latencies: the read, the bar, the join's reads and its ordering.
 #include <algorithm>
 
@@ -52,7 +52,7 @@ __device__ __forceinline__ void join(T &m, T &z, T &h, T m2, T z2, T h2) {
 }
 
 // the candidates a part passes on: what is left of them behind its bar, as a rule
-__host__ __device__ constexpr int slots_of(int top) { return top ? 3 * top + 8 : 0; }
+__host__ __device__ constexpr int slots_of(int top) { return top ? 3 * top + 4 : 0; }
 
 struct Shared {
   uint64_t held[WAVES][HELD];  // the waves' candidates
