@@ -22,9 +22,5 @@ constexpr int CACHE_RECENT = 128;  // positions whose float32 rows are kept (HK_
 __device__ __forceinline__ int value_byte(int t) {
   return ((t >> 2 & 1) << 4) | ((t >> 4) << 3) | ((t >> 3 & 1) << 2) | (t & 3);
 }
-// its inverse
-__device__ __forceinline__ int value_position(int byte) {
-  return ((byte >> 3 & 1) << 4) | ((byte >> 2 & 1) << 3) | ((byte >> 4) << 2) | (byte & 3);
-}
 
 }  // namespace ple

@@ -337,3 +337,23 @@ def test_the_node_host_gives_the_same(tmp_path):
     np.testing.assert_array_equal(out["last"]["ids"], last["ids"])
     assert out["threw"] == [True] * 4
     assert out["footprint"] + ck.size >= out["memoryBytes"]
+
+
+@pytest.mark.parametrize("form", ["llama", "qwen int6", "wide heads"])
+@pytest.mark.parametrize("start", [30, 1400])
+def test_replayed_steps_over_a_long_cache_equal_eager_ones(form, start, monkeypatch):
+    """a cache past the one-launch form: a step's parts are those of its position, whether the launch knows it or not"""
+    fields, got = dict(FORMS[form], seq_len=3000), []
+    for graph in ("1", "0"):
+        monkeypatch.setenv("PYODIDE_LLM_HIP_GRAPH", graph)
+        eng = opened(fields, 8, block=512)[0]
+        text = tokens(start + 1)
+        for at in range(0, start, 512):
+            eng.forwardMany(text[at:min(start, at + 512)], at)
+        randoms = [float(r) for r in np.random.default_rng(4).random(48)]
+        ids = eng.generateMany(text[-1], start, text, start + 1, 48, 1.0, 1.0, 1.0, randoms, [])
+        got.append((ids, np.array(eng.logits()), eng.keysAndValues(start, len(ids))))
+    assert len(got[0][0]) == 48 and got[0][0] == got[1][0]
+    np.testing.assert_array_equal(got[0][1], got[1][1])
+    for name in ("keys", "values"):
+        np.testing.assert_array_equal(got[0][2][name], got[1][2][name])
