@@ -328,7 +328,10 @@ int32_t hk_cache_append(const hk_cache *cache, const void *k, const void *v, int
  * h / (n_heads / n_kv_heads). q and out float32 with rows of n_heads * head_size values, q_stride and out_stride floats
  * apart; k and v the tokens' own rows as hk_cache_append took them with the same count and pos. Strides are multiples of
  * 4, pointers 16-byte aligned; n_heads is a multiple of n_kv_heads, at most HK_CACHE_GROUP_MOST times it. A q that is not
- * finite makes its own row NaN, a key or value the rows of the tokens that see it; no other row changes. workspace: at
+ * finite makes its own row NaN, a key or value the rows of the tokens that see it; no other row changes. Finite ones of any
+ * size are taken, but for two kinds: a query whose largest value lies below 2^-100 counts as zero against the 8-bit values
+ * (not against its own block's rows), and a block's 8-bit values whose scale is a denormal (none above 1.5e-36) count as
+ * zero. workspace: at
  * least hk_cache_workspace bytes of device memory (16-byte aligned; nothing in it is kept from one call to the next), not
  * shared by calls that may overlap. */
 int32_t hk_cache_attention(void *out, const void *q, const void *k, const void *v, const hk_cache *cache,

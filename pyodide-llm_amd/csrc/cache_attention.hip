@@ -38,6 +38,12 @@ constexpr float NONE = -1e30f;  // no maximum yet (finite: its differences stay 
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
+// 2^n of a whole n <= 0, what one reference is to another: a denormal too, which the exponential's instruction gives as 0
+// (values below 2^-106 in 8 bits beside an own block would vanish)
+__device__ __forceinline__ float power(float n) {
+  return __builtin_amdgcn_ldexpf(1.0f, (int)__builtin_fmaxf(n, -200.0f));
+}
+
 // four of a query's values as three words of digits: round(x m) = 65536 d0 + 256 d1 + d2, below 2^22. Added to 1.5 * 2^23
 // + 0x8080, the sum's low three bytes are d0 + 64, d1 + 128 and d2 + 128; they are gathered by value and taken back.
 // (16 instructions; with conversions, shifts and masks 72)
@@ -163,7 +169,7 @@ struct Tile {
   __device__ __forceinline__ void advance(float top, float bits) {
     const float up = __builtin_ceilf(top), m = __builtin_fmaxf(run.m, up), mw = __builtin_fmaxf(run.mw, up + bits);
     run.l *= __builtin_amdgcn_exp2f(run.m - m);
-    const float gamma = __builtin_amdgcn_exp2f(run.mw - mw);
+    const float gamma = power(run.mw - mw);
     if (__any(gamma != 1.0f)) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t) o[t] *= gamma;
@@ -363,7 +369,9 @@ struct Tile {
       top = __builtin_fmaxf(top, p[r]);
     }
     top = __builtin_fmaxf(top, other_half(top));
-    advance(top, 1.0f);
+    // (the reference lies 2^20 above the largest score: a probability comes as 2^-6 at most, and 32 of them times values of up to
+    // the type's largest stay below 2^128. Their real size is not known yet where a wave reads them a part at a time)
+    advance(top, 20.0f);
     const float factor = __builtin_amdgcn_exp2f(__builtin_fminf(run.m - run.mw + 14.0f, 126.0f));
     float sum = 0.0f;
 #pragma unroll
@@ -489,7 +497,7 @@ __global__ __launch_bounds__(256) void attend_join_rows_kernel(const CacheAttn a
     const float4 x = o[(int64_t)p * rows * QUADS], s = stats[(int64_t)p * rows];
     const float top = __builtin_fmaxf(m, s.x), high = __builtin_fmaxf(mw, s.z);
     l = l * __builtin_amdgcn_exp2f(m - top) + s.y * __builtin_amdgcn_exp2f(s.x - top);
-    const float f = __builtin_amdgcn_exp2f(mw - high), g = __builtin_amdgcn_exp2f(s.z - high);
+    const float f = power(mw - high), g = power(s.z - high);
     y = make_float4(y.x * f + x.x * g, y.y * f + x.y * g, y.z * f + x.z * g, y.w * f + x.w * g);
     m = top;
     mw = high;
@@ -575,7 +583,7 @@ __global__ __launch_bounds__(256, HS <= 128 ? 2 : 1) void attend_part_kernel(con
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float4 z = *reinterpret_cast<const float4 *>(x + w * rows * STRIDE);
-      const float f = __builtin_amdgcn_exp2f(stats[w][row][2] - mw);
+      const float f = power(stats[w][row][2] - mw);
       y.x = __builtin_fmaf(z.x, f, y.x);
       y.y = __builtin_fmaf(z.y, f, y.y);
       y.z = __builtin_fmaf(z.z, f, y.z);
@@ -655,7 +663,7 @@ __global__ __launch_bounds__(512, HS <= 128 ? 2 : 1) void attend_short_kernel(co
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       const float4 z = *reinterpret_cast<const float4 *>(from + w * rows * STRIDE);
-      const float f = __builtin_amdgcn_exp2f(stats[w][row][2] - mw);
+      const float f = power(stats[w][row][2] - mw);
       l += stats[w][row][1] * __builtin_amdgcn_exp2f(stats[w][row][0] - m);
       y.x = __builtin_fmaf(z.x, f, y.x);
       y.y = __builtin_fmaf(z.y, f, y.y);
@@ -706,7 +714,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const CacheAttn a, int
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     l += stat[j].y * __builtin_amdgcn_exp2f(stat[j].x - m);
-    scales[tid / 64][lane + 64 * j] = __builtin_amdgcn_exp2f(stat[j].z - mw);
+    scales[tid / 64][lane + 64 * j] = power(stat[j].z - mw);
   }
   l = wave_sum(l);
   wave_sync_lds();

@@ -417,3 +417,26 @@ def test_an_infinite_key_reaches_every_row_that_sees_it(sign):
     for p in (40, 41, 49):
         one = few.attention(q[p:p + 1], k[p:p + 1], v[p:p + 1], p, nh)
         assert np.isfinite(one[0, :2]).all() and np.isnan(one[0, 2:]).any(-1).all() == (p >= at)
+
+
+@pytest.mark.parametrize("nh, nkv, hs, pos, count", [(6, 6, 48, 40, 1), (8, 2, 128, 700, 1), (8, 2, 128, 20, 50), (4, 2, 256, 70, 40),
+                                                     (48, 48, 16, 20, 200), (96, 48, 64, 33, 170)])
+@pytest.mark.parametrize("size", [1e-35, 1e-30, 3e19, 1e35, 1e38])
+@pytest.mark.parametrize("which", ["all", "the last", "one in three"])
+def test_values_of_any_size(nh, nkv, hs, pos, count, size, which):
+    """values up to 3.3e38 and down to 1e-35, in the token's own block as behind it: the attention lies between them, and a row
+    that sees no large one keeps the bits of its small ones"""
+    rng = np.random.default_rng(count + hs)
+    n = pos + count
+    cache, model = Cache(nkv, hs, n), Model(nkv, hs, n)
+    k, v = rows(rng, n, nkv, hs)
+    large = np.zeros(n, dtype=bool)
+    large[slice(None) if which == "all" else slice(n - 1, None) if which == "the last" else slice(1, None, 3)] = True
+    v[large] = np.clip(v[large], -3.3, 3.3) * np.float32(size)
+    for a, b in ((0, pos), (pos, n)):
+        cache.append(k[a:b], v[a:b], a)
+        model.append(k[a:b], v[a:b], a)
+    q = rng.standard_normal((count, nh * hs)).astype(np.float32)
+    got = cache.attention(q, k[pos:], v[pos:], pos, nh)
+    for i in sorted({0, count // 3, count // 2, count - 2, count - 1} & set(range(count))):
+        within(got[i:i + 1], model, q[i:i + 1], pos + i, nh)
