@@ -353,14 +353,15 @@ int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t f
  * 8-bit values, and its float32 rows would be lost.) */
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
 
-/* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats apart
- * (stride >= n, any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens given [m][n_given] int32
- * (NaN where one is outside 0..n-1; null with n_given 0), the entropy [m] in nats (or null), and the `top`
- * (0..HK_LOGPROBS_TOP_MOST) largest alternatives, ids [m][top] int32 and logps [m][top], the lowest index first among
- * equals. A logit of minus infinity has probability 0: log probability minus infinity, nothing of the entropy, and no
- * alternative (id -1, log probability minus infinity, behind the others). A row whose largest logit is not finite has no
- * probabilities: NaN and id -1 throughout. All pointers are device memory. workspace: at least hk_logprobs_workspace bytes
- * (16-byte aligned), not shared by calls that may overlap. Neither allocates nor waits. */
+/* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats
+ * apart (stride >= n, any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens
+ * given [m][n_given] int32 (NaN where one is outside 0..n-1; null with n_given 0), the entropy [m] in nats (or null),
+ * and the `top` (0..HK_LOGPROBS_TOP_MOST) largest alternatives, ids [m][top] int32 and logps [m][top], the lowest index
+ * first among equals. No log probability is above 0, no entropy below. A logit of minus infinity has probability 0: log
+ * probability minus infinity, nothing of the entropy, and no alternative (id -1, log probability minus infinity, behind
+ * the others). A row whose largest logit is not finite has no probabilities: NaN and id -1 throughout. All pointers are
+ * device memory. workspace: at least hk_logprobs_workspace bytes (16-byte aligned), not shared by calls that may
+ * overlap. Neither allocates nor waits. */
 #define HK_LOGPROBS_TOP_MOST 32
 int32_t hk_logprobs(void *logp, void *entropy, void *ids, void *logps, const void *logits, int64_t stride,
                     const void *given, int32_t n_given, int32_t m, int32_t n, int32_t top, void *workspace,

@@ -186,8 +186,10 @@ __device__ __forceinline__ void finish(const LogprobArgs &a, int64_t row, double
                                        int held) {
   const float *x = a.logits + row * a.stride;
   const bool fine = z > 0.0 && m > (double)-__builtin_inff() && m < (double)__builtin_inff();
-  const double nan = __builtin_nan(""), logz = logf((float)z);
-  if (threadIdx.x == 0 && a.entropy) a.entropy[row] = (float)(fine ? logz - h / z : nan);
+  // (Z is 1 at least, the largest logit's own term, and the entropy not negative: where a peaked row's sums round below, a
+  // caller's log(1 - p) or square root would be no number)
+  const double nan = __builtin_nan(""), logz = z > 1.0 ? (double)logf((float)z) : 0.0, entropy = logz - h / z;
+  if (threadIdx.x == 0 && a.entropy) a.entropy[row] = (float)(!fine ? nan : entropy > 0.0 ? entropy : 0.0);
   for (int g = threadIdx.x; g < a.n_given; g += THREADS) {
     const int t = a.given[row * a.n_given + g];
     a.logp[row * a.n_given + g] = (float)(fine && t >= 0 && t < a.n ? (double)x[t] - m - logz : nan);

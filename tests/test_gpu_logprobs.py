@@ -202,3 +202,20 @@ def test_captured_calls_replay():
         hip_check(h.hipGraphExecDestroy(replay))
         hip_check(h.hipGraphDestroy(graph))
         hip_check(h.hipStreamDestroy(stream))
+
+
+@pytest.mark.parametrize("m, n", [(1500, 64), (100, 9000), (640, 4100)])
+def test_probabilities_and_entropies_have_their_sign(m, n):
+    """peaked rows: no probability above 1, no entropy below 0, whatever the largest logit rounds to"""
+    rng = np.random.default_rng(n)
+    x = np.empty((m, n), dtype=np.float32)
+    top = rng.uniform(-40, 40, m).astype(np.float32)
+    x[:] = top[:, None] - np.where(np.arange(m) % 2, 200.0, 25.0)[:, None]
+    at = rng.integers(0, n, m)
+    x[np.arange(m), at] = top
+    logp, h, ids, logps = run(x, at[:, None], 5)
+    assert (logp <= 0).all() and (logps <= 0).all() and (h >= 0).all()
+    # rows of one token: its term is 2^t, t from -1 to 0, times 2^-t, two exponentials within 2^-23 of themselves and a product
+    # rounded to 2^-24: Z within 2^-21 of 1. H is 2^t t plus -t Z, their roundings 2^-24 each and Z's error: with log Z 2^-20
+    assert (logp[1::2] >= -2.0 ** -21).all() and (h[1::2] <= 2.0 ** -20).all()
+    agree(x, at[:, None], 5)
