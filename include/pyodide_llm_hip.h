@@ -42,8 +42,11 @@ extern "C" {
 /* he_config.half_kv for a cache held in 8 bits (hk_cache): a quarter of float32's bytes a position, and contexts of up to
  * HK_CACHE_MOST positions. Its attention is hk_cache_attention's, in float32 accuracy over what the cache stands for, not
  * the reference's order: logits follow the reference's with the cache's rounding. A token's numbers do not depend on how
- * the tokens before it were split into calls, to the rounding of float32 sums. A step back to a position of the latest 96
- * finds its block's float32 rows; further back, the block's earlier positions stand as their 8-bit values. */
+ * the tokens before it were split into calls, to the rounding of float32 sums. Calls may be made at any position, as over
+ * the float32 cache: a token reads the rows that were last written, zeros where none were. The float32 rows of the latest
+ * 128 positions are held, counted from the furthest one that has run since the last step further back than that (the steps
+ * that a stopped he_generate_many ran past its end among them): a call at one of the latest 96 finds its block's earlier
+ * rows in float32, one further back finds them by their 8-bit values. */
 #define HE_KV_EIGHT 8
 
 /* The model: the fields of `plan` (public/llama2_numpy.py:1261-1270) the forward reads. */

@@ -158,10 +158,11 @@ struct he_engine {
   float *cos_t = nullptr, *sin_t = nullptr;
   void *keys = nullptr, *vals = nullptr;  // keys [layers][seq_len][kv_dim], values [layers][kv_dim][value_stride]
   // the cache in 8 bits: the scales and the recent float32 rows of every layer (keys and vals hold the bytes), the
-  // attention's workspace; positions rows_from..rows_to - 1 have their float32 rows among the recent ones, and the next
-  // token is taken to stand at cache_end
-  float *cache_scales = nullptr, *recent_keys = nullptr, *recent_values = nullptr, *cache_space = nullptr;
-  int32_t rows_from = 0, rows_to = 0, cache_end = 0;
+  // attention's workspace, a row of zeros; positions rows_from..rows_to - 1 have their float32 rows among the recent ones, the
+  // blocks before cache_whole are complete, and the next token is taken to stand at cache_end
+  float *cache_scales = nullptr, *recent_keys = nullptr, *recent_values = nullptr, *cache_space = nullptr,
+        *cache_zero_row = nullptr;
+  int32_t rows_from = 0, rows_to = 0, cache_whole = 0, cache_end = 0;
   // he_score and he_logprobs (made at their first call): a piece's logits, the log probabilities' workspace, what is asked
   // and what comes back
   float *score_logits = nullptr;
@@ -247,18 +248,67 @@ CacheView cache_view(const he_engine *e, int32_t l) {
           c.n_kv_heads, c.head_size, blocks};
 }
 
-// the cache in 8 bits before count tokens at pos: where their block's earlier float32 rows are no longer held (a step far
-// back), they are taken from its 8-bit values
+// count zero rows at pos.. into the cache in 8 bits, every layer
+int32_t cache_zeros(he_engine *e, int32_t pos, int32_t count) {
+  for (int32_t l = 0; l < e->c.n_layers; ++l) {
+    const CacheRows rows{cache_view(e, l), e->cache_zero_row, e->cache_zero_row, 0, count, pos, nullptr, 0};
+    HIP_TRY(launch_cache_append(rows, e->stream));
+  }
+  return HE_OK;
+}
+
+// the block that the last call ended in, where it had been complete: its 8-bit values made anew, the call's rows among them
+int32_t cache_settles(he_engine *e) {
+  const int32_t at = e->cache_end, to = at / 32 * 32 + 32;
+  if (at % 32 == 0 || to > e->cache_whole) return HE_OK;
+  for (int32_t l = 0; l < e->c.n_layers; ++l) {
+    const CacheView c = cache_view(e, l);
+    if (e->rows_to < to) HIP_TRY(launch_cache_read(c, nullptr, nullptr, e->rows_to, to - e->rows_to, -1, e->stream));
+    const int64_t row = (int64_t)(at % 128) * e->kvdim;  // (the rows behind `at` go through the append that quantizes)
+    const CacheRows rows{c, c.recent_keys + row, c.recent_values + row, e->kvdim, to - at, at, nullptr, 0};
+    HIP_TRY(launch_cache_append(rows, e->stream));
+  }
+  e->rows_to = std::max(e->rows_to, to);
+  return HE_OK;
+}
+
+// The cache in 8 bits before count tokens at pos. Positions rows_from..rows_to - 1 have their float32 rows among the
+// recent ones (rows_to the furthest: a step back leaves those behind it as they are), and every block before cache_whole
+// is complete. Within the rows, or where they end, nothing is to be done. Elsewhere the block's earlier rows (those not
+// held) are taken from its 8-bit values, and the block being filled, whose rows are held nowhere else, is first
+// completed with zeros, so that a return to it finds it. Positions passed over stand as zeros, as in the float32 cache.
 int32_t cache_moves(he_engine *e, int32_t pos, int32_t count) {
   if (!eight(e->c)) return HE_OK;
   const int32_t first = pos / 32 * 32;
-  const bool held = e->rows_from <= first && pos <= e->rows_to;
-  if (!held && pos > first)
-    for (int32_t l = 0; l < e->c.n_layers; ++l)
-      HIP_TRY(launch_cache_read(cache_view(e, l), nullptr, nullptr, first, pos - first, -1, e->stream));
-  if (!held) e->rows_from = first;
-  e->rows_to = e->cache_end = pos + count;
+  int32_t rc = first != e->cache_end / 32 * 32 ? cache_settles(e) : HE_OK;
+  if (rc) return rc;
+  if (pos > e->rows_to && e->rows_to >= e->cache_whole) {  // past all that has been written
+    int32_t at = e->rows_to;
+    if (at % 32) {
+      const int32_t up = std::min(pos, at / 32 * 32 + 32);
+      if ((rc = cache_zeros(e, at, up - at))) return rc;
+      at = up;
+    }
+    if (at < first) at = e->rows_from = first;  // (blocks that are zeros in 8 bits)
+    if (at < pos && (rc = cache_zeros(e, at, pos - at))) return rc;
+    e->rows_to = pos;
+  } else if (e->rows_from > first || pos > e->rows_to) {
+    if (e->rows_to > e->cache_whole) {
+      if ((rc = cache_zeros(e, e->rows_to, e->cache_whole + 32 - e->rows_to))) return rc;
+      e->cache_whole += 32;
+    }
+    const bool begun = e->rows_from <= first && e->rows_to > first;  // (the block's first rows are held)
+    const int32_t from = begun ? e->rows_to : first;
+    if (pos > from)
+      for (int32_t l = 0; l < e->c.n_layers; ++l)
+        HIP_TRY(launch_cache_read(cache_view(e, l), nullptr, nullptr, from, pos - from, -1, e->stream));
+    if (!begun) e->rows_from = first;
+    e->rows_to = pos;
+  }
+  e->cache_end = pos + count;
+  e->rows_to = std::max(e->rows_to, e->cache_end);
   e->rows_from = std::max(e->rows_from, e->rows_to - 128);
+  e->cache_whole = std::max(e->cache_whole, e->rows_to / 32 * 32);
   return HE_OK;
 }
 
@@ -279,7 +329,7 @@ void destroy(he_engine *e) {
                   e->best_v, e->best_i, e->state, e->step_ids, e->step_values, e->sample_probs, e->sample_index,
                   e->window, e->sample_token, e->sample_best, e->before, e->columns, e->picked, e->sink,
                   e->run_params, e->kept_logits, e->sample_parts, e->cache_scales, e->recent_keys, e->recent_values,
-                  e->cache_space, e->score_logits, e->score_space, e->score_io};
+                  e->cache_space, e->cache_zero_row, e->score_logits, e->score_space, e->score_io};
   for (void *p : ptrs)
     if (p) (void)hipFree(p);
   void *pinned[] = {e->host_ids, e->host_state, e->host_values, e->host_window, e->host_params};
@@ -418,6 +468,8 @@ int32_t allocate_state(he_engine *e, const float *rope_cos, const float *rope_si
     HIP_TRY(hipMemset(e->cache_scales, 0, blocks * c.n_kv_heads * 2 * sizeof(float)));
     HIP_TRY(hipMemset(e->recent_keys, 0, rows));
     HIP_TRY(hipMemset(e->recent_values, 0, rows));
+    ALLOC(e->cache_zero_row, sizeof(float) * e->kvdim);
+    HIP_TRY(hipMemset(e->cache_zero_row, 0, sizeof(float) * e->kvdim));
     int64_t space = 1;
     for (int32_t m = 1; m <= T; ++m) space = std::max(space, cache_attention_workspace(v, c.n_heads, m));
     ALLOC(e->cache_space, (size_t)space);

@@ -357,3 +357,127 @@ def test_replayed_steps_over_a_long_cache_equal_eager_ones(form, start, monkeypa
     np.testing.assert_array_equal(got[0][1], got[1][1])
     for name in ("keys", "values"):
         np.testing.assert_array_equal(got[0][2][name], got[1][2][name])
+
+
+def run_one_by_one(eng, ids, start=0):
+    for i, t in enumerate(ids):
+        eng.forward(t, start + i)
+
+
+@pytest.mark.parametrize("back", [0, 10, 33, 39])
+def test_a_look_back_leaves_the_rows_behind_it(back):
+    """a token run again at an earlier position (for its logits), then the conversation's next one: as without the look back"""
+    ids = tokens(60)
+    plain, eng = opened(FIELDS, 8)[0], opened(FIELDS, 8)[0]
+    for e in (plain, eng):
+        run_one_by_one(e, ids[:40])
+    eng.forward(ids[back], back)
+    for e in (plain, eng):
+        run_one_by_one(e, ids[40:], 40)
+    np.testing.assert_array_equal(eng.logits(), plain.logits())
+    a, b = (e.keysAndValues(0, 60) for e in (eng, plain))
+    for name in a:
+        np.testing.assert_array_equal(a[name], b[name])
+
+
+def first_layer(eng, count):
+    return rows_of(eng.keysAndValues(0, count), eng.config, count)[:, 0]
+
+
+def test_a_return_from_far_back_finds_the_last_block():
+    """far back and forward to the end again: the block that was being filled stands as its 8-bit values, not as zeros"""
+    ids = tokens(210)
+    eng, full = opened(FIELDS, 8)[0], opened(FIELDS, 0)[0]
+    for e in (eng, full):
+        run_one_by_one(e, ids[:200])
+        e.forward(ids[10], 10)
+        run_one_by_one(e, ids[200:], 200)
+    want = rows_of(full.keysAndValues(0, 210), full.config, 210)[:, 0]
+    model = cl.Model(2, 16, 300)
+    model.append(want[0, :200], want[1, :200], 0)
+    # the first block, its rows from 8 bits but the one run again, is quantized anew
+    again = model.read(0, 32, 1 << 40).astype(np.float32)
+    again[:, 10] = want[:, 10]
+    model.append(again[0], again[1], 0)
+    zeros = np.zeros((24, 2, 16), dtype=np.float32)
+    model.append(zeros, zeros, 200)
+    model.rewind(200)
+    model.append(want[0, 200:], want[1, 200:], 200)
+    np.testing.assert_array_equal(first_layer(eng, 210), model.read(0, 210, 210).astype(np.float32))
+
+
+@pytest.mark.parametrize("pos", [12, 31, 32, 50, 140])
+def test_positions_passed_over_stand_as_zeros(pos):
+    """as in the float32 cache"""
+    ids = tokens(20)
+    eng, full = opened(FIELDS, 8)[0], opened(FIELDS, 0)[0]
+    for e in (eng, full):
+        run_one_by_one(e, ids[:10])
+        run_one_by_one(e, ids[10:], pos)
+    n = pos + 10
+    want = rows_of(full.keysAndValues(0, n), full.config, n)[:, 0]
+    assert (want[:, 10:pos] == 0).all()
+    model = cl.Model(2, 16, 300)
+    model.append(want[0], want[1], 0)
+    np.testing.assert_array_equal(first_layer(eng, n), model.read(0, n, n).astype(np.float32))
+
+
+def test_a_position_run_again_with_another_token_is_read_so():
+    """another token at an earlier position, then the conversation's next one: every later token reads the new row, as over
+    the float32 cache, whether the position's block is still held in float32 (100) or not (10)"""
+    ids = tokens(190)
+    for at in (100, 10):
+        eng, full = opened(FIELDS, 8)[0], opened(FIELDS, 0)[0]
+        for e in (eng, full):
+            run_one_by_one(e, ids[:180])
+            e.forward(7, at)
+            run_one_by_one(e, ids[180:], 180)
+        want = rows_of(full.keysAndValues(0, 190), full.config, 190)[:, 0]
+        got = first_layer(eng, 190)
+        first = at // 32 * 32
+        steps = np.abs(want[:, first:first + 32]).max((1, 3), keepdims=True) / 127
+        assert (np.abs(got[:, first:first + 32] - want[:, first:first + 32]) <= 1.01 * steps).all()
+        old = rows_of(opened_after(ids[:180]).keysAndValues(0, 180), full.config, 180)[:, 0]
+        assert (np.abs(old[:, at] - want[:, at]) > 2 * steps[:, 0]).any()
+
+
+def opened_after(ids):
+    eng = opened(FIELDS, 8)[0]
+    run_one_by_one(eng, ids)
+    return eng
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_calls_at_any_positions_leave_the_rows_last_written(seed):
+    """calls here and there, far back and past the end: the first layer's cache is the float32 cache's but for roundings to 8
+    bits. A block is quantized at most once more than calls have touched it, each time off by half a step, at most 1 / 127 of
+    the head's largest value so far (another scale moves values that have been rounded before)"""
+    rng = np.random.default_rng(seed)
+    eng, full = opened(FIELDS, 8)[0], opened(FIELDS, 0)[0]
+    end = furthest = 0
+    largest, touched = np.zeros((2, 1, 2, 1)), np.ones(300 // 32 + 1)
+
+    def agree(n):
+        nonlocal largest
+        want = rows_of(full.keysAndValues(0, 300), full.config, 300)[:, 0]
+        largest = np.maximum(largest, np.abs(want).max((1, 3), keepdims=True))
+        got = rows_of(eng.keysAndValues(0, n), eng.config, n)[:, 0]
+        off = 0.501 * touched[np.arange(n) // 32][None, :, None, None] * largest / 127
+        assert (np.abs(got - want[:, :n]) <= off).all()
+
+    for _ in range(25):
+        pos = [end, int(rng.integers(0, furthest + 1)), max(0, end - int(rng.integers(0, 130))), furthest,
+               furthest + int(rng.integers(0, 60))][int(rng.choice(5, p=[0.3, 0.25, 0.25, 0.1, 0.1]))]
+        count = min(int(rng.choice([1, 1, 1, 3, 20, 64])), 280 - pos)
+        if count < 1:
+            continue
+        ids = [int(t) for t in rng.integers(3, 320, size=count)]
+        for e in (eng, full):
+            e.forwardMany(ids, pos) if count > 1 else e.forward(ids[0], pos)
+        end = pos + count
+        furthest = max(furthest, end)
+        touched[pos // 32:end // 32 + 1] += 1
+        agree(end)
+    for e in (eng, full):
+        e.forward(5, furthest)
+    agree(furthest + 1)
