@@ -64,7 +64,7 @@ typedef struct he_config {
   int32_t qkv_bias;          /* Qwen2: bq, bk, bv are added after the q, k, v matmuls (public/forward.js:1038-1042) */
   int32_t relaxed;           /* 1: activations with bias 64, matmul_q8r order; 0: bias 0, matmul_q8 lane order */
   int32_t half_kv;           /* keys and values kept in float16 (public/forward.js:762, kernels/kernel.ts:570-608);
-                                HE_KV_EIGHT: in 8 bits (below), a form of the engine's own */
+                                HE_KV_EIGHT: in 8 bits (above), a form of the engine's own */
   float rms_norm_eps;        /* plan.rms_norm_eps (RMSNorm; LayerNorm's is 1e-5, kernels/kernel.ts:627) */
   int32_t arch;              /* plan.arch: HE_ARCH_* */
   int32_t rotary;            /* plan.rotary: the values of each head RoPE turns (neox); 0 or head_size: all */
@@ -184,7 +184,8 @@ int32_t he_logprobs(he_engine *e, const int32_t *given, int32_t n_given, int32_t
                     int32_t *ids, float *logps);
 
 /* engine.keysAndValues(from, count) (public/forward.js:1939-1953): the cache at positions from..from+count-1 as
- * float32 [layers][count][kv_dim], keys then values (host). A cache in 8 bits: as the next token would read them. */
+ * float32 [layers][count][kv_dim], keys then values (host). A cache in 8 bits: as the next token would read them; past
+ * the last call's end by their 8-bit values, zeros where a block has not been complete. */
 int32_t he_kv_read(he_engine *e, int32_t from, int32_t count, float *keys, float *values);
 
 /* external().read(offset, length) (public/forward.js:574): bytes of the checkpoint as the device holds them. */

@@ -1408,7 +1408,8 @@ int32_t he_logits(he_engine *e, float *out) {
 }
 
 namespace {
-// he_kv_read of the cache in 8 bits: as the token at cache_end reads the positions
+// he_kv_read of the cache in 8 bits: as the token at cache_end reads the positions, those behind it by their 8-bit values (zeros
+// in a block that has not been complete)
 int32_t eight_read(he_engine *e, int32_t from, int32_t count, float *keys, float *values) {
   if (count == 0) return HE_OK;
   const size_t floats = (size_t)count * e->kvdim;
@@ -1416,8 +1417,13 @@ int32_t eight_read(he_engine *e, int32_t from, int32_t count, float *keys, float
   int32_t rc = dev_alloc(&rows, 2 * floats * sizeof(float));
   if (rc) return rc;
   hipError_t err = hipSuccess;
+  const int32_t before = std::max(0, std::min(count, e->cache_end - from));
+  const size_t read = (size_t)before * e->kvdim;
   for (int32_t l = 0; l < e->c.n_layers && err == hipSuccess; ++l) {
-    err = launch_cache_read(cache_view(e, l), rows, rows + floats, from, count, e->cache_end / 32, e->stream);
+    const CacheView c = cache_view(e, l);
+    if (before) err = launch_cache_read(c, rows, rows + floats, from, before, e->cache_end / 32, e->stream);
+    if (err == hipSuccess && before < count)
+      err = launch_cache_read(c, rows + read, rows + floats + read, from + before, count - before, -1, e->stream);
     if (err == hipSuccess)
       err = hipMemcpyAsync(keys + l * floats, rows, floats * sizeof(float), hipMemcpyDeviceToHost, e->stream);
     if (err == hipSuccess)

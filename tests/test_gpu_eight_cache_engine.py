@@ -481,3 +481,20 @@ def test_calls_at_any_positions_leave_the_rows_last_written(seed):
     for e in (eng, full):
         e.forward(5, furthest)
     agree(furthest + 1)
+
+
+@pytest.mark.parametrize("count", [20, 140, 160])
+def test_rows_behind_the_end_are_no_other_positions(count):
+    """keysAndValues past the last token: zeros where no token has been, as the float32 cache's"""
+    eng = opened(FIELDS, 8)[0]
+    eng.forwardMany(tokens(count)[:64], 0)
+    for at in range(64, count, 64):
+        eng.forwardMany(tokens(count)[at:at + 64], at)
+    got = rows_of(eng.keysAndValues(0, 200), eng.config, 200)
+    assert (got[:, :, count:] == 0).all()
+    kv = rows_of(eng.keysAndValues(0, count), eng.config, count)
+    np.testing.assert_array_equal(got[:, :, :count], kv)
+    inside = rows_of(eng.keysAndValues(count - 5, 20), eng.config, 20)
+    np.testing.assert_array_equal(inside, got[:, :, count - 5:count + 15])
+    beyond = eng.keysAndValues(count + 3, 9)
+    assert all((beyond[name] == 0).all() for name in beyond)
