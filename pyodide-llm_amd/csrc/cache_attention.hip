@@ -804,7 +804,7 @@ hipError_t launch(const CacheAttn &a, hipStream_t s) {
     return hipGetLastError();
   }
   const size_t bytes = std::max<size_t>(4 * l.rows * (HS + 4), 4 * 16 * 64) * sizeof(float);
-  if (bytes > 65536) {
+  if (bytes + sizeof(float[4][32][3]) > 65536) {  // (and `stats`)
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(attend_part_kernel<HS>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (err != hipSuccess) return err;

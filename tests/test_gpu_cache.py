@@ -440,3 +440,15 @@ def test_values_of_any_size(nh, nkv, hs, pos, count, size, which):
     got = cache.attention(q, k[pos:], v[pos:], pos, nh)
     for i in sorted({0, count // 3, count // 2, count - 2, count - 1} & set(range(count))):
         within(got[i:i + 1], model, q[i:i + 1], pos + i, nh)
+
+
+@pytest.mark.parametrize("nh, nkv, hs", [(31, 1, 128), (62, 2, 128), (15, 1, 256), (32, 1, 96)])
+@pytest.mark.parametrize("pos, count", [(700, 1), (690, 5)])
+def test_groups_whose_outputs_fill_the_workgroups_memory(nh, nkv, hs, pos, count):
+    rng = np.random.default_rng(nh)
+    cache, model = Cache(nkv, hs, pos + count), Model(nkv, hs, pos + count)
+    k, v = rows(rng, pos + count, nkv, hs)
+    cache.append(k, v, 0)
+    model.append(k, v, 0)
+    q = rng.standard_normal((count, nh * hs)).astype(np.float32)
+    within(cache.attention(q, k[pos:], v[pos:], pos, nh), model, q, pos, nh)
