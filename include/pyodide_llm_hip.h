@@ -320,10 +320,19 @@ typedef struct hk_cache {
 
 /* The rows of count tokens at positions pos.. into the cache: k and v float32, a token's kv heads side by side
  * (n_kv_heads * head_size values), kv_stride floats a row (a multiple of 4; k and v 16-byte aligned). Every block that
- * becomes complete is quantized; rows of other positions stay as they are. pos is where the last call ended, or any
- * position of the latest HK_CACHE_RECENT - HK_CACHE_BLOCK (tokens taken again), or the first of a block; before one
- * anywhere else, hk_cache_rewind. A value that is not finite leaves its block's scale (for its head) not finite: the block
- * stands for NaN from then on, for the tokens of later blocks. */
+ * becomes complete is quantized; rows of other positions stay as they are. A value that is not finite leaves its block's
+ * scale (for its head) not finite: the block stands for NaN from then on, for the tokens of later blocks.
+ *
+ * pos is where the last call ended, or before it (the tokens from there on are taken again). A call inside a block needs
+ * the block's earlier rows in float32. Those held are the latest HK_CACHE_RECENT behind the furthest position written, no
+ * further back than the block of the last rewind: with
+ *   earliest = furthest = 0 before the first call,
+ * a call at pos, in the block that starts at first = pos - pos % HK_CACHE_BLOCK, finds them if
+ *   max(earliest, furthest - HK_CACHE_RECENT) <= first and pos <= furthest
+ * (so that the latest HK_CACHE_RECENT - HK_CACHE_BLOCK before the furthest can always be taken again, unless a rewind came
+ * between; a step back does not move the furthest). Where it does not, hk_cache_rewind goes first (a call at first itself
+ * needs none), and earliest = first, furthest = pos from then on. After the call, furthest is pos + count where that is
+ * more. */
 int32_t hk_cache_append(const hk_cache *cache, const void *k, const void *v, int32_t kv_stride, int32_t count,
                         int32_t pos, void *stream);
 
@@ -346,15 +355,15 @@ int32_t hk_cache_attention(void *out, const void *q, const void *k, const void *
 int64_t hk_cache_workspace(const hk_cache *cache, int32_t n_heads, int32_t count);
 
 /* Positions from..from + count - 1 as a token at position end (from + count <= end) would read them: those before end's
- * block by their 8-bit values, that block's by their float32 rows; keys and values float32
- * [count][n_kv_heads * head_size], 16-byte aligned. */
+ * block by their 8-bit values, that block's by their float32 rows (end is where the last call ended, or one that a call could
+ * be made at without a rewind); keys and values float32 [count][n_kv_heads * head_size], 16-byte aligned. */
 int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t from, int32_t count, int32_t end,
                       void *stream);
 
-/* Goes back to position pos, further than the latest HK_CACHE_RECENT - HK_CACHE_BLOCK: its block is complete and its earlier
- * float32 rows are no longer held, so they are taken from the block's 8-bit values. The next hk_cache_append is at pos.
- * (Within the latest positions no call is needed, and none may be made in a block that has not been complete: it has no
- * 8-bit values, and its float32 rows would be lost.) */
+/* Goes back to position pos where hk_cache_append cannot by itself: its block is complete and its earlier float32 rows are no
+ * longer held, so they are taken from the block's 8-bit values. The next hk_cache_append is at pos. (Where the rows are held
+ * no call is needed, and none may be made in a block that has not been complete: it has no 8-bit values, and its float32
+ * rows would be lost.) */
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
 
 /* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats

@@ -452,3 +452,40 @@ def test_groups_whose_outputs_fill_the_workgroups_memory(nh, nkv, hs, pos, count
     model.append(k, v, 0)
     q = rng.standard_normal((count, nh * hs)).astype(np.float32)
     within(cache.attention(q, k[pos:], v[pos:], pos, nh), model, q, pos, nh)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_steps_back_one_after_the_other(seed):
+    """steps back by the rule hk_cache_append states: the float32 rows that are held lie behind the furthest position
+    written, not behind the last call's end; anywhere else goes through hk_cache_rewind. The first sequence: 300 positions,
+    one token at 204, then back to 120"""
+    nh, nkv, hs, seq = 4, 2, 32, 700
+    rng = np.random.default_rng(seed)
+    cache, model = Cache(nkv, hs, seq), Model(nkv, hs, seq)
+    start = furthest = end = whole = 0
+    for step in range(12):
+        if seed == 0 and step < 3:
+            pos, count = ((0, 300), (204, 1), (120, 50))[step]
+        else:
+            back = [0, int(rng.integers(0, 97)), int(rng.integers(0, end + 1))][int(rng.integers(0, 3))]
+            pos = max(0, end - back)
+            count = min(int(rng.choice([1, 2, 30, 100, 200])), seq - pos)
+            if count < 1:
+                pos, count = 450, 1
+        first = pos // BLOCK * BLOCK
+        if not (max(start, furthest - RECENT) <= first and pos <= furthest):
+            if pos % BLOCK:
+                cache.rewind(pos)
+                model.rewind(pos)
+            start, furthest = first, pos
+        k, v = rows(rng, count, nkv, hs)
+        cache.append(k, v, pos)
+        model.append(k, v, pos)
+        end = pos + count
+        furthest, whole = max(furthest, end), max(whole, end)
+        same_blocks(cache, model, whole)
+        q = rng.standard_normal((count, nh * hs)).astype(np.float32)
+        got = cache.attention(q, k, v, pos, nh)
+        for i in {0, count - 1}:
+            within(got[i:i + 1], model, q[i:i + 1], pos + i, nh)
+        np.testing.assert_array_equal(cache.read(0, end, end), model.read(0, end, end).astype(np.float32))
