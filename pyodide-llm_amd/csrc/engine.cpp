@@ -1189,7 +1189,8 @@ int32_t he_generate_many(he_engine *e, int32_t token, int32_t pos, const int32_t
   (void)length;
   if (!e || !ids || !n_ids) return fail(HE_E_ARG, "a required pointer is null");
   if (count < 1) return fail(HE_E_ARG, "count must be at least 1");
-  if ((int64_t)pos + count > e->c.seq_len) return fail(HE_E_STATE, "the steps run past the context (seq_len)");
+  if (pos < 0 || (int64_t)pos + count > e->c.seq_len)
+    return fail(HE_E_STATE, "the steps run past the context (seq_len)");
   if (token < 0 || token >= e->c.vocab_size) return fail(HE_E_ARG, "a token is outside the vocabulary");
   if (n_history < 0 || (n_history > 0 && !history)) return fail(HE_E_ARG, "history is null");
   for (int32_t i = std::max(0, n_history - REPETITION_WINDOW); i < n_history; ++i)

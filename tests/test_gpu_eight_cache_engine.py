@@ -498,3 +498,15 @@ def test_rows_behind_the_end_are_no_other_positions(count):
     np.testing.assert_array_equal(inside, got[:, :, count - 5:count + 15])
     beyond = eng.keysAndValues(count + 3, 9)
     assert all((beyond[name] == 0).all() for name in beyond)
+
+
+@pytest.mark.parametrize("kv", [0, 8])
+def test_steps_before_the_first_position_are_refused(kv):
+    """by replayed steps too, whose position only the device looks at"""
+    eng = opened(FIELDS, kv)[0]
+    eng.forwardMany(tokens(5), 0)
+    assert len(eng.generateMany(7, 5, [], 0, 6, 0.0, 0.9, 1.0, [], [])) == 6  # (from here on steps are replayed)
+    for pos in (-1, -64, -2147483648):
+        with pytest.raises(package().HipError):
+            eng.generateMany(7, pos, [], 0, 6, 0.0, 0.9, 1.0, [], [])
+    assert len(eng.generateMany(7, 11, [], 0, 6, 0.0, 0.9, 1.0, [], [])) == 6
