@@ -510,3 +510,182 @@ def test_steps_before_the_first_position_are_refused(kv):
         with pytest.raises(package().HipError):
             eng.generateMany(7, pos, [], 0, 6, 0.0, 0.9, 1.0, [], [])
     assert len(eng.generateMany(7, 11, [], 0, 6, 0.0, 0.9, 1.0, [], [])) == 6
+
+
+def distribution(x):
+    x = x.astype(np.float64)
+    return x - x.max(-1, keepdims=True) - np.log(np.exp(x - x.max(-1, keepdims=True)).sum(-1, keepdims=True))
+
+
+def held_together(got, lp, given, top):
+    """score()'s rows against the rows' whole distributions lp (float64, each off by 2^-16 at most)"""
+    np.testing.assert_allclose(got["logp"], np.take_along_axis(lp, given, 1), atol=2.0 ** -15, rtol=0)
+    np.testing.assert_allclose(got["entropy"], -(np.exp(lp) * lp).sum(-1), atol=1e-3, rtol=0)
+    order = np.argsort(-lp, axis=1, kind="stable")[:, :top]
+    np.testing.assert_allclose(got["logps"], np.take_along_axis(lp, order, 1), atol=2.0 ** -15, rtol=0)
+    np.testing.assert_allclose(np.take_along_axis(lp, got["ids"].astype(np.int64), 1), got["logps"], atol=2.0 ** -15, rtol=0)
+    assert all(len(set(row)) == top for row in got["ids"].tolist())
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+def test_scores_over_8_bits_are_of_one_pass(form):
+    """every output of a pass over 8 bits against the log probabilities of the whole vocabulary that the same pass gives; and
+    the distributions near the steps' own (a row of another token lies ten times as far)"""
+    ids = tokens(150)
+    vocab = np.tile(np.arange(320), (150, 1))
+    lp = opened(FORMS[form], 8)[0].score(ids, 0, given=vocab)["logp"].astype(np.float64)
+    np.testing.assert_allclose(np.exp(lp).sum(1), 1.0, atol=1e-4)
+    given = np.random.default_rng(1).integers(0, 320, (150, 3))
+    held_together(opened(FORMS[form], 8)[0].score(ids, 0, given=given, top=7), lp, given, 7)
+    text = opened(FORMS[form], 8)[0].score(ids, 0, top=7)
+    held_together({n: x[:-1] for n, x in text.items()}, lp[:-1], np.array(ids[1:])[:, None], 7)
+    assert np.isnan(text["logp"][-1, 0])
+    one = opened(FORMS[form], 8)[0]
+    steps = []
+    for i, t in enumerate(ids):
+        one.forward(t, i)
+        steps.append(distribution(one.logits()))
+    steps = np.array(steps)
+    near = np.sqrt(np.mean((steps - lp) ** 2, 1))
+    for shift in (1, 2, 7):
+        assert near.max() < np.sqrt(np.mean((steps[shift:] - lp[:-shift]) ** 2, 1)).min()
+
+
+def test_one_tokens_scores_over_8_bits_are_its_steps():
+    """a pass of one token is the step that forward() runs: its log probabilities are those of the step's logits"""
+    ids = tokens(120)
+    eng, one = opened(FIELDS, 8)[0], opened(FIELDS, 8)[0]
+    for i, t in enumerate(ids):
+        one.forward(t, i)
+        got, lp = eng.score([t], i, given=[[5, 9]], top=4), distribution(one.logits())[None]
+        held_together(got, lp, np.array([[5, 9]]), 4)
+
+
+@pytest.mark.parametrize("kv", [0, 8])
+def test_scores_of_a_long_text_and_a_large_vocabulary(kv):
+    """more tokens than a pass runs and than logits are held at once; rows in several parts; fewer tokens asked about first, so
+    that what holds them grows: every output of every row"""
+    fields = dict(FIELDS, vocab_size=9001, seq_len=1500)
+    eng, cfg = opened(fields, kv, 2048)[:2]
+    few = eng.score(tokens(3, 9001), 0, top=2)
+    ids = tokens(1400, 9001, seed=5)
+    given = np.random.default_rng(2).integers(0, 9001, (1400, 2))
+    got = eng.score(ids, 0, given=given, top=6)
+    if kv == 0:
+        one, lp = opened(fields, 0)[0], []
+        for i, t in enumerate(ids):
+            one.forward(t, i)
+            lp.append(distribution(one.logits()))
+        held_together(got, np.array(lp), given, 6)
+    else:
+        # the same pass again, asked for a part of the vocabulary: what it shares with the first is the same to the bit
+        again = eng.score(ids, 0, given=got["ids"], top=0)
+        np.testing.assert_array_equal(again["logp"], got["logps"])
+        np.testing.assert_array_equal(again["entropy"], got["entropy"])
+        full = opened(fields, 0, 2048)[0].score(ids, 0, given=given, top=6)
+        assert np.mean(np.abs(full["logp"] - got["logp"])) < 0.05 < np.mean(np.abs(full["logp"][1:] - got["logp"][:-1]))
+        assert np.mean(full["ids"][:, 0] == got["ids"][:, 0]) > 0.9
+    assert few["ids"].shape == (3, 2)
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+def test_a_turn_taken_again_is_the_turn_itself(form):
+    """back within the latest positions, once and twice: the logits and the cache of a conversation that was split the same way
+    and never went on, to the bit"""
+    first, other, third = tokens(150), tokens(150, seed=9), tokens(150, seed=10)
+    eng, plain = (opened(FORMS[form], 8)[0] for _ in range(2))
+    for e in (eng, plain):
+        e.forwardMany(first[:60], 0)
+        e.forwardMany(first[60:100], 60)
+    eng.forwardMany(first[100:150], 100)
+    for at, ids in ((100, other), (70, third)):
+        for e in (eng, plain):
+            if at == 100 or e is eng:
+                e.forwardMany(ids[:30], at)
+                e.forward(ids[30], at + 30)
+        if at == 70:
+            plain = opened(FORMS[form], 8)[0]
+            plain.forwardMany(first[:60], 0)
+            plain.forwardMany(first[60:70], 60)
+            plain.forwardMany(ids[:30], at)
+            plain.forward(ids[30], at + 30)
+        if at == 100:
+            np.testing.assert_array_equal(eng.logits(), plain.logits())
+            a, b = (e.keysAndValues(0, at + 31) for e in (eng, plain))
+            for name in a:
+                np.testing.assert_array_equal(a[name], b[name])
+        else:  # (positions 60..69 came with another split: the same keys and values in the first layer)
+            np.testing.assert_array_equal(*(rows_of(e.keysAndValues(0, 101), e.config, 101)[:, 0] for e in (eng, plain)))
+
+
+WIDE = dict(dim=1024, hidden_dim=2048, n_layers=2, n_heads=8, n_kv_heads=2, head_size=128, vocab_size=2000, seq_len=1200,
+            shared_classifier=1)
+
+
+def attention32(cache, q, pos, nh):
+    """cl.Model.attention of one token in NumPy's float32"""
+    hs, first = cache.hs, pos // cl.BLOCK
+    q = q.reshape(nh, hs).astype(np.float32)
+    k, v = (np.concatenate([cache.eight(w, b) for b in range(first)] + [cache.rows[w, first * cl.BLOCK:pos + 1]]).astype(np.float32)
+            for w in range(2))
+    out = np.zeros((1, nh, hs))
+    for h in range(nh):
+        g = h // (nh // cache.nkv)
+        s = k[:, g] @ q[h] / np.float32(np.sqrt(hs))
+        e = np.exp(s - s.max())
+        out[0, h] = e @ v[:, g] / e.sum()
+    return out, None
+
+
+@pytest.mark.parametrize("fields", [WIDE, dict(WIDE, dim=2048, n_heads=16, n_kv_heads=8),
+                                    dict(WIDE, n_heads=4, n_kv_heads=4, head_size=256)])
+def test_wider_models(fields, monkeypatch):
+    """the first layer's cache exactly; logits as near to the oracle's kernels with the attention over the NumPy cache in float64
+    as with that attention in NumPy's float32 (twice as far at most: both are float32 roundings that move an activation to the
+    next of its steps, more of them the wider a layer is); replayed steps equal to eager ones to the bit"""
+    ids = tokens(1000, 2000)
+    full, cfg = opened(fields, 0, 1024)[:2]
+    eight, _, tensors, ck, cos, sin = opened(fields, 8, 1024)
+    for e in (full, eight):
+        e.forwardMany(ids, 0)
+    want = rows_of(full.keysAndValues(0, 1000), cfg, 1000)[:, 0]
+    model = cl.Model(cfg.n_kv_heads, cfg.head_size, cfg.seq_len)
+    model.append(want[0], want[1], 0)
+    np.testing.assert_array_equal(rows_of(eight.keysAndValues(0, 1000), cfg, 1000)[:, 0],
+                                  model.read(0, 1000, 1000).astype(np.float32))
+    ref, other = (Forward(cfg, tensors, ck, cos, sin) for _ in range(2))
+    for cache in other.caches:
+        cache.attention = lambda q, pos, nh, cache=cache: attention32(cache, q, pos, nh)
+    own, inherent, prompts = [], [], []
+    for i, t in enumerate(ids[:110]):
+        want = ref.step(t, i)
+        eight.forward(t, i)
+        for x, off in ((eight.logits(), own), (other.step(t, i), inherent)):
+            off.append(np.sqrt(np.mean((x - want) ** 2)) / want.std())
+        if i >= 100:
+            prompt = opened(fields, 8, 1024)[0]
+            prompt.forwardMany(ids[:i], 0)
+            prompt.forward(t, i)
+            prompts.append(np.sqrt(np.mean((prompt.logits() - want) ** 2)) / want.std())
+    assert np.mean(own[32:]) < 2 * np.mean(inherent[32:]), (np.mean(own[32:]), np.mean(inherent[32:]))
+    assert np.mean(prompts) < 2 * np.mean(inherent[32:])
+    got = []
+    for graph in ("1", "0"):
+        monkeypatch.setenv("PYODIDE_LLM_HIP_GRAPH", graph)
+        eng = opened(fields, 8, 1024)[0]
+        eng.forwardMany(ids[:-1], 0)
+        got.append((eng.generateMany(ids[-1], 999, [], 0, 60, 0.0, 0.9, 1.0, [], []), np.array(eng.logits())))
+    assert got[0][0] == got[1][0]
+    np.testing.assert_array_equal(got[0][1], got[1][1])
+
+
+def test_scores_at_the_end_of_a_long_text_follow_the_float32_caches():
+    """40,000 positions behind the tokens, nearly as many as the ordered attention takes"""
+    n, ids = 40000, tokens(40200)
+    full, eight = opened(dict(FIELDS, seq_len=40400), 0, 1024)[0], opened(dict(FIELDS, seq_len=45000), 8, 1024)[0]
+    lp = []
+    for e in (full, eight):
+        for at in range(0, n, 1024):
+            e.forwardMany(ids[at:min(n, at + 1024)], at)
+        lp.append(e.score(ids[n:], n, given=[[5, 9, 77, 200]] * 200)["logp"])
+    assert np.sqrt(np.mean((lp[0] - lp[1]) ** 2)) < 0.1 * np.sqrt(np.mean((lp[0][1:] - lp[1][:-1]) ** 2))
