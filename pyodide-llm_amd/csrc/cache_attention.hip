@@ -13,10 +13,11 @@
 // scales differ.
 //
 // What bounds it: 32 rows by 32 positions of 128 channels take 28 MFMAs (890 cycles) and about 290 VALU instructions (1200),
-// and the two add up, whichever wave of a SIMD they are of: 2048 tokens of 32 / 8 heads of 128 from the start take 93 us, 1001
-// of 28 / 4 at 20,003 570 to 610 (500 TFLOP/s of the attention's 4 hs a score). One token over 131,077 positions, 268 MB,
-// takes 54 to 58 us (4.7 TB/s; a plain streaming read of as much 44); over 4077 9.6, which is latency: a chain of loads,
-// products and two barriers for the token's own block, a second launch that joins the parts.
+// and a launch takes about as long as the two one after the other (two waves a SIMD, each with its own in turn): 2048 tokens of
+// 32 / 8 heads of 128 from the start take 88 to 92 us, 1001 of 28 / 4 at 20,003 580 to 590 (500 TFLOP/s of the attention's 4 hs
+// a score). One token over 131,077 positions, 268 MB, takes 54 us (4.9 TB/s; a plain streaming read of as much 44); over 4077
+// 9.6, which is latency: a chain of loads, products and two barriers for the token's own block, a second launch that joins the
+// parts.
 #include <algorithm>
 
 #include "cache.hpp"
@@ -30,7 +31,6 @@ typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float DIGITS = 4160000.0f;  // a query's largest value in digits (below 2^22 - 0x8080)
