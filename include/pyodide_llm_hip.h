@@ -366,7 +366,7 @@ int32_t hk_cache_read(void *keys, void *values, const hk_cache *cache, int32_t f
  * rows would be lost.) */
 int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream);
 
-/* The log probabilities of tokens under softmax(logits) of m rows of n (at most 2^30) float32 logits, stride floats
+/* The log probabilities of tokens under softmax(logits) of m rows of n float32 logits (each at most 2^30), stride floats
  * apart (stride >= n, any alignment of 4 bytes): logp[i][g] = log softmax(row i)[given[i][g]] for the n_given tokens
  * given [m][n_given] int32 (NaN where one is outside 0..n-1; null with n_given 0), the entropy [m] in nats (or null),
  * and the `top` (0..HK_LOGPROBS_TOP_MOST) largest alternatives, ids [m][top] int32 and logps [m][top], the lowest index

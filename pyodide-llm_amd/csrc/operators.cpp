@@ -150,8 +150,8 @@ int32_t hk_cache_rewind(const hk_cache *cache, int32_t pos, void *stream) {
 }
 
 int64_t hk_logprobs_workspace(int32_t m, int32_t n, int32_t top) {
-  if (m < 1 || n < 1 || n > 1 << 30 || top < 0 || top > HK_LOGPROBS_TOP_MOST)
-    return failed(HE_E_ARG, "hk_logprobs: m and n are at least 1, n at most 2^30, top in 0..HK_LOGPROBS_TOP_MOST (32)");
+  if (m < 1 || m > 1 << 30 || n < 1 || n > 1 << 30 || top < 0 || top > HK_LOGPROBS_TOP_MOST)
+    return failed(HE_E_ARG, "hk_logprobs: m and n are in 1..2^30, top in 0..HK_LOGPROBS_TOP_MOST (32)");
   return logprobs_workspace(m, n, top);
 }
 

@@ -102,3 +102,10 @@ def test_reads_into_rows_that_are_not_aligned(change):
     to = dict(keys=1 << 20, values=1 << 21)
     to.update(change)
     refused(package().library().hk_cache_read(to["keys"], to["values"], ctypes.byref(cache()), 0, 4, 8, None), text=b"16-byte")
+
+
+@pytest.mark.parametrize("m, n", [((1 << 30) + 1, 1), (2147483647, 1), (1, (1 << 30) + 1), (2147483647, 2147483647)])
+def test_more_rows_or_logits_than_are_counted(m, n):
+    refused(package().library().hk_logprobs_workspace(m, n, 0), text=b"2^30")
+    refused(package().library().hk_logprobs(1 << 21, 1 << 22, None, None, 1 << 20, n, 1 << 25, 1, m, n, 0, 1 << 26, 1 << 40, None),
+            text=b"2^30")
