@@ -383,6 +383,112 @@ int32_t hk_logprobs(void *logp, void *entropy, void *ids, void *logps, const voi
 /* the bytes of workspace an hk_logprobs of these sizes takes (negative: HE_E_ARG) */
 int64_t hk_logprobs_workspace(int32_t m, int32_t n, int32_t top);
 
+/* ---- a cache in pages, which several sequences share, and the attention of their new tokens (no counterpart in the
+ * reference: its caches hold one sequence) ----
+ *
+ * The buffers are the caller's (device memory, 16-byte aligned):
+ *   keys, values  [n_layers][n_pages][n_kv_heads][page_size][head_size], float32, or float16 with half
+ *   tables int32  [n_seqs][table_size]: the page of a sequence's positions page_size * slot.., or -1 where it has none
+ *   refs   int32  [n_pages]: how many entries of the tables name the page; 0: free
+ * The tables start as -1, the refs as 0. page_size is one of 32, 64, 128, 256, head_size one of 16, 32, 48, 64, 96, 128, 256,
+ * n_seqs at most HK_PAGES_SEQS_MOST, table_size * page_size at most HK_PAGES_MOST, n_pages at most HK_PAGES_PAGES_MOST.
+ *
+ * A sequence is a row of the tables; how many positions it has is the caller's to know. The lists that a call takes (sequences,
+ * positions, lengths) are device memory too, so that a captured graph may be replayed with others. A negative sequence in a
+ * list is passed over: lists may be filled up. None of these calls allocates or waits: they may be captured into a graph.
+ * Calls on one cache are ordered by the caller (one stream, or events); hk_pages_append and hk_pages_attention of different
+ * layers may overlap.
+ *
+ * A step of a program that answers n sequences: hk_pages_reserve for each one's next position, then layer by layer
+ * hk_pages_append of the new keys and values and hk_pages_attention over one position more. */
+#define HK_PAGES_SEQS_MOST 8192
+#define HK_PAGES_MOST 1073741824
+#define HK_PAGES_PAGES_MOST 16777216
+typedef struct hk_pages {
+  void *keys;
+  void *values;
+  void *tables;
+  void *refs;
+  int32_t n_layers;
+  int32_t n_pages;
+  int32_t n_kv_heads;
+  int32_t page_size;
+  int32_t head_size;
+  int32_t half;
+  int32_t n_seqs;
+  int32_t table_size;
+} hk_pages;
+
+/* Sequences that go on from others: for each i < n (1..HK_PAGES_SEQS_MOST), sequence to[i] holds the pages of sequence from[i]
+ * that its first lengths[i] positions lie in, and no others; what it held before is given back. Nothing is copied: the pages
+ * are shared until hk_pages_reserve parts them. All entries take from the tables as they were before the call, so that beams
+ * may change places in one call. A sequence may be in `from` often, in `to` once. *status (device int32, or null): 0, or -1
+ * where the lists are not such as this (a sequence past the tables, or in `to` twice; a length outside 0..table_size *
+ * page_size): then nothing is changed. */
+int32_t hk_pages_fork(const hk_pages *pages, const void *to, const void *from, const void *lengths, int32_t n, void *status,
+                      void *stream);
+
+/* Room to write: for each i < n (1..HK_PAGES_SEQS_MOST), every position starts[i]..ends[i] - 1 of sequence seqs[i] gets a page
+ * that it alone names. Where there is none yet, or one that is shared as the call begins, the lowest free page is taken, in
+ * the order of the list and of its positions; of a shared page with positions before starts[i], those rows are copied, in all
+ * layers. A sequence may be listed once. *status (device int32, or null): 0; or how many free pages are lacking, or -1 where
+ * the lists are not such as this (a sequence past the tables or listed twice, a position outside 0..table_size * page_size):
+ * then nothing is changed. workspace: at least hk_pages_workspace bytes (16-byte aligned), not shared by calls that may
+ * overlap. */
+int32_t hk_pages_reserve(const hk_pages *pages, const void *seqs, const void *starts, const void *ends, int32_t n,
+                         void *status, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Sequences that end, or are cut: sequence seqs[i] keeps the pages of its first kept[i] positions (kept null: none) and gives
+ * the others back. Sequences past the tables are passed over; of one listed twice the smaller number holds. */
+int32_t hk_pages_free(const hk_pages *pages, const void *seqs, const void *kept, int32_t n, void *stream);
+
+/* The pages in use together at the pool's beginning: of u pages in use, those at u or past it go to the free places below, in
+ * order (the first to the lowest), the others stay; the tables and refs follow. *used (device int32, or null) is u: the pages
+ * from it on are free then. workspace as for hk_pages_reserve. */
+int32_t hk_pages_compact(const hk_pages *pages, void *used, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* the bytes of workspace that hk_pages_reserve and hk_pages_compact take (negative: HE_E_ARG) */
+int64_t hk_pages_workspace(const hk_pages *pages);
+
+/* The keys and values of n rows into layer `layer`: row i to position positions[i] of sequence seqs[i] (seqs null: i). k and v
+ * float32, n_kv_heads * head_size values a row, kv_stride floats apart (a multiple of 4; k and v 16-byte aligned), rounded to
+ * the nearest, ties to even, where the cache is half. Rows whose sequence or position is outside the tables, or whose position
+ * has no page, are dropped. No two rows go to one position. */
+int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, const void *v, int32_t kv_stride,
+                        const void *seqs, const void *positions, int32_t n, void *stream);
+
+/* The attention of one token a row: out[i][h] = softmax_j(q[i][h] . k_j / sqrt(head_size)) v_j over the positions j <
+ * lengths[i] of sequence seqs[i] (seqs null: i) in layer `layer`, query head h with kv head h / (n_heads / n_kv_heads). q and
+ * out float32, n_heads * head_size values a row, q_stride and out_stride floats apart (multiples of 4; pointers 16-byte
+ * aligned); n_heads is a multiple of n_kv_heads, at most HK_CACHE_GROUP_MOST times it; n in 1..65535. Several
+ * rows may be of one sequence (the tokens of a turn, at lengths one apart). lengths[i] is at most `longest`, which the
+ * launches are made for. A row of length 0 (or less), or of a negative sequence, is zeros; one whose length is past `longest`
+ * or the tables, or whose sequence is, or a position of which has no page, is NaN. What lies behind a row's length has no
+ * part in it, whatever it is. A q that is not finite makes its own row NaN, a key that is not finite the rows that see it,
+ * a value that is not finite their channel not finite. Sums are float32's; a half cache's products keep float32's bits.
+ * workspace: at least hk_pages_attention_workspace bytes (16-byte aligned; nothing in it is kept from one call to the next),
+ * not shared by calls that may overlap. */
+int32_t hk_pages_attention(void *out, const void *q, const hk_pages *pages, int32_t layer, int32_t n_heads,
+                           int32_t q_stride, int32_t out_stride, const void *seqs, const void *lengths, int32_t n,
+                           int32_t longest, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* the bytes of workspace an hk_pages_attention of n rows of at most `longest` positions takes (negative: HE_E_ARG) */
+int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int32_t n, int32_t longest);
+
+/* ---- 4-bit matrices (no counterpart in the reference: its matrices have 8 and 6 bits) ----
+ *
+ * y[t][r] = sum_g ws xs[t][g] (sum over the 32 columns i of group g of w[r][i] (xq[t][i] - bias)) for m tokens and rows
+ * r < rows: w in -8..7, its scale ws one a row and `group` (32, 64 or 128) columns; xq [m][k] and xs [m][k / 32] as
+ * hk_quantize_x leaves them with the same bias (64 or 0). The sums within a group are exact in int32; those over the groups
+ * float32's, in an order of the kernel's own. y is [m][rows] float32. k is a multiple of 32.
+ *
+ * A row of w, and its scales, are filled up with zeros to a multiple of 128 columns. 128 columns are 64 bytes; the 16-byte chunk j of them holds
+ * in byte 4 t + i column 32 t + 4 j + i in its low four bits and column 32 t + 16 + 4 j + i in its high four (two's complement).
+ * ws is [rows][those columns / group], float32, or float16 with half_scales. w is 16-byte aligned, xq 4-byte; the others lie
+ * as their types do, ws 16-byte aligned. Neither allocates nor waits. */
+int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, const void *ws, int32_t m, int32_t rows,
+                       int32_t k, int32_t bias, int32_t group, int32_t half_scales, void *stream);
+
 /* The memory's read ceiling, kernels/ceilings.ts:9-25 read(p, bytes, passes) on the device: bytes (a multiple of 64)
  * at the device pointer p read by a streaming kernel in each of a few launch shapes (8 to 16 loads of 16 bytes a lane
  * in flight, 256 to 2048 blocks), one untimed pass then passes timed ones a shape. *checksum is read()'s: the xor of

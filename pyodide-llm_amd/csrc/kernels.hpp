@@ -236,6 +236,54 @@ struct CacheAttn {
 hipError_t launch_cache_attention(const CacheAttn &a, hipStream_t s);
 int64_t cache_attention_workspace(const CacheView &c, int32_t nh, int32_t count);
 
+// ---- the cache in pages (hk_pages), which several sequences share ----
+// the pools keys / values [layers][n_pages][nkv][page][hs] (float16 or float32), the tables int32 [n_seqs][slots] (a page, or -1)
+// and the pages' counts of table entries
+struct PagesView {
+  void *keys, *values;
+  int32_t *tables, *refs;
+  int32_t layers, n_pages, nkv, page, hs, half, n_seqs, slots;
+};
+constexpr int32_t PAGES_SEQS_MOST = 8192;  // HK_PAGES_SEQS_MOST: sequences of the tables, and entries of a call's lists
+hipError_t launch_pages_fork(const PagesView &c, const int32_t *to, const int32_t *from, const int32_t *lengths, int32_t n,
+                             int32_t *status, hipStream_t s);
+hipError_t launch_pages_reserve(const PagesView &c, const int32_t *seqs, const int32_t *starts, const int32_t *ends, int32_t n,
+                                int32_t *status, int32_t *workspace, hipStream_t s);
+hipError_t launch_pages_free(const PagesView &c, const int32_t *seqs, const int32_t *kept, int32_t n, hipStream_t s);
+hipError_t launch_pages_compact(const PagesView &c, int32_t *used, int32_t *workspace, hipStream_t s);
+int64_t pages_workspace(const PagesView &c);  // bytes, of reserve and of compact
+// rows k / v [count][stride] (kv heads side by side) of layer `layer` to positions[i] of sequence seqs[i] (null: i)
+struct PagesRows {
+  PagesView c;
+  const float *k, *v;
+  const int32_t *seqs, *positions;
+  int32_t layer, stride, count;
+};
+hipError_t launch_pages_append(const PagesRows &a, hipStream_t s);
+// the attention of rows q [rows][q_stride] over the first lengths[i] (at most `longest`) positions of sequence seqs[i] (null: i)
+struct PagesAttn {
+  PagesView c;
+  const float *q;
+  float *out;
+  const int32_t *seqs, *lengths;
+  int32_t layer, nh, q_stride, out_stride, rows, longest;
+  float *workspace;  // pages_attention_workspace() bytes
+  int32_t chunk, parts;  // set by the launch: positions a part, parts of the longest row
+};
+hipError_t launch_pages_attention(const PagesAttn &a, hipStream_t s);
+int64_t pages_attention_workspace(const PagesView &c, int32_t nh, int32_t rows, int32_t longest);
+
+// ---- products with 4-bit matrices (hk_matmul_four) ----
+struct FourArgs {
+  float *y;                // [m][rows]
+  const int8_t *xq;        // [m][k]
+  const float *xs;         // [m][k / 32]
+  const uint8_t *w;        // [rows][k up to a multiple of 128, / 2]
+  const void *ws;          // [rows][k up to a multiple of 128, / group], float16 or float32
+  int32_t m, rows, k, bias, group, half;
+};
+hipError_t launch_matmul_four(const FourArgs &a, hipStream_t s);
+
 // the log probabilities of given tokens [m][n_given], the entropy [m] and the top alternatives [m][top] of m rows of
 // logits (stride floats apart) over n tokens
 constexpr int32_t LOGPROBS_TOP_MOST = 32;

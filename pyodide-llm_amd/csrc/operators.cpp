@@ -1,9 +1,10 @@
 // operators.cpp — the C ABI of the operators that stand beside the engine's own kernels (include/pyodide_llm_hip.h): the cache
-// held in 8 bits with its attention, and the log probabilities. Arguments are checked here, before any launch; nothing
+// held in 8 bits with its attention, the cache in pages with its own, products with 4-bit matrices, and the log probabilities. Arguments are checked here, before any launch; nothing
 // allocates or waits.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/pyodide_llm_hip.h"
@@ -15,6 +16,7 @@ using namespace ple;
 namespace {
 
 static_assert(HK_CACHE_BLOCK == CACHE_BLOCK && HK_CACHE_RECENT == CACHE_RECENT, "the cache's sizes");
+static_assert(HK_PAGES_SEQS_MOST == PAGES_SEQS_MOST, "the sequences of a cache in pages");
 static_assert(HK_LOGPROBS_TOP_MOST == LOGPROBS_TOP_MOST, "the alternatives a row");
 
 bool aligned(const void *p, uintptr_t to = 16) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -75,9 +77,194 @@ int32_t heads_of(const char *what, const CacheView &v, int32_t n_heads) {
   return HE_OK;
 }
 
+int32_t pages_of(const char *what, const hk_pages *p, PagesView &v) {
+  if (!p) return failed(HE_E_ARG, std::string(what) + ": pages is null");
+  if (!cache_head_size(p->head_size))
+    return failed(HE_E_ARG, std::string(what) + ": head_size is one of 16, 32, 48, 64, 96, 128, 256");
+  if (p->page_size != 32 && p->page_size != 64 && p->page_size != 128 && p->page_size != 256)
+    return failed(HE_E_ARG, std::string(what) + ": page_size is one of 32, 64, 128, 256");
+  if (p->n_layers < 1 || p->n_layers > 1024 || p->n_kv_heads < 1 || p->n_kv_heads > 1024)
+    return failed(HE_E_ARG, std::string(what) + ": n_layers and n_kv_heads are in 1..1024");
+  if (p->n_pages < 1 || p->n_pages > HK_PAGES_PAGES_MOST || p->n_seqs < 1 || p->n_seqs > HK_PAGES_SEQS_MOST)
+    return failed(HE_E_ARG, std::string(what) + ": n_pages is in 1..HK_PAGES_PAGES_MOST (16777216), n_seqs in 1..HK_PAGES_SEQS_MOST (8192)");
+  if (p->table_size < 1 || (int64_t)p->table_size * p->page_size > HK_PAGES_MOST)
+    return failed(HE_E_ARG, std::string(what) + ": table_size is at least 1, table_size * page_size at most HK_PAGES_MOST (1073741824)");
+  v = {p->keys, p->values, reinterpret_cast<int32_t *>(p->tables), reinterpret_cast<int32_t *>(p->refs), p->n_layers, p->n_pages,
+       p->n_kv_heads, p->page_size, p->head_size, p->half != 0, p->n_seqs, p->table_size};
+  return HE_OK;
+}
+
+int32_t pools_of(const char *what, const hk_pages *p, PagesView &v) {
+  const int32_t rc = pages_of(what, p, v);
+  if (rc) return rc;
+  const void *ptrs[] = {v.keys, v.values, v.tables, v.refs};
+  for (const void *x : ptrs)
+    if (!x || !aligned(x)) return failed(HE_E_ARG, std::string(what) + ": a buffer of the pages is null or not 16-byte aligned");
+  return HE_OK;
+}
+
+int32_t list_of(const char *what, int32_t n, int32_t most, std::initializer_list<const void *> lists) {
+  if (n < 1 || n > most) return failed(HE_E_ARG, std::string(what) + ": n is in 1.." + std::to_string(most));
+  for (const void *x : lists)
+    if (!x || !aligned(x, 4)) return failed(HE_E_ARG, std::string(what) + ": a list is null or not 4-byte aligned");
+  return HE_OK;
+}
+
+// (a list or an output that may be left out)
+int32_t maybe_of(const char *what, const void *p) {
+  return aligned(p, 4) ? HE_OK : failed(HE_E_ARG, std::string(what) + ": a list, status or used is not 4-byte aligned");
+}
+
+int32_t workspace_of(const char *what, const void *workspace, int64_t bytes, int64_t need, const char *from) {
+  if (need > 0 && (!workspace || !aligned(workspace) || bytes < need))
+    return failed(HE_E_ARG, std::string(what) + ": the workspace is null, not 16-byte aligned or smaller than " + from);
+  return HE_OK;
+}
+
+int32_t page_heads_of(const char *what, const PagesView &v, int32_t n_heads) {
+  if (n_heads < 1 || n_heads % v.nkv || n_heads / v.nkv > HK_CACHE_GROUP_MOST)
+    return failed(HE_E_ARG, std::string(what) + ": n_heads is a multiple of n_kv_heads, at most 32 times it");
+  return HE_OK;
+}
+
+const int32_t *ints(const void *p) { return reinterpret_cast<const int32_t *>(p); }
+
 }  // namespace
 
 extern "C" {
+
+int32_t hk_pages_fork(const hk_pages *pages, const void *to, const void *from, const void *lengths, int32_t n, void *status,
+                      void *stream) {
+  const char *what = "hk_pages_fork";
+  PagesView v;
+  int32_t rc = pools_of(what, pages, v);
+  if (!rc) rc = list_of(what, n, HK_PAGES_SEQS_MOST, {to, from, lengths});
+  if (!rc) rc = maybe_of(what, status);
+  if (rc) return rc;
+  return launched(what, launch_pages_fork(v, ints(to), ints(from), ints(lengths), n, reinterpret_cast<int32_t *>(status),
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+
+int32_t hk_pages_reserve(const hk_pages *pages, const void *seqs, const void *starts, const void *ends, int32_t n,
+                         void *status, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *what = "hk_pages_reserve";
+  PagesView v;
+  int32_t rc = pools_of(what, pages, v);
+  if (!rc) rc = list_of(what, n, HK_PAGES_SEQS_MOST, {seqs, starts, ends});
+  if (!rc) rc = maybe_of(what, status);
+  if (!rc) rc = workspace_of(what, workspace, workspace_bytes, pages_workspace(v), "hk_pages_workspace");
+  if (rc) return rc;
+  return launched(what, launch_pages_reserve(v, ints(seqs), ints(starts), ints(ends), n, reinterpret_cast<int32_t *>(status),
+                                             reinterpret_cast<int32_t *>(workspace), reinterpret_cast<hipStream_t>(stream)));
+}
+
+int32_t hk_pages_free(const hk_pages *pages, const void *seqs, const void *kept, int32_t n, void *stream) {
+  const char *what = "hk_pages_free";
+  PagesView v;
+  int32_t rc = pools_of(what, pages, v);
+  if (!rc) rc = list_of(what, n, HK_PAGES_SEQS_MOST, {seqs});
+  if (!rc) rc = maybe_of(what, kept);
+  if (rc) return rc;
+  return launched(what, launch_pages_free(v, ints(seqs), ints(kept), n, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int32_t hk_pages_compact(const hk_pages *pages, void *used, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *what = "hk_pages_compact";
+  PagesView v;
+  int32_t rc = pools_of(what, pages, v);
+  if (!rc) rc = maybe_of(what, used);
+  if (!rc) rc = workspace_of(what, workspace, workspace_bytes, pages_workspace(v), "hk_pages_workspace");
+  if (rc) return rc;
+  return launched(what, launch_pages_compact(v, reinterpret_cast<int32_t *>(used), reinterpret_cast<int32_t *>(workspace),
+                                             reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t hk_pages_workspace(const hk_pages *pages) {
+  PagesView v;
+  const int32_t rc = pages_of("hk_pages_workspace", pages, v);
+  return rc ? rc : pages_workspace(v);
+}
+
+int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, const void *v, int32_t kv_stride,
+                        const void *seqs, const void *positions, int32_t n, void *stream) {
+  const char *what = "hk_pages_append";
+  PagesRows a;
+  int32_t rc = pools_of(what, pages, a.c);
+  if (!rc) rc = list_of(what, n, 1 << 20, {positions});
+  if (!rc) rc = maybe_of(what, seqs);
+  if (rc) return rc;
+  if (layer < 0 || layer >= a.c.layers) return failed(HE_E_ARG, "hk_pages_append: layer is outside 0..n_layers - 1");
+  if (!k || !v || !aligned(k) || !aligned(v)) return failed(HE_E_ARG, "hk_pages_append: k or v is null or not 16-byte aligned");
+  if (kv_stride < a.c.nkv * a.c.hs || kv_stride % 4)
+    return failed(HE_E_ARG, "hk_pages_append: kv_stride is a multiple of 4, at least n_kv_heads * head_size");
+  a.k = reinterpret_cast<const float *>(k);
+  a.v = reinterpret_cast<const float *>(v);
+  a.seqs = ints(seqs);
+  a.positions = ints(positions);
+  a.layer = layer;
+  a.stride = kv_stride;
+  a.count = n;
+  return launched(what, launch_pages_append(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int32_t hk_pages_attention(void *out, const void *q, const hk_pages *pages, int32_t layer, int32_t n_heads,
+                           int32_t q_stride, int32_t out_stride, const void *seqs, const void *lengths, int32_t n,
+                           int32_t longest, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *what = "hk_pages_attention";
+  PagesAttn a;
+  int32_t rc = pools_of(what, pages, a.c);
+  if (!rc) rc = page_heads_of(what, a.c, n_heads);
+  if (!rc) rc = list_of(what, n, 65535, {lengths});
+  if (!rc) rc = maybe_of(what, seqs);
+  if (rc) return rc;
+  if (layer < 0 || layer >= a.c.layers) return failed(HE_E_ARG, "hk_pages_attention: layer is outside 0..n_layers - 1");
+  if (!out || !q || !aligned(out) || !aligned(q))
+    return failed(HE_E_ARG, "hk_pages_attention: out or q is null or not 16-byte aligned");
+  const int64_t width = (int64_t)n_heads * a.c.hs;
+  if (q_stride < width || out_stride < width || q_stride % 4 || out_stride % 4)
+    return failed(HE_E_ARG, "hk_pages_attention: q_stride and out_stride are multiples of 4, at least n_heads * head_size");
+  if (longest < 0 || longest > a.c.slots * a.c.page)
+    return failed(HE_E_ARG, "hk_pages_attention: longest is in 0..table_size * page_size");
+  rc = workspace_of(what, workspace, workspace_bytes, pages_attention_workspace(a.c, n_heads, n, longest),
+                    "hk_pages_attention_workspace");
+  if (rc) return rc;
+  a.q = reinterpret_cast<const float *>(q);
+  a.out = reinterpret_cast<float *>(out);
+  a.seqs = ints(seqs);
+  a.lengths = ints(lengths);
+  a.layer = layer;
+  a.nh = n_heads;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.rows = n;
+  a.longest = longest;
+  a.workspace = reinterpret_cast<float *>(workspace);
+  return launched(what, launch_pages_attention(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int32_t n, int32_t longest) {
+  const char *what = "hk_pages_attention_workspace";
+  PagesView v;
+  int32_t rc = pages_of(what, pages, v);
+  if (!rc) rc = page_heads_of(what, v, n_heads);
+  if (!rc && (n < 1 || n > 65535)) rc = failed(HE_E_ARG, "hk_pages_attention_workspace: n is in 1..65535");
+  if (!rc && (longest < 0 || longest > v.slots * v.page))
+    rc = failed(HE_E_ARG, "hk_pages_attention_workspace: longest is in 0..table_size * page_size");
+  return rc ? rc : pages_attention_workspace(v, n_heads, n, longest);
+}
+
+int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, const void *ws, int32_t m, int32_t rows,
+                       int32_t k, int32_t bias, int32_t group, int32_t half_scales, void *stream) {
+  if (m < 1 || m > 65535 || rows < 1 || rows > 1 << 28 || k < GS || k % GS || k > 1 << 24)
+    return failed(HE_E_ARG, "hk_matmul_four: m is in 1..65535, rows in 1..2^28, k a multiple of 32 up to 2^24");
+  if (bias != 0 && bias != 64) return failed(HE_E_ARG, "hk_matmul_four: bias is 0 or 64");
+  if (group != 32 && group != 64 && group != 128) return failed(HE_E_ARG, "hk_matmul_four: group is 32, 64 or 128");
+  if (!y || !xq || !xs || !w || !ws || !aligned(y, 4) || !aligned(xq, 4) || !aligned(xs, 4) || !aligned(w) || !aligned(ws))
+    return failed(HE_E_ARG, "hk_matmul_four: a pointer is null, w or ws not 16-byte aligned, or y, xq or xs not 4-byte");
+  const FourArgs a = {reinterpret_cast<float *>(y), reinterpret_cast<const int8_t *>(xq), reinterpret_cast<const float *>(xs),
+                      reinterpret_cast<const uint8_t *>(w), ws, m, rows, k, bias, group, half_scales != 0};
+  return launched("hk_matmul_four", launch_matmul_four(a, reinterpret_cast<hipStream_t>(stream)));
+}
 
 int32_t hk_cache_append(const hk_cache *cache, const void *k, const void *v, int32_t kv_stride, int32_t count,
                         int32_t pos, void *stream) {

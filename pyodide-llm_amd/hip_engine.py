@@ -55,6 +55,40 @@ KV_EIGHT = 8  # HE_KV_EIGHT: HeConfig.half_kv of a cache held in 8 bits
 TOP_MOST = 32  # HK_LOGPROBS_TOP_MOST
 
 
+class HkPages(ctypes.Structure):
+    """hk_pages: a cache in pages, by the device addresses of its buffers (pages_shapes() sizes them)"""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("keys", "values", "tables", "refs")] + [
+        (name, ctypes.c_int32) for name in ("n_layers", "n_pages", "n_kv_heads", "page_size", "head_size", "half", "n_seqs",
+                                            "table_size")]
+
+
+def pages_shapes(n_layers, n_pages, n_kv_heads, page_size, head_size, half, n_seqs, table_size):
+    """{buffer of HkPages: (shape, NumPy dtype, what it starts as)} (include/pyodide_llm_hip.h hk_pages)"""
+    pool = (n_layers, n_pages, n_kv_heads, page_size, head_size), "float16" if half else "float32", 0
+    return {"keys": pool, "values": pool, "tables": ((n_seqs, table_size), "int32", -1), "refs": ((n_pages,), "int32", 0)}
+
+
+def quantize_four(matrix, group=32, half_scales=False):
+    """a float matrix [rows][k] (k a multiple of 32) as hk_matmul_four takes it: (w, ws), rows filled up to a multiple of 128
+    columns. A group's scale is its largest magnitude / 7, rounded to its type; a value is the nearest multiple of it (ties to
+    even) in -8..7. A group without a finite scale above 0 is zeros."""
+    x = np.asarray(matrix, dtype=np.float32)
+    if x.ndim != 2 or x.shape[1] % 32 or not x.size:
+        raise ValueError("quantize_four() takes a matrix whose columns are a multiple of 32")
+    if group not in (32, 64, 128):
+        raise ValueError("quantize_four(): group is 32, 64 or 128")
+    rows, k = x.shape
+    x = np.pad(x, ((0, 0), (0, -k % 128))).reshape(rows, -1, group)
+    with np.errstate(over="ignore", invalid="ignore"):
+        ws = (np.abs(x).max(-1) / np.float32(7)).astype(np.float16 if half_scales else np.float32)
+        ws = np.where(np.isfinite(ws), ws, ws.dtype.type(0))
+        wide = ws.astype(np.float64)[..., None]
+        q = np.where(wide > 0, np.rint(np.clip(x / np.where(wide > 0, wide, 1.0), -8, 7)), 0.0).astype(np.int8)
+    # [row][of 128][t][low / high][j][i] -> [row][of 128][j][t][i]
+    q = q.reshape(rows, -1, 4, 2, 4, 4).transpose(3, 0, 1, 4, 2, 5).astype(np.uint8) & 15
+    return np.ascontiguousarray((q[0] | q[1] << 4).reshape(rows, -1)), ws
+
+
 def cache_shapes(n_kv_heads, head_size, seq_len):
     """{buffer of HkCache: (shape, NumPy dtype)} (include/pyodide_llm_hip.h hk_cache)"""
     blocks = -(-seq_len // CACHE_BLOCK)
@@ -134,6 +168,15 @@ def library():
             "hk_cache_rewind": (I32, [P, I32, P]),
             "hk_logprobs": (I32, [P, P, P, P, P, I64, P, I32, I32, I32, I32, P, I64, P]),
             "hk_logprobs_workspace": (I64, [I32, I32, I32]),
+            "hk_pages_fork": (I32, [P, P, P, P, I32, P, P]),
+            "hk_pages_reserve": (I32, [P, P, P, P, I32, P, P, I64, P]),
+            "hk_pages_free": (I32, [P, P, P, I32, P]),
+            "hk_pages_compact": (I32, [P, P, P, I64, P]),
+            "hk_pages_workspace": (I64, [P]),
+            "hk_pages_append": (I32, [P, I32, P, P, I32, P, P, I32, P]),
+            "hk_pages_attention": (I32, [P, P, P, I32, I32, I32, I32, P, P, I32, I32, P, I64, P]),
+            "hk_pages_attention_workspace": (I64, [P, I32, I32, I32]),
+            "hk_matmul_four": (I32, [P, P, P, P, P, I32, I32, I32, I32, I32, I32, P]),
             "hk_read_ceiling": (I32, [P, ctypes.c_int64, I32, P, P, P]),
             "hk_read_floor": (I32, [P, ctypes.c_int64, ctypes.c_int64, I32, P, P]),
             "hk_valu_ceiling": (I32, [I32, F, F, F, P, P, P, P]),
