@@ -484,8 +484,8 @@ int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int
  *
  * A row of w, and its scales, are filled up with zeros to a multiple of 128 columns. 128 columns are 64 bytes; the 16-byte chunk j of them holds
  * in byte 4 t + i column 32 t + 4 j + i in its low four bits and column 32 t + 16 + 4 j + i in its high four (two's complement).
- * ws is [rows][those columns / group], float32, or float16 with half_scales. w is 16-byte aligned, xq 4-byte; the others lie
- * as their types do, ws 16-byte aligned. Neither allocates nor waits. */
+ * ws is [rows][those columns / group], float32, or float16 with half_scales. w, ws and xq are 16-byte aligned, y and xs
+ * 4-byte. Neither allocates nor waits. */
 int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, const void *ws, int32_t m, int32_t rows,
                        int32_t k, int32_t bias, int32_t group, int32_t half_scales, void *stream);
 

@@ -259,8 +259,8 @@ int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, c
     return failed(HE_E_ARG, "hk_matmul_four: m is in 1..65535, rows in 1..2^28, k a multiple of 32 up to 2^24");
   if (bias != 0 && bias != 64) return failed(HE_E_ARG, "hk_matmul_four: bias is 0 or 64");
   if (group != 32 && group != 64 && group != 128) return failed(HE_E_ARG, "hk_matmul_four: group is 32, 64 or 128");
-  if (!y || !xq || !xs || !w || !ws || !aligned(y, 4) || !aligned(xq, 4) || !aligned(xs, 4) || !aligned(w) || !aligned(ws))
-    return failed(HE_E_ARG, "hk_matmul_four: a pointer is null, w or ws not 16-byte aligned, or y, xq or xs not 4-byte");
+  if (!y || !xq || !xs || !w || !ws || !aligned(y, 4) || !aligned(xq) || !aligned(xs, 4) || !aligned(w) || !aligned(ws))
+    return failed(HE_E_ARG, "hk_matmul_four: a pointer is null, w, ws or xq not 16-byte aligned, or y or xs not 4-byte");
   const FourArgs a = {reinterpret_cast<float *>(y), reinterpret_cast<const int8_t *>(xq), reinterpret_cast<const float *>(xs),
                       reinterpret_cast<const uint8_t *>(w), ws, m, rows, k, bias, group, half_scales != 0};
   return launched("hk_matmul_four", launch_matmul_four(a, reinterpret_cast<hipStream_t>(stream)));

@@ -62,10 +62,21 @@ def test_products_at_sizes_where_they_can_go_wrong(rows, k, m, group, half):
 @pytest.mark.parametrize("m", [3, 4, 6, 7, 8, 9, 12, 15, 17, 24, 31, 32, 47, 48, 49, 63, 64, 65, 100, 130])
 def test_any_number_of_tokens(m):
     rng = np.random.default_rng(m)
-    for rows, k in ((100, 416), (1500, 1024)):
+    for rows, k in ((100, 416), (1500, 1024), (20, 40000)):
         xq, xs, w, ws = inputs(rng, m, rows, k, 64, 32, False)
         want, off = product(xq, xs, w, ws, k, 64, 32)
         assert (np.abs(four(xq, xs, w, ws, rows, k, 64, 32) - want) <= off).all()
+
+
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("k", [512, 544, 1024, 1056, 2048, 2080, 4096, 4128, 8192, 8224, 16384, 16416, 32768, 32800])
+def test_rows_of_every_length(m, k):
+    """one token and two, at the lengths between the kernel's shapes; more rows than a launch has places for at the shorter"""
+    rng = np.random.default_rng(k)
+    rows = 70001 if k < 600 else 37
+    xq, xs, w, ws = inputs(rng, m, rows, k, 64, 64, True)
+    want, off = product(xq, xs, w, ws, k, 64, 64)
+    assert (np.abs(four(xq, xs, w, ws, rows, k, 64, 64) - want) <= off).all()
 
 
 def test_every_pair_of_values():

@@ -122,7 +122,7 @@ def test_attention_workspaces_that_are_refused():
     (dict(k=0), b"k a multiple"), (dict(k=48), b"k a multiple"), (dict(k=(1 << 24) + 32), b"k a multiple"), (dict(bias=1), b"bias"),
     (dict(group=16), b"group"), (dict(group=256), b"group"), (dict(group=0), b"group"), (dict(y=None), b"pointer"),
     (dict(xq=None), b"pointer"), (dict(xs=None), b"pointer"), (dict(w=None), b"pointer"), (dict(ws=None), b"pointer"),
-    (dict(w=(1 << 20) + 8), b"16-byte"), (dict(ws=(1 << 20) + 8), b"16-byte"), (dict(xq=(1 << 20) + 2), b"4-byte"),
+    (dict(w=(1 << 20) + 8), b"16-byte"), (dict(ws=(1 << 20) + 8), b"16-byte"), (dict(xq=(1 << 20) + 8), b"16-byte"),
     (dict(y=(1 << 20) + 2), b"4-byte"), (dict(xs=(1 << 20) + 1), b"4-byte")])
 def test_products_that_are_refused(change, text):
     args = dict(y=1 << 20, xq=1 << 20, xs=1 << 20, w=1 << 20, ws=1 << 20, m=2, rows=10, k=64, bias=64, group=32, half=0)
