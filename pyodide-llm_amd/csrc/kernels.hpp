@@ -268,7 +268,10 @@ struct PagesAttn {
   const int32_t *seqs, *lengths;
   int32_t layer, nh, q_stride, out_stride, rows, longest;
   float *workspace;  // pages_attention_workspace() bytes
-  int32_t chunk, parts;  // set by the launch: positions a part, parts of the longest row
+  // set by the launch: the pieces that the rows' positions are cut into, at most; pieces a row and their positions (parts 0: by
+  // the lengths, about `pieces` in all)
+  int64_t most;
+  int32_t parts, chunk, pieces;
 };
 hipError_t launch_pages_attention(const PagesAttn &a, hipStream_t s);
 int64_t pages_attention_workspace(const PagesView &c, int32_t nh, int32_t rows, int32_t longest);

@@ -24,6 +24,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BLOCK = 32;   // positions a wave takes at a time
 constexpr int WAVES = 4;
+constexpr int UNIT = BLOCK * WAVES, LEAST = 2;  // positions of a piece: a multiple of UNIT, at least LEAST of them
+constexpr int PLANNED = 256;  // rows a launch's workgroups look through
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float INF = __builtin_inff();
 constexpr float AHEAD = 8.0f;     // how far (log2) a score may lie above the reference before that moves
@@ -58,35 +60,131 @@ __device__ __forceinline__ float column_max(float x) {
   return column(x, [](float a, float b) { return __builtin_fmaxf(a, b); });
 }
 
-// a wave's accumulators and statistics
+template <int BYTES>
+struct Bits {
+  typedef uint16_t type;
+};
+template <>
+struct Bits<4> {
+  typedef uint32_t type;
+};
+
+// channels a lane reads at once of a value row whose `rest` channels are left
+template <bool HALF>
+__host__ __device__ constexpr int width(int rest) {
+  return HALF && rest >= 128 ? 8 : rest >= 64 ? 4 : rest >= 32 ? 2 : 1;
+}
+
+// a lane's values of 32 positions: channels BASE + W c.. of its eight positions, and those past BASE + 16 W
+template <int HS, bool HALF, int BASE = 0>
+struct Values {
+  typedef typename Kind<HALF>::type T;
+  static constexpr int W = width<HALF>(HS - BASE), AT = BASE / 16;
+  typedef T piece __attribute__((ext_vector_type(W)));
+  piece x[8];
+  Values<HS, HALF, BASE + 16 * W> rest;
+
+  __device__ __forceinline__ void read(const T *v, int c, int j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = *reinterpret_cast<const piece *>(v + ((e & 4) * 4 + 4 * j + (e & 3)) * HS + BASE + W * c);
+    rest.read(v, c, j);
+  }
+  // zeros at the positions from `left` on (what lies behind the row's end may be anything): by masks, since selects of these
+  // vectors became a branch under whose exec mask the compiler reused a value's registers (wrong outputs at heads of 128)
+  __device__ __forceinline__ void cut(int left, int j) {
+    typedef typename Bits<sizeof(T)>::type bits __attribute__((ext_vector_type(W)));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int32_t keep = ((e & 4) * 4 + 4 * j + (e & 3) - left) >> 31;  // all ones before it
+      x[e] = __builtin_bit_cast(piece, __builtin_bit_cast(bits, x[e]) & (bits)((typename Bits<sizeof(T)>::type)keep));
+    }
+    rest.cut(left, j);
+  }
+  // tiles of 16 channels: channel i of each lane's
+  __device__ __forceinline__ void add(f32x4 *o, const f16x8 &ph, const f32x4 (&p)[2]) const {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (HALF) {
+        f16x8 a;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = x[e][i];
+        o[AT + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[AT + i], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          o[AT + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e][i], p[e >> 2][e & 3], o[AT + i], 0, 0, 0);
+      }
+    }
+    rest.add(o, ph, p);
+  }
+};
+template <int HS, bool HALF>
+struct Values<HS, HALF, HS> {
+  typedef typename Kind<HALF>::type T;
+  __device__ __forceinline__ void read(const T *, int, int) {}
+  __device__ __forceinline__ void cut(int, int) {}
+  __device__ __forceinline__ void add(f32x4 *, const f16x8 &, const f32x4 (&)[2]) const {}
+};
+
+// a wave's queries, accumulators and statistics
 template <int HS, bool HALF>
 struct Wave {
   typedef typename Kind<HALF>::type T;
-  static constexpr int KEYS = HALF ? (HS + 31) / 32 : HS / 16;  // loads of a key row
+  typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));  // 16 bytes
+  static constexpr int KEYS = HALF ? (HS + 31) / 32 : HS / 16;       // of them a lane takes of a key row
   static constexpr int TILES = HS / 16;
-  f16x8 qh[HALF ? KEYS : 1];
-  float4 qf[HALF ? 1 : KEYS];
-  float up;        // what a product is multiplied by: a score in log2
-  float top = -INF, reference = 0.0f, sum = 0.0f;
+  float4 raw[HALF ? 2 * KEYS : KEYS];
+  f16x8 q[HALF ? KEYS : 1];
+  chunk k[2][KEYS];
+  Values<HS, HALF> v;
+  float up, up_low;  // what a product is multiplied by: a score in log2
+  // the scores' reference, and how far above it one may lie (-INF: there is no reference yet)
+  float reference = 0.0f, bar = -INF, sum = 0.0f;
   f32x4 o[TILES];
-  int lane, c, j;  // the lane, its column and its quarter
+  int c, j;  // the lane's column and quarter
 
-  // the row's queries of the tile's heads as products take them
-  __device__ __forceinline__ void queries(const float *q, int heads, float scale) {
-    const int h = HALF ? c & 7 : c;
-    const bool mine = h < heads;
-    if constexpr (HALF) {
-      float x[KEYS][8], most = 0.0f;
+  __device__ __forceinline__ static bool within(int d) { return HS % 32 == 0 || !HALF || d < HS; }
+
+  __device__ __forceinline__ void read_queries(const float *from, int heads) {
+    const int h = min(HALF ? c & 7 : c, heads - 1);  // (columns past the heads: the last one's, to no end)
+#pragma unroll
+    for (int s = 0; s < KEYS; ++s) {
+      const int d = HALF ? 32 * s + 8 * j : 16 * s + 4 * j;
+      const float *at = from + h * HS + (within(d) ? d : 0);
+      if constexpr (HALF) {
+        raw[2 * s] = *reinterpret_cast<const float4 *>(at);
+        raw[2 * s + 1] = *reinterpret_cast<const float4 *>(at + 4);
+      } else {
+        raw[s] = *reinterpret_cast<const float4 *>(at);
+      }
+    }
+  }
+  __device__ __forceinline__ void read_keys(const T *from) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int s = 0; s < KEYS; ++s) {
-        const int d = 32 * s + 8 * j;
-        const bool in = mine && (HS % 32 == 0 || d < HS);
-        const float4 a = in ? *reinterpret_cast<const float4 *>(q + h * HS + d) : make_float4(0, 0, 0, 0),
-                     b = in ? *reinterpret_cast<const float4 *>(q + h * HS + d + 4) : make_float4(0, 0, 0, 0);
-        x[s][0] = a.x, x[s][1] = a.y, x[s][2] = a.z, x[s][3] = a.w;
-        x[s][4] = b.x, x[s][5] = b.y, x[s][6] = b.z, x[s][7] = b.w;
+        const int d = HALF ? 32 * s + 8 * j : 16 * s + 4 * j;
+        k[t][s] = *reinterpret_cast<const chunk *>(from + (16 * t + c) * HS + (within(d) ? d : 0));
+      }
+  }
+  __device__ __forceinline__ void read_values(const T *from) { v.read(from, c, j); }
+
+  // the queries as the products take them
+  __device__ __forceinline__ void begin() {
+    const float scale = LOG2E / __builtin_sqrtf((float)HS);
+    if constexpr (HALF) {
+      float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(x[s][i]));
+      for (int s = 0; s < KEYS; ++s) {
+        if (!within(32 * s + 8 * j)) raw[2 * s] = raw[2 * s + 1] = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 x = raw[2 * s + i];
+          most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x.x), __builtin_fabsf(x.y)),
+                                                       __builtin_fmaxf(__builtin_fabsf(x.z), __builtin_fabsf(x.w))));
+        }
       }
       most = column_max(most);
       const int e = __builtin_amdgcn_frexp_expf(most);  // |q| < 2^e; (of 0 and of what is not finite 0)
@@ -94,175 +192,280 @@ struct Wave {
       for (int s = 0; s < KEYS; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float y = __builtin_amdgcn_ldexpf(x[s][i], 15 - e);
+          const float4 x = raw[2 * s + i / 4];
+          const float y = __builtin_amdgcn_ldexpf(i % 4 == 0 ? x.x : i % 4 == 1 ? x.y : i % 4 == 2 ? x.z : x.w, 15 - e);
           const _Float16 hi = (_Float16)y;
-          const _Float16 lo = (_Float16)((y - (float)hi) * LOW);
-          qh[s][i] = c < 8 ? hi : lo;
+          q[s][i] = c < 8 ? hi : (_Float16)((y - (float)hi) * LOW);
         }
-      up = __builtin_amdgcn_ldexpf(scale * LOG2E, e - 15);
-      if (c >= 8) up = up / LOW;
+      up = __builtin_amdgcn_ldexpf(scale, e - 15);
+      up_low = __builtin_amdgcn_ldexpf(scale, e - 26);
     } else {
-#pragma unroll
-      for (int s = 0; s < KEYS; ++s)
-        qf[s] = mine ? *reinterpret_cast<const float4 *>(q + h * HS + 16 * s + 4 * j) : make_float4(0, 0, 0, 0);
-      up = scale * LOG2E;
+      up = scale;
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) o[t] = f32x4{0, 0, 0, 0};
   }
 
-  // the scores of 32 positions whose key rows begin at k: position 16 t + 4 j + r of column c in s[t][r]
-  __device__ __forceinline__ void scores(const T *k, f32x4 (&s)[2]) const {
+  // position 16 t + 4 j + r of column c in s[t][r]
+  __device__ __forceinline__ void products(f32x4 (&s)[2]) const {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f32x4{0, 0, 0, 0};
-      const T *row = k + (16 * t + c) * HS;
+    for (int t = 0; t < 2; ++t) s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < KEYS; ++i) {
+    for (int i = 0; i < KEYS; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         if constexpr (HALF) {
-          const int d = 32 * i + 8 * j;
-          f16x8 x = {};
-          if (HS % 32 == 0 || d < HS) x = *reinterpret_cast<const f16x8 *>(row + d);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh[i], s[t], 0, 0, 0);
+          f16x8 x = k[t][i];
+          if constexpr (HS % 32 != 0) {  // (the last load's upper half is past the row)
+            typedef uint32_t words __attribute__((ext_vector_type(4)));
+            if (i == KEYS - 1) x = __builtin_bit_cast(f16x8, __builtin_bit_cast(words, x) & (words)((uint32_t)((j - 2) >> 31)));
+          }
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[i], s[t], 0, 0, 0);
         } else {
-          const float4 x = *reinterpret_cast<const float4 *>(row + 16 * i + 4 * j);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, qf[i].x, s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, qf[i].y, s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, qf[i].z, s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, qf[i].w, s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i].x, raw[i].x, s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i].y, raw[i].y, s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i].z, raw[i].z, s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i].w, raw[i].w, s[t], 0, 0, 0);
         }
       }
-    }
   }
 
-  // channels BASE.. of the values: tiles of 16 from tile AT on
-  template <int BASE, int AT>
-  __device__ __forceinline__ void values(const T *v, int left, const f16x8 &ph, const f32x4 (&p)[2]) {
-    constexpr int REST = HS - BASE;
-    if constexpr (REST > 0) {
-      constexpr int W = HALF && REST >= 128 ? 8 : REST >= 64 ? 4 : REST >= 32 ? 2 : 1;  // channels a lane
-      typedef T piece __attribute__((ext_vector_type(W)));
-      piece x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int t = (e & 4) * 4 + 4 * j + (e & 3);
-        x[e] = *reinterpret_cast<const piece *>(v + t * HS + BASE + W * c);
-        if (t >= left) x[e] = piece(0);  // (what lies behind the row's end may be anything)
-      }
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if constexpr (HALF) {
-          f16x8 a;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a[e] = x[e][i];
-          o[AT + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[AT + i], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            o[AT + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e][i], p[e >> 2][e & 3], o[AT + i], 0, 0, 0);
-        }
-      }
-      values<BASE + 16 * W, AT + W>(v, left, ph, p);
-    }
-  }
-
-  // 32 positions, `left` of them (or more) before the row's end
-  __device__ __forceinline__ void block(const T *k, const T *v, int left) {
-    f32x4 s[2];
-    scores(k, s);
+  // the products' scores (log2) over the reference, and the largest of the lane's: one rounding at their own size, not at the
+  // scores'
+  __device__ __forceinline__ float scores(const f32x4 (&s)[2], f32x4 (&x)[2], int left) const {
     float most = -INF;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = s[t][r] * up;
-        if (HALF) x = x + other_half(x);
-        if (16 * t + 4 * j + r >= left) x = -INF;
-        s[t][r] = x;
-        most = __builtin_fmaxf(most, x);
+        float y;
+        if constexpr (HALF) {
+          const float other = other_half(s[t][r]);
+          y = __builtin_fmaf(c < 8 ? other : s[t][r], up_low, __builtin_fmaf(c < 8 ? s[t][r] : other, up, -reference));
+        } else {
+          y = __builtin_fmaf(s[t][r], up, -reference);
+        }
+        if (16 * t + 4 * j + r >= left) y = -INF;
+        x[t][r] = y;
+        most = __builtin_fmaxf(most, y);
       }
-    if (__any(most > top + AHEAD)) {
-      const float next = __builtin_fmaxf(top, column_max(most));
-      const float other = next > -INF ? next : 0.0f, less = __builtin_amdgcn_exp2f(top - other);
-      top = next;
-      reference = other;
-      sum *= less;
+    return most;
+  }
+
+  // the probabilities of the products' scores, as the second product takes them; `left` of the positions are the row's
+  __device__ __forceinline__ void probabilities(const f32x4 (&s)[2], int left, f16x8 &ph, f32x4 (&p)[2]) {
+    const float most = scores(s, p, left);
+    if (__any(most > bar)) {
+      const float next = column_max(most);
+      if (next > -INF) {
+        const float more = bar > -INF ? __builtin_fmaxf(next, 0.0f) : next;
+        const float less = bar > -INF ? __builtin_amdgcn_exp2f(-more) : 0.0f;
+        reference += more;
+        bar = AHEAD;
+        sum *= less;
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        // a product's output has the column's statistics in its own lane
-        o[t] *= less;
+        for (int t = 0; t < TILES; ++t) o[t] *= less;
       }
+      scores(s, p, left);
     }
-    f16x8 ph = {};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float p = __builtin_amdgcn_exp2f(s[t][r] - reference);
-        sum += p;
+        float x = __builtin_amdgcn_exp2f(p[t][r]);
+        sum += x;
         if constexpr (HALF) {
-          p *= PIECE_UP;
-          const _Float16 hi = (_Float16)p, lo = (_Float16)((p - (float)hi) * LOW);
-          ph[4 * t + r] = c < 8 ? hi : lo;
+          x *= PIECE_UP;
+          const _Float16 hi = (_Float16)x;
+          ph[4 * t + r] = c < 8 ? hi : (_Float16)((x - (float)hi) * LOW);
         }
-        s[t][r] = p;
+        p[t][r] = x;
       }
-    values<0, 0>(v, left, ph, s);
   }
 };
 
-// channel of element r of quarter j's output in tile n (Wave::values' order)
+// channel of element r of quarter j's output in tile n (Values' order)
 template <int HS, bool HALF>
 __device__ __forceinline__ constexpr int channel(int n, int row) {
-  int base = 0, at = 0;
-  while (true) {
-    const int rest = HS - base, w = HALF && rest >= 128 ? 8 : rest >= 64 ? 4 : rest >= 32 ? 2 : 1;
-    if (n < at + w) return base + w * row + n - at;
-    base += 16 * w;
-    at += w;
+  int base = 0;
+  while (n >= base / 16 + width<HALF>(HS - base)) base += 16 * width<HALF>(HS - base);
+  return base + width<HALF>(HS - base) * row + n - base / 16;
+}
+
+// Which positions of which row a workgroup takes. Up to PLANNED rows a launch, every workgroup works that out from all lengths:
+// the rows' positions, in units of UNIT, over the pieces that the launch is made for, are a piece's; a row longer than one has
+// several, one after another, so that all are about equal whatever the rows' lengths are. Of more rows each has the same
+// number of pieces (which lie behind its end if it is short).
+struct Piece {
+  int row, seq, len;    // len 0: no attention (zeros)
+  bool wrong;           // a row that cannot be (NaN)
+  int chunk;            // positions a piece
+  int first, part;      // the row's first piece, and which of the row's this is
+};
+
+__device__ __forceinline__ bool impossible(const PagesAttn &a, int seq, int len) {
+  return len > 0 && seq >= 0 && (seq >= a.c.n_seqs || len > a.longest || len > a.c.slots * a.c.page);
+}
+
+// the sum over the wave's lanes up to this one
+__device__ __forceinline__ uint32_t up_to(uint32_t x) {
+#define STEP(from, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, from, rows, 0xF, false)
+  STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8
+  STEP(0x112, 0xF);
+  STEP(0x114, 0xF);
+  STEP(0x118, 0xF);
+  STEP(0x142, 0xA);  // the first and third rows' last lanes to the next rows
+  STEP(0x143, 0xC);  // the first half's to the second
+#undef STEP
+  return x;
+}
+
+// `find`: the row, or the piece whose row is looked for (past the last: row -1)
+template <bool ROW>
+__device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane) {
+  Piece p;
+  if (a.parts) {
+    p.row = ROW ? find : find / a.parts;
+    p.part = ROW ? 0 : find % a.parts;
+    p.first = p.row * a.parts;
+    p.chunk = a.chunk;
+    p.len = a.lengths[p.row];
+    p.seq = a.seqs ? a.seqs[p.row] : p.row;
+    p.wrong = impossible(a, p.seq, p.len);
+    if (p.seq < 0 || p.len < 0 || p.wrong) p.len = 0;
+    return p;
   }
+  int len, seq, units;
+  bool wrong;
+  auto read = [&](int row) {
+    len = seq = 0;
+    if (row < a.rows) {
+      len = a.lengths[row];
+      seq = a.seqs ? a.seqs[row] : row;
+    }
+    wrong = impossible(a, seq, len);
+    if (seq < 0 || len < 0 || wrong) len = 0;
+    units = (len + UNIT - 1) / UNIT;
+  };
+  read(lane);
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up_to(units), 63);
+  for (int base = 64; base < a.rows; base += 64) {
+    read(base + lane);
+    total += (uint32_t)__builtin_amdgcn_readlane((int)up_to(units), 63);
+  }
+  // units a piece
+  const int each = min(max(LEAST, (int)((total + a.pieces - 1) / a.pieces)), (a.longest + UNIT - 1) / UNIT);
+  p.chunk = each * UNIT;
+  p.row = -1;
+  for (int base = 0, before = 0; base < a.rows; base += 64) {
+    if (a.rows > 64) read(base + lane);
+    const int mine = base + lane < a.rows ? max(1, (units + each - 1) / each) : 0;
+    const int upto = before + (int)up_to(mine);
+    const uint64_t here = __ballot(ROW ? base + lane == find : upto > find && upto - mine <= find);
+    if (here) {
+      const int l = __builtin_ctzll(here);
+      p.row = base + l;
+      p.first = __builtin_amdgcn_readlane(upto - mine, l);
+      p.part = ROW ? 0 : find - p.first;
+      p.len = __builtin_amdgcn_readlane(len, l);
+      p.seq = __builtin_amdgcn_readlane(seq, l);
+      p.wrong = __builtin_amdgcn_readlane(wrong ? 1 : 0, l);
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return p;
+}
+
+// a piece's results: references and sums [piece][head], then outputs [piece][head][HS]
+__device__ __forceinline__ float2 *statistics(const PagesAttn &a, int64_t piece, int h) {
+  return reinterpret_cast<float2 *>(a.workspace) + piece * a.nh + h;
+}
+template <int HS>
+__device__ __forceinline__ float *outputs(const PagesAttn &a, int64_t piece, int h) {
+  return a.workspace + ((a.most * a.nh * 2 + 3) & ~3) + (piece * a.nh + h) * HS;
+}
+
+// waves a SIMD that the registers are kept for: a block's keys and values, the queries and the outputs
+constexpr int occupancy(int hs, bool half) {
+  return half ? (hs <= 64 ? 4 : hs <= 128 ? 3 : 1) : (hs <= 48 ? 4 : hs <= 64 ? 3 : hs <= 128 ? 2 : 1);
 }
 
 template <int HS, bool HALF>
-__global__ __launch_bounds__(64 * WAVES) void attend_kernel(const PagesAttn a) {
+__global__ __launch_bounds__(64 * WAVES, occupancy(HS, HALF)) void attend_kernel(const PagesAttn a) {
   typedef typename Kind<HALF>::type T;
   constexpr int HEADS = Kind<HALF>::heads;
   __shared__ float tops[WAVES][HEADS], sums[WAVES][HEADS];
   __shared__ float outs[WAVES][HEADS][HS];
   const PagesView &c = a.c;
   const int group = a.nh / c.nkv, tiles = (group + HEADS - 1) / HEADS;
-  const int part = blockIdx.x, g = blockIdx.y / tiles, first = g * group + blockIdx.y % tiles * HEADS, row = blockIdx.z;
+  const int g = blockIdx.y / tiles, first = g * group + blockIdx.y % tiles * HEADS;
   const int heads = min(HEADS, (g + 1) * group - first);
-  const int tid = threadIdx.x, wave = tid >> 6;
-  int len = a.lengths[row];
-  const int32_t seq = a.seqs ? a.seqs[row] : row;
-  if (seq < 0 || len < 0) len = 0;
-  const bool wrong = len > 0 && (seq >= c.n_seqs || len > a.longest || len > c.slots * c.page);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const Piece piece = piece_of<false>(a, blockIdx.x, lane);
+  const int row = piece.row, len = piece.len;
+  if (row < 0) return;
   float *out = a.out + (int64_t)row * a.out_stride + (int64_t)first * HS;
-  if (len == 0 || wrong) {
-    if (part == 0)
-      for (int i = tid; i < heads * HS; i += 64 * WAVES) out[i] = wrong ? __builtin_nanf("") : 0.0f;
+  if (len == 0) {
+    if (piece.part == 0)
+      for (int i = tid; i < heads * HS; i += 64 * WAVES) out[i] = piece.wrong ? __builtin_nanf("") : 0.0f;
     return;
   }
-  const int p0 = part * a.chunk, p1 = min(len, p0 + a.chunk);
-  if (p0 >= len) return;
-  Wave<HS, HALF> w;
-  w.lane = tid & 63;
-  w.c = w.lane & 15;
-  w.j = w.lane >> 4;
-  w.queries(a.q + (int64_t)row * a.q_stride + (int64_t)first * HS, heads, 1.0f / __builtin_sqrtf((float)HS));
-  const int32_t *table = c.tables + (int64_t)seq * c.slots;
+  const int64_t begin = (int64_t)piece.part * piece.chunk;
+  if (begin >= len) return;
+  const int p0 = (int)begin + BLOCK * wave;  // the wave's first block
+  const int p1 = (int)min((int64_t)len, begin + piece.chunk);
+  // the pages of the wave's next 64 blocks, a lane each
+  const int32_t *table = c.tables + (int64_t)piece.seq * c.slots;
+  const int shift = __builtin_ctz(c.page);
   bool lost = false;
-  for (int p = p0 + BLOCK * wave; p < p1; p += BLOCK * WAVES) {
-    int32_t page = table[p / c.page];
-    if ((uint32_t)page >= (uint32_t)c.n_pages) page = 0, lost = true;
-    const int64_t at = ((((int64_t)a.layer * c.n_pages + page) * c.nkv + g) * c.page + p % c.page) * HS;
-    w.block(reinterpret_cast<const T *>(c.keys) + at, reinterpret_cast<const T *>(c.values) + at, p1 - p);
+  auto pages = [&](int p) {
+    const int64_t mine = p + (int64_t)lane * (BLOCK * WAVES);
+    const int32_t page = mine < p1 ? table[mine >> shift] : 0;
+    const bool none = (uint32_t)page >= (uint32_t)c.n_pages;
+    lost = lost || __any(none);
+    return none ? 0 : page;
+  };
+  Wave<HS, HALF> w;
+  w.c = lane & 15;
+  w.j = lane >> 4;
+  w.read_queries(a.q + (int64_t)row * a.q_stride + (int64_t)first * HS, heads);
+  int32_t held = pages(p0);
+  const int64_t layer = (int64_t)a.layer * c.n_pages;
+  auto place = [&](int p, int turn) {
+    if (turn % 64 == 0 && turn) held = pages(p);
+    const int64_t page = __builtin_amdgcn_readlane(held, turn % 64);
+    return (((layer + page) * c.nkv + g) * c.page + (p & (c.page - 1))) * HS;
+  };
+  const T *keys = reinterpret_cast<const T *>(c.keys), *values = reinterpret_cast<const T *>(c.values);
+  int64_t at = 0;
+  if (p0 < p1) {
+    at = place(p0, 0);
+    w.read_keys(keys + at);
+    w.read_values(values + at);
+  }
+  w.begin();
+  for (int p = p0, turn = 0; p < p1; p += BLOCK * WAVES, ++turn) {
+    f32x4 s[2], prob[2];
+    f16x8 ph;
+    w.products(s);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool more = p + BLOCK * WAVES < p1;
+    if (more) {
+      at = place(p + BLOCK * WAVES, turn + 1);
+      w.read_keys(keys + at);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    w.probabilities(s, p1 - p, ph, prob);
+    if (p1 - p < BLOCK) w.v.cut(p1 - p, w.j);
+    w.v.add(w.o, ph, prob);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) w.read_values(values + at);
   }
   if (lost) w.sum = __builtin_nanf("");
   w.sum = column_sum(w.sum);
   if (w.j == 0 && w.c < HEADS) {
-    tops[wave][w.c] = w.top;
+    tops[wave][w.c] = w.bar > -INF ? w.reference : -INF;
     sums[wave][w.c] = w.sum;
   }
 #pragma unroll
@@ -277,7 +480,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(const PagesAttn a) {
       if (w.c < HEADS) outs[wave][w.c][channel<HS, HALF>(t, 4 * w.j + r)] = x;
     }
   __syncthreads();
-  const bool whole = len <= a.chunk;
+  const bool whole = len <= piece.chunk;
   for (int i = tid; i < heads * HS; i += 64 * WAVES) {
     const int h = i / HS, d = i % HS;
     float top = tops[0][h];
@@ -294,57 +497,102 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(const PagesAttn a) {
     if (whole) {
       out[i] = o / sum;
     } else {
-      float *to = a.workspace + (((int64_t)row * a.nh + first + h) * a.parts + part) * (HS + 2);
-      to[2 + d] = o;
-      if (d == 0) to[0] = top, to[1] = sum;
+      outputs<HS>(a, blockIdx.x, first + h)[d] = o;
+      if (d == 0) *statistics(a, blockIdx.x, first + h) = make_float2(top, sum);
     }
   }
 }
 
-// the parts of a (row, head) whose positions are more than one part's
+// the pieces of a (row, head) with more than one: a thread takes four channels of every EACH-th
 template <int HS>
-__global__ __launch_bounds__(HS) void join_kernel(const PagesAttn a) {
-  const int row = blockIdx.y, h = blockIdx.x, d = threadIdx.x;
-  const int len = a.lengths[row];
-  const int32_t seq = a.seqs ? a.seqs[row] : row;
-  if (seq < 0 || seq >= a.c.n_seqs || len <= a.chunk || len > a.longest || len > a.c.slots * a.c.page) return;
-  const int parts = (len + a.chunk - 1) / a.chunk;
-  const float *from = a.workspace + ((int64_t)row * a.nh + h) * a.parts * (HS + 2);
+__global__ __launch_bounds__(256) void join_kernel(const PagesAttn a) {
+  constexpr int QUADS = HS / 4, EACH = 256 / QUADS;
+  __shared__ float tops[4];
+  __shared__ float sums[EACH];
+  __shared__ float4 outs[EACH][QUADS];
+  const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
+  const Piece piece = piece_of<true>(a, row, tid & 63);
+  if (piece.len <= piece.chunk) return;
+  const int parts = (int)(((int64_t)piece.len + piece.chunk - 1) / piece.chunk);
+  const float2 *stats = statistics(a, piece.first, h);
+  const float4 *from = reinterpret_cast<const float4 *>(outputs<HS>(a, piece.first, h));
   float top = -INF;
-  for (int p = 0; p < parts; ++p) top = __builtin_fmaxf(top, from[p * (HS + 2)]);
+  for (int p = tid; p < parts; p += 256) top = __builtin_fmaxf(top, stats[(int64_t)p * a.nh].x);
+  top = wave_all(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
   if (!(top > -INF)) top = 0.0f;
-  float sum = 0.0f, o = 0.0f;
-  for (int p = 0; p < parts; ++p) {
-    const float f = __builtin_amdgcn_exp2f(from[p * (HS + 2)] - top);
-    sum += from[p * (HS + 2) + 1] * f;
-    o += from[p * (HS + 2) + 2 + d] * f;
+  const int part = tid / QUADS, d = tid % QUADS;
+  float sum = 0.0f;
+  float4 o = make_float4(0, 0, 0, 0);
+  if (part < EACH) {
+    for (int p = part; p < parts; p += EACH) {
+      const float2 own = stats[(int64_t)p * a.nh];
+      const float f = __builtin_amdgcn_exp2f(own.x - top);
+      const float4 x = from[(int64_t)p * a.nh * QUADS + d];
+      sum += own.y * f;
+      o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+    }
+    if (d == 0) sums[part] = sum;
+    outs[part][d] = o;
   }
-  a.out[(int64_t)row * a.out_stride + (int64_t)h * HS + d] = o / sum;
+  __syncthreads();
+  if (tid < HS) {
+    float y = 0.0f;
+    sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      y += reinterpret_cast<const float *>(outs[e])[tid];
+      sum += sums[e];
+    }
+    a.out[(int64_t)row * a.out_stride + (int64_t)h * HS + tid] = y / sum;
+  }
 }
-
-// positions a part takes, a multiple of the waves' blocks
-int32_t chunk_of(const PagesView &c, int32_t nh, int32_t rows, int32_t longest) { return 512; }
 
 template <int HS>
 void launch(const PagesAttn &a, hipStream_t s) {
   const int group = a.nh / a.c.nkv, most = a.c.half ? 8 : 16;
-  const dim3 grid(a.parts, a.c.nkv * ((group + most - 1) / most), a.rows);
+  const dim3 grid(a.most, a.c.nkv * ((group + most - 1) / most));
   if (a.c.half) hipLaunchKernelGGL((attend_kernel<HS, true>), grid, dim3(64 * WAVES), 0, s, a);
   else hipLaunchKernelGGL((attend_kernel<HS, false>), grid, dim3(64 * WAVES), 0, s, a);
-  if (a.parts > 1) hipLaunchKernelGGL(join_kernel<HS>, dim3(a.nh, a.rows), dim3(HS), 0, s, a);
+  if (a.most > a.rows) hipLaunchKernelGGL(join_kernel<HS>, dim3(a.nh, a.rows), dim3(256), 0, s, a);
+}
+
+// how a launch of `rows` rows of at most `longest` positions is cut
+void cut(PagesAttn &a) {
+  const int group = a.nh / a.c.nkv, most = a.c.half ? 8 : 16, tiles = a.c.nkv * ((group + most - 1) / most);
+  a.parts = a.pieces = 0;
+  if (a.longest <= (LEAST + 1) * UNIT) {  // every row one piece
+    a.parts = 1;
+    a.chunk = std::max(a.longest, 1);
+    a.most = a.rows;
+  } else if (a.rows <= PLANNED) {
+    const int places = 256 * occupancy(a.c.hs, a.c.half) / tiles;
+    a.pieces = std::max(1, places - std::min(a.rows, places) / 2);
+    a.most = std::min<int64_t>(a.pieces + a.rows, (int64_t)a.rows * ((a.longest + LEAST * UNIT - 1) / (LEAST * UNIT)));
+  } else {
+    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(16384 / ((int64_t)a.rows * tiles), (a.longest + 2047) / 2048));
+    a.chunk = ((a.longest + a.parts - 1) / a.parts + UNIT - 1) / UNIT * UNIT;
+    a.most = (int64_t)a.rows * a.parts;
+  }
 }
 
 }  // namespace
 
 int64_t pages_attention_workspace(const PagesView &c, int32_t nh, int32_t rows, int32_t longest) {
-  const int64_t chunk = chunk_of(c, nh, rows, longest), parts = (longest + chunk - 1) / chunk;
-  return parts > 1 ? 4 * (int64_t)rows * nh * parts * (c.hs + 2) : 0;
+  PagesAttn a = {};
+  a.c = c;
+  a.nh = nh;
+  a.rows = rows;
+  a.longest = longest;
+  cut(a);
+  return a.most > rows ? 4 * (((a.most * nh * 2 + 3) & ~3) + a.most * nh * c.hs) : 0;
 }
 
 hipError_t launch_pages_attention(const PagesAttn &args, hipStream_t s) {
   PagesAttn a = args;
-  a.chunk = chunk_of(a.c, a.nh, a.rows, a.longest);
-  a.parts = std::max(1, (a.longest + a.chunk - 1) / a.chunk);
+  cut(a);
   switch (a.c.hs) {
     case 16: launch<16>(a, s); break;
     case 32: launch<32>(a, s); break;
