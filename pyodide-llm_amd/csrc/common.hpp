@@ -161,6 +161,19 @@ __device__ __forceinline__ float wave_top(float x) {
   return wave_all(x, [](float a, float b) { return wmax(a, b); });
 }
 
+// the sum over the wave's lanes up to this one
+__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
+#define STEP(from, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, from, rows, 0xF, false)
+  STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8
+  STEP(0x112, 0xF);
+  STEP(0x114, 0xF);
+  STEP(0x118, 0xF);
+  STEP(0x142, 0xA);  // the first and third rows' last lanes to the next rows
+  STEP(0x143, 0xC);  // the first half's to the second
+#undef STEP
+  return x;
+}
+
 __device__ __forceinline__ float add32(float acc, const float4 v[8]) {
 #pragma unroll
   for (int u = 0; u < 8; ++u) {

@@ -255,8 +255,8 @@ int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int
 
 int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, const void *ws, int32_t m, int32_t rows,
                        int32_t k, int32_t bias, int32_t group, int32_t half_scales, void *stream) {
-  if (m < 1 || m > 65535 || rows < 1 || rows > 1 << 28 || k < GS || k % GS || k > 1 << 24)
-    return failed(HE_E_ARG, "hk_matmul_four: m is in 1..65535, rows in 1..2^28, k a multiple of 32 up to 2^24");
+  if (m < 1 || m > 65535 || rows < 1 || rows > 1 << 26 || k < GS || k % GS || k > 1 << 24)
+    return failed(HE_E_ARG, "hk_matmul_four: m is in 1..65535, rows in 1..2^26, k a multiple of 32 up to 2^24");
   if (bias != 0 && bias != 64) return failed(HE_E_ARG, "hk_matmul_four: bias is 0 or 64");
   if (group != 32 && group != 64 && group != 128) return failed(HE_E_ARG, "hk_matmul_four: group is 32, 64 or 128");
   if (!y || !xq || !xs || !w || !ws || !aligned(y, 4) || !aligned(xq) || !aligned(xs, 4) || !aligned(w) || !aligned(ws))

@@ -307,19 +307,6 @@ __device__ __forceinline__ bool impossible(const PagesAttn &a, int seq, int len)
   return len > 0 && seq >= 0 && (seq >= a.c.n_seqs || len > a.longest || len > a.c.slots * a.c.page);
 }
 
-// the sum over the wave's lanes up to this one
-__device__ __forceinline__ uint32_t up_to(uint32_t x) {
-#define STEP(from, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, from, rows, 0xF, false)
-  STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8
-  STEP(0x112, 0xF);
-  STEP(0x114, 0xF);
-  STEP(0x118, 0xF);
-  STEP(0x142, 0xA);  // the first and third rows' last lanes to the next rows
-  STEP(0x143, 0xC);  // the first half's to the second
-#undef STEP
-  return x;
-}
-
 // `find`: the row, or the piece whose row is looked for (past the last: row -1)
 template <bool ROW>
 __device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane) {
@@ -348,10 +335,10 @@ __device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane
     units = (len + UNIT - 1) / UNIT;
   };
   read(lane);
-  uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up_to(units), 63);
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)wave_up_to(units), 63);
   for (int base = 64; base < a.rows; base += 64) {
     read(base + lane);
-    total += (uint32_t)__builtin_amdgcn_readlane((int)up_to(units), 63);
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_up_to(units), 63);
   }
   // units a piece
   const int each = min(max(LEAST, (int)((total + a.pieces - 1) / a.pieces)), (a.longest + UNIT - 1) / UNIT);
@@ -360,7 +347,7 @@ __device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane
   for (int base = 0, before = 0; base < a.rows; base += 64) {
     if (a.rows > 64) read(base + lane);
     const int mine = base + lane < a.rows ? max(1, (units + each - 1) / each) : 0;
-    const int upto = before + (int)up_to(mine);
+    const int upto = before + (int)wave_up_to(mine);
     const uint64_t here = __ballot(ROW ? base + lane == find : upto > find && upto - mine <= find);
     if (here) {
       const int l = __builtin_ctzll(here);

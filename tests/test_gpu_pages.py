@@ -189,6 +189,39 @@ def test_pages_of_every_size_and_no_list(page, half):
     within(pages.attention(0, q, None, lengths, 8, longest=model.slots * page), model, 0, q, None, lengths, 8)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows", [63, 64, 65, 130, 256, 257, 700])
+def test_many_rows(rows, half):
+    """launches that plan their pieces from up to 256 rows' lengths, and ones of more; empty, short and long rows, some that
+    cannot be, over the pages of a few sequences"""
+    rng = np.random.default_rng(rows)
+    held = [3000, 700, 64]
+    model = filled(rng, 1, 2, 32, 32, half, held)
+    pages = Pages(model)
+    seqs = rng.integers(0, 3, rows)
+    lengths = np.array([int(rng.integers(0, min(held[s], 200) + 1)) for s in seqs])
+    for i in (0, rows // 2, rows - 1):  # the long ones, at the lists' ends
+        seqs[i], lengths[i] = 0, 3000 - i
+    seqs[1], seqs[2], lengths[3] = -1, 3, 3001  # (no sequence, none such, past `longest`)
+    q = rng.standard_normal((rows, 6 * 32)).astype(np.float32)
+    got = pages.attention(0, q, seqs.tolist(), lengths.tolist(), 6, longest=3000)
+    wrong = [i for i in (2, 3) if lengths[i] > 0]
+    assert np.isnan(got[wrong]).all() and (got[1] == 0).all()
+    keep = np.array([i for i in range(rows) if i not in (2, 3)])
+    within(got[keep], model, 0, q[keep], seqs[keep].tolist(), lengths[keep].tolist(), 6)
+
+
+def test_pieces_of_more_pages_than_a_wave_looks_up_at_once():
+    """more rows than are planned for, so many heads that a row is one piece: 9000 positions of one sequence to a workgroup"""
+    rng = np.random.default_rng(12)
+    model = filled(rng, 1, 64, 32, 16, True, [9000])
+    pages = Pages(model)
+    lengths = [9000, 8999, 8193, 8192] + [int(n) for n in rng.integers(1, 40, 296)]
+    q = rng.standard_normal((300, 64 * 16)).astype(np.float32)
+    got = pages.attention(0, q, [0] * 300, lengths, 64)
+    within(got, model, 0, q, [0] * 300, lengths, 64)
+
+
 def test_a_turn_of_one_sequence():
     """the tokens of a turn as rows one position apart, and a fork's rows beside them"""
     rng = np.random.default_rng(1)

@@ -118,7 +118,7 @@ def test_attention_workspaces_that_are_refused():
 
 
 @pytest.mark.parametrize("change, text", [
-    (dict(m=0), b"m is in"), (dict(m=65536), b"m is in"), (dict(rows=0), b"rows"), (dict(rows=(1 << 28) + 1), b"rows"),
+    (dict(m=0), b"m is in"), (dict(m=65536), b"m is in"), (dict(rows=0), b"rows"), (dict(rows=(1 << 26) + 1), b"rows"),
     (dict(k=0), b"k a multiple"), (dict(k=48), b"k a multiple"), (dict(k=(1 << 24) + 32), b"k a multiple"), (dict(bias=1), b"bias"),
     (dict(group=16), b"group"), (dict(group=256), b"group"), (dict(group=0), b"group"), (dict(y=None), b"pointer"),
     (dict(xq=None), b"pointer"), (dict(xs=None), b"pointer"), (dict(w=None), b"pointer"), (dict(ws=None), b"pointer"),
