@@ -49,37 +49,36 @@ __device__ __forceinline__ T quad_sums(const T (&s)[4], int j) {
   return (high ? b : a) + dpp_xor2(high ? a : b);
 }
 
-// ---- one token or two ----
+// ---- one token ----
 
 // LANES lanes a row (16, 64 or all waves'), which take its chunks LANES apart, STEPS of them at most; they take four rows at a
 // time and go on the launch's rows further. A lane's activations stay in its registers from row to row. Bound by the weights'
-// bytes.
-template <int LANES, int STEPS, int M, bool HALF>
+// bytes where there are many (128,256 rows of 4096 columns, 271 MB in 48.8 us, 5.6 TB/s), by latency where not (4096 rows, 10.5
+// MB, 5.5 us).
+template <int LANES, int STEPS, bool HALF>
 __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
   constexpr int ROWS = WAVES * 64 / LANES * 4;  // a workgroup takes at a time
   constexpr bool WIDE = LANES > 64;
-  __shared__ float parts[WIDE ? 2 : 1][M][4][WAVES];
+  __shared__ float parts[WIDE ? 2 : 1][4][WAVES];
   const int nc = (a.k + 127) / 128, l = threadIdx.x % LANES, j = threadIdx.x & 3;
   const int shift = a.group == 32 ? 0 : a.group == 64 ? 1 : 2;
-  uint32_t x[M][STEPS][8];
-  float xs[M][STEPS];
+  uint32_t x[STEPS][8];
+  float xs[STEPS];
 #pragma unroll
-  for (int t = 0; t < M; ++t)
+  for (int s = 0; s < STEPS; ++s) {
+    const int q = l + LANES * s, first = 32 * q - 28 * j;  // (the chunk's first column: 128 of 128s, 4 j)
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int q = l + LANES * s, first = 32 * q - 28 * j;  // (the chunk's first column: 128 of 128s, 4 j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int column = first + 16 * e;
-        uint32_t v = 0;
-        if (column < a.k) {
-          v = *reinterpret_cast<const uint32_t *>(a.xq + (int64_t)t * a.k + column);
-          if (a.bias) v = centre4(v);
-        }
-        x[t][s][e] = v;
+    for (int e = 0; e < 8; ++e) {
+      const int column = first + 16 * e;
+      uint32_t v = 0;
+      if (column < a.k) {
+        v = *reinterpret_cast<const uint32_t *>(a.xq + column);
+        if (a.bias) v = centre4(v);
       }
-      xs[t][s] = q < a.k / 32 ? a.xs[(int64_t)t * (a.k / 32) + q] : 0.0f;
+      x[s][e] = v;
     }
+    xs[s] = q < a.k / 32 ? a.xs[q] : 0.0f;
+  }
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS, turn ^= 1) {
     const int64_t row0 = base + threadIdx.x / LANES * 4;
@@ -96,45 +95,34 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
         ws[r][s] = HALF ? (float)reinterpret_cast<const _Float16 *>(a.ws)[at] : reinterpret_cast<const float *>(a.ws)[at];
       }
     }
+    float acc[4];
 #pragma unroll
-    for (int t = 0; t < M; ++t) {
-      float acc[4];
+    for (int r = 0; r < 4; ++r) {
+      acc[r] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        acc[r] = 0.0f;
+      for (int s = 0; s < STEPS; ++s) {
+        const uint32_t in[4] = {w[r][s].x, w[r][s].y, w[r][s].z, w[r][s].w};
+        int32_t sums[4];
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          const uint32_t in[4] = {w[r][s].x, w[r][s].y, w[r][s].z, w[r][s].w};
-          int32_t sums[4];
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            sums[g] = dot4(low_bits(in[g]), x[t][s][2 * g], dot4(high_bits(in[g]), x[t][s][2 * g + 1], 0));
-          acc[r] = __builtin_fmaf((float)quad_sums(sums, j), ws[r][s] * xs[t][s], acc[r]);
-        }
+        for (int g = 0; g < 4; ++g) sums[g] = dot4(low_bits(in[g]), x[s][2 * g], dot4(high_bits(in[g]), x[s][2 * g + 1], 0));
+        acc[r] = __builtin_fmaf((float)quad_sums(sums, j), ws[r][s] * xs[s], acc[r]);
       }
-      float y = quad_sums(acc, j);  // row j's, over the lane's quad
-      y += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x124, 0xF, 0xF, true));  // row_ror:4
-      y += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x128, 0xF, 0xF, true));  // row_ror:8
-      if (LANES >= 64) {
-        y += __shfl_xor(y, 16);
-        y += __shfl_xor(y, 32);
-      }
-      if (WIDE) {
-        if ((threadIdx.x & 63) < 4) parts[turn][t][j][threadIdx.x >> 6] = y;
-      } else if (l < 4 && row0 + j < a.rows) {
-        a.y[(int64_t)t * a.rows + row0 + j] = y * SIXTEENTH;
-      }
+    }
+    float y = quad_sums(acc, j);  // row j's, over the lane's quad
+    y += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x124, 0xF, 0xF, true));  // row_ror:4
+    y += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), 0x128, 0xF, 0xF, true));  // row_ror:8
+    if (LANES >= 64) {
+      y += __shfl_xor(y, 16);
+      y += __shfl_xor(y, 32);
     }
     if (WIDE) {  // (the next turn's go to the other half: one barrier)
+      if ((threadIdx.x & 63) < 4) parts[turn][j][threadIdx.x >> 6] = y;
       __syncthreads();
-      if (threadIdx.x < 4 * M) {
-        const int t = threadIdx.x >> 2;
-        float y = 0.0f;
+      y = 0.0f;
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) y += parts[turn][t][j][k];
-        if (row0 + j < a.rows) a.y[(int64_t)t * a.rows + row0 + j] = y * SIXTEENTH;
-      }
+      for (int k = 0; k < WAVES; ++k) y += parts[turn][j][k];
     }
+    if (l < 4 && row0 + j < a.rows) a.y[row0 + j] = y * SIXTEENTH;
   }
 }
 
@@ -192,75 +180,66 @@ struct Carrier {
   }
 };
 
-// a wave's weights of 16 RT rows: DEEP times 128 columns of them, GEMM_WAVES apart, and their scales
-template <int RT, int DEEP, int GROUP, bool HALF>
+// what a product of 16 tokens and 128 columns takes of them, of one lane
+struct Operand {
+  uint4 lo, hi;
+  float4 f[4];
+};
+template <int TILES, int PLACES>
+__device__ __forceinline__ Operand operand(const Tokens<TILES, PLACES> &tokens, int tile, int place) {
+  const int lane = threadIdx.x & 63;
+  Operand x;
+  x.lo = tokens.x[tile][place][0][lane];
+  x.hi = tokens.x[tile][place][1][lane];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) x.f[g] = tokens.xs[tile][place][g][lane >> 4];
+  return x;
+}
+
+// a lane's weights of 128 columns and their scales, a row's
+template <int GROUP, bool HALF>
 struct Weights {
   static constexpr int EACH = 128 / GROUP;
   typedef typename Scale<HALF>::type scales __attribute__((ext_vector_type(EACH)));
-  uint4 in[RT][DEEP];
-  scales sc[RT][DEEP];
+  uint4 in;
+  scales sc;
 
-  __device__ __forceinline__ void read(const FourArgs &a, int64_t row0, int place, int nc) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int64_t row = min(row0 + 16 * r + (lane & 15), (int64_t)a.rows - 1);
-      const uint4 *w = reinterpret_cast<const uint4 *>(a.w) + row * nc * 4 + (lane >> 4);
-      const scales *ws = reinterpret_cast<const scales *>(a.ws) + row * nc;
-#pragma unroll
-      for (int d = 0; d < DEEP; ++d) {
-        const int q = min(place + GEMM_WAVES * d, nc - 1);
-        in[r][d] = w[q * 4];
-        sc[r][d] = ws[q];
-      }
-    }
+  __device__ __forceinline__ void read(const FourArgs &a, int64_t row, int place, int nc) {
+    in = reinterpret_cast<const uint4 *>(a.w)[(row * nc + place) * 4 + ((threadIdx.x & 63) >> 4)];
+    sc = reinterpret_cast<const scales *>(a.ws)[row * nc + place];
   }
-
-  // their products with the tokens at places GEMM_WAVES d + wave of `left`
-  template <int TILES, int PLACES>
-  __device__ __forceinline__ void multiply(const Tokens<TILES, PLACES> &tokens, int left, float4 (&acc)[RT][TILES]) const {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // D = X W^T, 16 tokens by 16 rows: a lane has one row's sums for four tokens, so that the row's scales are its own and the
+  // tokens' come four at a time
+  __device__ __forceinline__ void multiply(const Operand &x, float4 &acc) const {
+    const uint32_t bits[4] = {in.x, in.y, in.z, in.w};
+    const long av[4] = {(long)((uint64_t)x.lo.y << 32 | x.lo.x), (long)((uint64_t)x.lo.w << 32 | x.lo.z),
+                        (long)((uint64_t)x.hi.y << 32 | x.hi.x), (long)((uint64_t)x.hi.w << 32 | x.hi.z)};
+    i32x4 s[4];
 #pragma unroll
-    for (int d = 0; d < DEEP; ++d) {
-      const int q = GEMM_WAVES * d + wave;
-      if (q >= left) break;
-      long b[RT][4];
+    for (int g = 0; g < 4; ++g)
+      s[g] = __builtin_amdgcn_mfma_i32_16x16x32_i8(av[g], (long)((uint64_t)high_bits(bits[g]) << 32 | low_bits(bits[g])),
+                                                   i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const uint32_t bits[4] = {in[r][d].x, in[r][d].y, in[r][d].z, in[r][d].w};
+    for (int g = 0; g < 4; g += 4 / EACH) {
+      float4 y;  // of the groups that share a scale
 #pragma unroll
-        for (int g = 0; g < 4; ++g) b[r][g] = (long)((uint64_t)high_bits(bits[g]) << 32 | low_bits(bits[g]));
+      for (int i = 0; i < 4 / EACH; ++i) {
+        const i32x4 v = s[g + i];
+        const float4 f = x.f[g + i];
+        if (i == 0) {
+          y = make_float4((float)v[0] * f.x, (float)v[1] * f.y, (float)v[2] * f.z, (float)v[3] * f.w);
+        } else {
+          y.x = __builtin_fmaf((float)v[0], f.x, y.x);
+          y.y = __builtin_fmaf((float)v[1], f.y, y.y);
+          y.z = __builtin_fmaf((float)v[2], f.z, y.z);
+          y.w = __builtin_fmaf((float)v[3], f.w, y.w);
+        }
       }
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        const uint4 lo = tokens.x[t][q][0][lane], hi = tokens.x[t][q][1][lane];
-        const long av[4] = {(long)((uint64_t)lo.y << 32 | lo.x), (long)((uint64_t)lo.w << 32 | lo.z),
-                            (long)((uint64_t)hi.y << 32 | hi.x), (long)((uint64_t)hi.w << 32 | hi.z)};
-#pragma unroll
-        for (int g = 0; g < 4; g += 4 / EACH)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            float4 y;  // of the groups that share a scale
-#pragma unroll
-            for (int i = 0; i < 4 / EACH; ++i) {
-              const i32x4 s = __builtin_amdgcn_mfma_i32_16x16x32_i8(av[g + i], b[r][g + i], i32x4{0, 0, 0, 0}, 0, 0, 0);
-              const float4 fs = tokens.xs[t][q][g + i][lane >> 4];
-              if (i == 0) {
-                y = make_float4((float)s[0] * fs.x, (float)s[1] * fs.y, (float)s[2] * fs.z, (float)s[3] * fs.w);
-              } else {
-                y.x = __builtin_fmaf((float)s[0], fs.x, y.x);
-                y.y = __builtin_fmaf((float)s[1], fs.y, y.y);
-                y.z = __builtin_fmaf((float)s[2], fs.z, y.z);
-                y.w = __builtin_fmaf((float)s[3], fs.w, y.w);
-              }
-            }
-            const float scale = (float)sc[r][d][g * EACH / 4];
-            acc[r][t].x = __builtin_fmaf(y.x, scale, acc[r][t].x);
-            acc[r][t].y = __builtin_fmaf(y.y, scale, acc[r][t].y);
-            acc[r][t].z = __builtin_fmaf(y.z, scale, acc[r][t].z);
-            acc[r][t].w = __builtin_fmaf(y.w, scale, acc[r][t].w);
-          }
-      }
+      const float scale = (float)sc[g * EACH / 4];
+      acc.x = __builtin_fmaf(y.x, scale, acc.x);
+      acc.y = __builtin_fmaf(y.y, scale, acc.y);
+      acc.z = __builtin_fmaf(y.z, scale, acc.z);
+      acc.w = __builtin_fmaf(y.w, scale, acc.w);
     }
   }
 };
@@ -280,43 +259,49 @@ __device__ __forceinline__ void finish(const FourArgs &a, const float4 *sums, in
   }
 }
 
-// D = X W^T, 16 tokens by 16 rows a product: a lane has one row's sums for four tokens, so that the row's scales are its own and
-// the tokens' come from LDS four at a time. The waves of a workgroup take the 128s of columns in turn.
-
-// Up to 16 tokens of up to 4096 columns: they stay in LDS, and the workgroup goes from row to row, the next rows' weights on
-// their way meanwhile.
-constexpr int RESIDENT = 32;  // 128s of columns
-template <int GROUP, bool HALF>
-__global__ __launch_bounds__(GEMM_THREADS, 4) void rows_kernel(const FourArgs a) {
-  constexpr int DEEP = RESIDENT / GEMM_WAVES;
-  __shared__ Tokens<1, RESIDENT> tokens;
-  __shared__ float4 sums[GEMM_THREADS];  // (half of a CU's LDS in all)
-  const int nc = (a.k + 127) / 128, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Up to 16 tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves sharing
+// their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One workgroup a
+// CU: two have twice the loads on their way and came out slower (14336 rows of 4096 columns 18.8 us against 15.0). 16 tokens of
+// these take 14.3 us, 34 MB; of 128,256 rows 67 (4.1 TB/s; the weights' 64 bytes a row and load cost a sixth of it, measured
+// with as many in one piece).
+template <int DEEP, int GROUP, bool HALF>
+__global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a) {
+  __shared__ Tokens<1, GEMM_WAVES * DEEP> tokens;
+  __shared__ float4 sums[GEMM_THREADS];
+  const int nc = (a.k + 127) / 128, first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * DEEP, mine = threadIdx.x & 15;
   const int64_t step = (int64_t)gridDim.x * 16;
-  Weights<1, DEEP, GROUP, HALF> w;
-  w.read(a, (int64_t)blockIdx.x * 16, wave, nc);
-  Carrier<1, RESIDENT> carrier;
-  carrier.read(a, 0, 0);
-  carrier.write(a, 0, tokens);
+  Weights<GROUP, HALF> w[DEEP];
+  auto row = [&](int64_t row0) { return min(row0 + mine, (int64_t)a.rows - 1); };
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d) w[d].read(a, row((int64_t)blockIdx.x * 16), min(first + d, nc - 1), nc);
+  {
+    Carrier<1, GEMM_WAVES * DEEP> carrier;
+    carrier.read(a, 0, 0);
+    carrier.write(a, 0, tokens);
+  }
   __syncthreads();
   for (int64_t row0 = (int64_t)blockIdx.x * 16; row0 < a.rows; row0 += step) {
-    Weights<1, DEEP, GROUP, HALF> next;
-    if (row0 + step < a.rows) next.read(a, row0 + step, wave, nc);
-    __builtin_amdgcn_sched_barrier(0);
-    float4 acc[1][1] = {{make_float4(0, 0, 0, 0)}};
-    w.multiply(tokens, nc, acc);
-    sums[threadIdx.x] = acc[0][0];
+    const int64_t next = row(row0 + step);
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {  // (places past the columns: zeros)
+      const Weights<GROUP, HALF> now = w[d];
+      const Operand x = operand(tokens, 0, first + d);
+      now.multiply(x, acc);
+      w[d].read(a, next, min(first + d, nc - 1), nc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sums[threadIdx.x] = acc;
     __syncthreads();
     finish<1>(a, sums, 0, row0);
     __syncthreads();
-    w = next;
   }
 }
 
 // Any number of tokens and columns: 16 RT rows by 16 TILES tokens a workgroup, the activations a stage at a time, the next
 // stage's on their way meanwhile.
 template <int RT, int TILES, int GROUP, bool HALF>
-__global__ __launch_bounds__(GEMM_THREADS, RT * TILES <= 2 ? 4 : 2) void stages_kernel(const FourArgs a) {
+__global__ __launch_bounds__(GEMM_THREADS, TILES == 1 && (HALF || GROUP > 32) ? 4 : 2) void stages_kernel(const FourArgs a) {
   constexpr int DEEP = 4 / TILES, STAGE = GEMM_WAVES * DEEP;
   __shared__ Tokens<TILES, STAGE> tokens;
   const int nc = (a.k + 127) / 128, t0 = blockIdx.y * (16 * TILES), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -328,16 +313,31 @@ __global__ __launch_bounds__(GEMM_THREADS, RT * TILES <= 2 ? 4 : 2) void stages_
     for (int t = 0; t < TILES; ++t) acc[r][t] = make_float4(0, 0, 0, 0);
   Carrier<TILES, STAGE> carrier;
   carrier.read(a, t0, 0);
+  int64_t row[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) row[r] = min(row0 + 16 * r + (threadIdx.x & 15), (int64_t)a.rows - 1);
   for (int c0 = 0; c0 < nc; c0 += STAGE) {
-    Weights<RT, DEEP, GROUP, HALF> w;
-    w.read(a, row0, c0 + wave, nc);
+    Weights<GROUP, HALF> w[RT][DEEP];
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) w[r][d].read(a, row[r], min(c0 + wave * DEEP + d, nc - 1), nc);
     __builtin_amdgcn_sched_barrier(0);
     if (c0) __syncthreads();  // (the last stage's have been read)
     carrier.write(a, c0, tokens);
     __syncthreads();
     if (c0 + STAGE < nc) carrier.read(a, t0, c0 + STAGE);
     __builtin_amdgcn_sched_barrier(0);
-    w.multiply(tokens, nc - c0, acc);
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      if (c0 + wave * DEEP + d >= nc) break;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const Operand x = operand(tokens, t, wave * DEEP + d);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) w[r][d].multiply(x, acc[r][t]);
+      }
+    }
   }
   float4 *sums = reinterpret_cast<float4 *>(tokens.x);
 #pragma unroll
@@ -350,22 +350,20 @@ __global__ __launch_bounds__(GEMM_THREADS, RT * TILES <= 2 ? 4 : 2) void stages_
   }
 }
 
-template <int LANES, int STEPS, int M, bool HALF>
+template <int LANES, int STEPS, bool HALF>
 void launch_gemv(const FourArgs &a, hipStream_t s) {
   constexpr int ROWS = WAVES * 64 / LANES * 4;
   const int blocks = std::min((a.rows + ROWS - 1) / ROWS, 1024);
-  hipLaunchKernelGGL((gemv_kernel<LANES, STEPS, M, HALF>), dim3(blocks), dim3(64 * WAVES), 0, s, a);
+  hipLaunchKernelGGL((gemv_kernel<LANES, STEPS, HALF>), dim3(blocks), dim3(64 * WAVES), 0, s, a);
 }
 
-template <bool HALF>
+template <int DEEP, bool HALF>
 void launch_rows(const FourArgs &a, hipStream_t s) {
-  // one workgroup a CU, two where each has many turns (14336 rows 15.8 us against 17.6, 128,256 rows 83 against 73); as many
-  // turns for all as for the most
-  const int blocks = (a.rows + 15) / 16, most = blocks > 2048 ? 512 : 256;
-  const int turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns;
-  if (a.group == 32) hipLaunchKernelGGL((rows_kernel<32, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
-  else if (a.group == 64) hipLaunchKernelGGL((rows_kernel<64, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((rows_kernel<128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  // as many turns for every workgroup as for the most
+  const int blocks = (a.rows + 15) / 16, turns = (blocks + 255) / 256, grid = (blocks + turns - 1) / turns;
+  if (a.group == 32) hipLaunchKernelGGL((rows_kernel<DEEP, 32, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else if (a.group == 64) hipLaunchKernelGGL((rows_kernel<DEEP, 64, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((rows_kernel<DEEP, 128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
 }
 
 template <int RT, int TILES, bool HALF>
@@ -393,21 +391,19 @@ void launch_gemm(const FourArgs &a, hipStream_t s) {
 template <bool HALF>
 void launch(const FourArgs &a, hipStream_t s) {
   const int chunks = (a.k + 127) / 128 * 4;
-  // two tokens go this way only over many short rows, whose 128s of columns are fewer than the other kernel's waves (32000 rows
-  // of 768 columns: 8.8 us against 15.8; 2304 of 768: 6.1, 5.3; 4096 of 4096: 7.3, 6.9; 4096 of 14336: 17.8, 13.8)
-  if (a.m == 2 && chunks <= 32 && a.rows > 8192) {
-    if (chunks <= 16) launch_gemv<16, 1, 2, HALF>(a, s);
-    else launch_gemv<16, 2, 2, HALF>(a, s);
-  } else if (a.m == 1 && chunks <= 1024) {
-    if (chunks <= 16) launch_gemv<16, 1, 1, HALF>(a, s);
-    else if (chunks <= 32) launch_gemv<16, 2, 1, HALF>(a, s);
-    else if (chunks <= 64) launch_gemv<64, 1, 1, HALF>(a, s);
-    else if (chunks <= 128) launch_gemv<64, 2, 1, HALF>(a, s);
-    else if (chunks <= 256) launch_gemv<64, 4, 1, HALF>(a, s);
-    else if (chunks <= 512) launch_gemv<256, 2, 1, HALF>(a, s);
-    else launch_gemv<256, 4, 1, HALF>(a, s);
-  } else if (a.m <= 16 && chunks <= 4 * RESIDENT) {
-    launch_rows<HALF>(a, s);
+  // (two tokens by the first kernel: 4096 rows of 4096 columns 7.3 us against 6.9, of 14336 17.8, 13.8; 32000 of 768 the same)
+  if (a.m == 1 && chunks <= 1024) {
+    if (chunks <= 16) launch_gemv<16, 1, HALF>(a, s);
+    else if (chunks <= 32) launch_gemv<16, 2, HALF>(a, s);
+    else if (chunks <= 64) launch_gemv<64, 1, HALF>(a, s);
+    else if (chunks <= 128) launch_gemv<64, 2, HALF>(a, s);
+    else if (chunks <= 256) launch_gemv<64, 4, HALF>(a, s);
+    else if (chunks <= 512) launch_gemv<256, 2, HALF>(a, s);
+    else launch_gemv<256, 4, HALF>(a, s);
+  } else if (a.m <= 16 && chunks <= 128) {
+    if (chunks <= 32) launch_rows<1, HALF>(a, s);
+    else if (chunks <= 64) launch_rows<2, HALF>(a, s);
+    else launch_rows<4, HALF>(a, s);
   } else if (a.m <= 16) {
     launch_gemm<1, HALF>(a, s);
   } else if (a.m <= 32) {
