@@ -52,9 +52,10 @@ __device__ __forceinline__ T quad_sums(const T (&s)[4], int j) {
 // ---- one token ----
 
 // LANES lanes a row (16, 64 or all waves'), which take its chunks LANES apart, STEPS of them at most; they take four rows at a
-// time and go on the launch's rows further. A lane's activations stay in its registers from row to row. Bound by the weights'
-// bytes where there are many (128,256 rows of 4096 columns, 271 MB in 48.8 us, 5.6 TB/s), by latency where not (4096 rows, 10.5
-// MB, 5.5 us).
+// time and go on the launch's rows further. A lane's activations stay in its registers from row to row. No load is conditional,
+// which would wait for each: what lies past the columns is taken as zero. Bound by the weights' bytes where there are many
+// (128,256 rows of 4096 columns, 271 MB in 48.1 us, 5.6 TB/s), by latency where not (4096 rows, 10.5 MB, 4.0 us; 5.5 with
+// conditional loads).
 template <int LANES, int STEPS, bool HALF>
 __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
   constexpr int ROWS = WAVES * 64 / LANES * 4;  // a workgroup takes at a time
@@ -70,14 +71,11 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int column = first + 16 * e;
-      uint32_t v = 0;
-      if (column < a.k) {
-        v = *reinterpret_cast<const uint32_t *>(a.xq + column);
-        if (a.bias) v = centre4(v);
-      }
-      x[s][e] = v;
+      x[s][e] = *reinterpret_cast<const uint32_t *>(a.xq + min(column, a.k - 4));
+      if (column >= a.k) x[s][e] = a.bias ? 0x40404040u : 0;
     }
-    xs[s] = q < a.k / 32 ? a.xs[q] : 0.0f;
+    xs[s] = a.xs[min(q, a.k / 32 - 1)];
+    if (q >= a.k / 32) xs[s] = 0.0f;
   }
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.rows; base += (int64_t)gridDim.x * ROWS, turn ^= 1) {
@@ -94,6 +92,12 @@ __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
         const int64_t at = row * (nc * 4 >> shift) + (q >> shift);
         ws[r][s] = HALF ? (float)reinterpret_cast<const _Float16 *>(a.ws)[at] : reinterpret_cast<const float *>(a.ws)[at];
       }
+    }
+    if (base == (int64_t)blockIdx.x * ROWS && a.bias) {  // (here, so that the first rows are asked for before)
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = centre4(x[s][e]);
     }
     float acc[4];
 #pragma unroll

@@ -325,13 +325,11 @@ __device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane
   int len, seq, units;
   bool wrong;
   auto read = [&](int row) {
-    len = seq = 0;
-    if (row < a.rows) {
-      len = a.lengths[row];
-      seq = a.seqs ? a.seqs[row] : row;
-    }
+    const int at = min(row, a.rows - 1);
+    len = a.lengths[at];
+    seq = a.seqs ? a.seqs[at] : at;
     wrong = impossible(a, seq, len);
-    if (seq < 0 || len < 0 || wrong) len = 0;
+    if (seq < 0 || len < 0 || wrong || row >= a.rows) len = 0;
     units = (len + UNIT - 1) / UNIT;
   };
   read(lane);
@@ -407,8 +405,8 @@ __global__ __launch_bounds__(64 * WAVES, occupancy(HS, HALF)) void attend_kernel
   const int shift = __builtin_ctz(c.page);
   bool lost = false;
   auto pages = [&](int p) {
-    const int64_t mine = p + (int64_t)lane * (BLOCK * WAVES);
-    const int32_t page = mine < p1 ? table[mine >> shift] : 0;
+    const int64_t mine = min(p + (int64_t)lane * (BLOCK * WAVES), (int64_t)p1 - 1);  // (past the last: the last position's)
+    const int32_t page = table[mine >> shift];
     const bool none = (uint32_t)page >= (uint32_t)c.n_pages;
     lost = lost || __any(none);
     return none ? 0 : page;
@@ -550,7 +548,10 @@ void launch(const PagesAttn &a, hipStream_t s) {
 void cut(PagesAttn &a) {
   const int group = a.nh / a.c.nkv, most = a.c.half ? 8 : 16, tiles = a.c.nkv * ((group + most - 1) / most);
   a.parts = a.pieces = 0;
-  if (a.longest <= (LEAST + 1) * UNIT) {  // every row one piece
+  // every row one piece where cutting it and joining its pieces takes longer: a block of a wave after another 1.3 us, the join
+  // about 4 (one row of 512 positions 12.3 us against 9.7 and the join); where the rows fill the CUs by themselves up to twice
+  // as many (96 rows of up to 900 positions of 8 heads 44 us against 49 and 5)
+  if (a.longest <= 5 * UNIT || (a.longest <= 8 * UNIT && (int64_t)a.rows * tiles >= 256)) {
     a.parts = 1;
     a.chunk = std::max(a.longest, 1);
     a.most = a.rows;
