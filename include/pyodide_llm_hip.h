@@ -391,7 +391,8 @@ int64_t hk_logprobs_workspace(int32_t m, int32_t n, int32_t top);
  *   tables int32  [n_seqs][table_size]: the page of a sequence's positions page_size * slot.., or -1 where it has none
  *   refs   int32  [n_pages]: how many entries of the tables name the page; 0: free
  * The tables start as -1, the refs as 0. page_size is one of 32, 64, 128, 256, head_size one of 16, 32, 48, 64, 96, 128, 256,
- * n_seqs at most HK_PAGES_SEQS_MOST, table_size * page_size at most HK_PAGES_MOST, n_pages at most HK_PAGES_PAGES_MOST.
+ * n_seqs at most HK_PAGES_SEQS_MOST, table_size * page_size and n_seqs * table_size at most HK_PAGES_MOST, n_pages at most
+ * HK_PAGES_PAGES_MOST, n_layers and n_kv_heads at most 1024.
  *
  * A sequence is a row of the tables; how many positions it has is the caller's to know. The lists that a call takes (sequences,
  * positions, lengths) are device memory too, so that a captured graph may be replayed with others. A negative sequence in a
@@ -431,7 +432,8 @@ int32_t hk_pages_fork(const hk_pages *pages, const void *to, const void *from, c
 /* Room to write: for each i < n (1..HK_PAGES_SEQS_MOST), every position starts[i]..ends[i] - 1 of sequence seqs[i] gets a page
  * that it alone names. Where there is none yet, or one that is shared as the call begins, the lowest free page is taken, in
  * the order of the list and of its positions; of a shared page with positions before starts[i], those rows are copied, in all
- * layers. A sequence may be listed once. *status (device int32, or null): 0; or how many free pages are lacking, or -1 where
+ * layers (what the sequence held from starts[i] on does not come along: the sequence goes on from there). A sequence may be
+ * listed once. *status (device int32, or null): 0; or how many free pages are lacking, or -1 where
  * the lists are not such as this (a sequence past the tables or listed twice, a position outside 0..table_size * page_size):
  * then nothing is changed. workspace: at least hk_pages_workspace bytes (16-byte aligned), not shared by calls that may
  * overlap. */
@@ -453,7 +455,8 @@ int64_t hk_pages_workspace(const hk_pages *pages);
 /* The keys and values of n rows into layer `layer`: row i to position positions[i] of sequence seqs[i] (seqs null: i). k and v
  * float32, n_kv_heads * head_size values a row, kv_stride floats apart (a multiple of 4; k and v 16-byte aligned), rounded to
  * the nearest, ties to even, where the cache is half. Rows whose sequence or position is outside the tables, or whose position
- * has no page, are dropped. No two rows go to one position. */
+ * has no page, are dropped. No two rows go to one position; a page that other sequences name too changes for them as well
+ * (hk_pages_reserve parts it). */
 int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, const void *v, int32_t kv_stride,
                         const void *seqs, const void *positions, int32_t n, void *stream);
 
@@ -464,8 +467,11 @@ int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, con
  * rows may be of one sequence (the tokens of a turn, at lengths one apart). lengths[i] is at most `longest`, which the
  * launches are made for. A row of length 0 (or less), or of a negative sequence, is zeros; one whose length is past `longest`
  * or the tables, or whose sequence is, or a position of which has no page, is NaN. What lies behind a row's length has no
- * part in it, whatever it is. A q that is not finite makes its own row NaN, a key that is not finite the rows that see it,
- * a value that is not finite their channel not finite. Sums are float32's; a half cache's products keep float32's bits.
+ * part in it, whatever it is. A q that is not finite makes its own row NaN; a key that is not finite changes the rows that see it
+ * alone (NaN, unless it takes their score to minus infinity, which has no weight), a value that is not finite makes their channel
+ * not finite. Sums are float32's, of values weighted by exp(score - the largest score so far); a half cache's products keep
+ * float32's bits. The same call gives the same bits; how a row's sums are split, and so their last ones, goes by all rows'
+ * lengths.
  * workspace: at least hk_pages_attention_workspace bytes (16-byte aligned; nothing in it is kept from one call to the next),
  * not shared by calls that may overlap. */
 int32_t hk_pages_attention(void *out, const void *q, const hk_pages *pages, int32_t layer, int32_t n_heads,

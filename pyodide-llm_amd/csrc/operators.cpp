@@ -87,8 +87,10 @@ int32_t pages_of(const char *what, const hk_pages *p, PagesView &v) {
     return failed(HE_E_ARG, std::string(what) + ": n_layers and n_kv_heads are in 1..1024");
   if (p->n_pages < 1 || p->n_pages > HK_PAGES_PAGES_MOST || p->n_seqs < 1 || p->n_seqs > HK_PAGES_SEQS_MOST)
     return failed(HE_E_ARG, std::string(what) + ": n_pages is in 1..HK_PAGES_PAGES_MOST (16777216), n_seqs in 1..HK_PAGES_SEQS_MOST (8192)");
-  if (p->table_size < 1 || (int64_t)p->table_size * p->page_size > HK_PAGES_MOST)
-    return failed(HE_E_ARG, std::string(what) + ": table_size is at least 1, table_size * page_size at most HK_PAGES_MOST (1073741824)");
+  if (p->table_size < 1 || (int64_t)p->table_size * p->page_size > HK_PAGES_MOST ||
+      (int64_t)p->table_size * p->n_seqs > HK_PAGES_MOST)
+    return failed(HE_E_ARG, std::string(what) + ": table_size is at least 1, table_size * page_size and n_seqs * table_size at "
+                                                "most HK_PAGES_MOST (1073741824)");
   v = {p->keys, p->values, reinterpret_cast<int32_t *>(p->tables), reinterpret_cast<int32_t *>(p->refs), p->n_layers, p->n_pages,
        p->n_kv_heads, p->page_size, p->head_size, p->half != 0, p->n_seqs, p->table_size};
   return HE_OK;

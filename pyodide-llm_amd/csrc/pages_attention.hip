@@ -28,19 +28,21 @@ constexpr int UNIT = BLOCK * WAVES, LEAST = 2;  // positions of a piece: a multi
 constexpr int PLANNED = 256;  // rows a launch's workgroups look through
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float INF = __builtin_inff();
-constexpr float AHEAD = 8.0f;     // how far (log2) a score may lie above the reference before that moves
-constexpr float PIECE_UP = 64.0f;  // probabilities go up to 2^AHEAD, their float16 halves to 2^14
+constexpr float PIECE_UP = 64.0f;  // what float16 halves of probabilities are raised by: up to 2^14
 constexpr float LOW = 2048.0f;     // the second half's scale
 
 template <bool HALF>
 struct Kind {
   typedef _Float16 type;
-  static constexpr int heads = 8, widest = 8;
+  static constexpr int heads = 8;
+  // how far (log2) a score may lie above the reference before that moves
+  static constexpr float ahead = 8.0f;
 };
 template <>
 struct Kind<false> {
   typedef float type;
-  static constexpr int heads = 16, widest = 4;
+  static constexpr int heads = 16;
+  static constexpr float ahead = 0.0f;  // (values of any size: no probability is above 1)
 };
 
 // lane ^ 8 within 16: the other half of a column's products
@@ -261,7 +263,7 @@ struct Wave {
         const float more = bar > -INF ? __builtin_fmaxf(next, 0.0f) : next;
         const float less = bar > -INF ? __builtin_amdgcn_exp2f(-more) : 0.0f;
         reference += more;
-        bar = AHEAD;
+        bar = Kind<HALF>::ahead;
         sum *= less;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) o[t] *= less;

@@ -170,7 +170,7 @@ def test_attention_at_lengths_where_it_can_go_wrong(nh, nkv, hs, half):
     got = pages.attention(1, q, seqs.tolist(), lens, nh, pad=8)
     within(got, model, 1, q, seqs.tolist(), lens, nh)
     assert (got[lens.index(0)] == 0).all()
-    # one at a time: the same bits, whatever the other rows are, as long as the launches are made for the same length
+    # one at a time (cut into pieces by its own length alone)
     for i in (lens.index(1030), lens.index(33)):
         alone = pages.attention(1, q[i:i + 1], [int(seqs[i])], [lens[i]], nh, longest=1030)
         within(alone, model, 1, q[i:i + 1], [int(seqs[i])], [lens[i]], nh)
@@ -291,6 +291,19 @@ def test_queries_of_any_size(half, scale):
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("keys, values", [(1e-6, 1.0), (1.0, 1e-6), (1e-6, 1e-6), (1.0, 3e-8)])
+def test_keys_and_values_next_to_nothing(half, keys, values):
+    """(in float16: denormals) against queries that make their scores count"""
+    rng = np.random.default_rng(13)
+    lengths = [3, 200, 900]
+    model = filled(rng, 1, 1, 32, 64, half, lengths)
+    model.keys[:] = model.keys * np.float32(keys)
+    model.values[:] = model.values * np.float32(values)
+    q = (rng.standard_normal((3, 4 * 64)) / keys).astype(np.float32)
+    within(Pages(model).attention(0, q, None, lengths, 4), model, 0, q, None, lengths, 4)
+
+
+@pytest.mark.parametrize("half", [False, True])
 def test_a_score_that_grows(half):
     """every block of positions with scores far above the last one's, and far below"""
     lengths, hs = [1200, 1200], 32
@@ -301,6 +314,28 @@ def test_a_score_that_grows(half):
             model.keys[0, model.tables[s, b], 0] = sign * b * 3.0 + 0.1 * rng.standard_normal((32, hs))
     q = np.full((2, 2 * hs), 0.5, dtype=np.float32)
     within(Pages(model).attention(0, q, None, lengths, 2), model, 0, q, None, lengths, 2)
+
+
+def test_large_values_behind_scores_that_grow():
+    """values near float32's largest: none is weighted by more than 1 on the way, however the scores grow from block to block"""
+    rng = np.random.default_rng(14)
+    model = filled(rng, 1, 1, 32, 32, False, [1200])
+    for b in range(38):
+        model.keys[0, model.tables[0, b], 0] = b * 0.7 + 0.1 * rng.standard_normal((32, 32))
+    model.values[:] = model.values * np.float32(1e36)
+    q = np.full((1, 2 * 32), 0.5, dtype=np.float32)
+    within(Pages(model).attention(0, q, None, [1200], 2), model, 0, q, None, [1200], 2)
+
+
+def test_keys_of_minus_infinity_have_no_weight():
+    """in a float32 cache, where the query's value is above 0: the other rows' scores stand"""
+    rng = np.random.default_rng(15)
+    model = filled(rng, 1, 1, 32, 32, False, [100])
+    q = np.abs(rng.standard_normal((1, 2 * 32))).astype(np.float32) + np.float32(0.1)
+    model.keys[0, model.tables[0, 1], 0, 3, 5] = -np.inf  # position 35
+    got = Pages(model).attention(0, q, None, [100], 2)
+    model.keys[0, model.tables[0, 1], 0, 3] = -1e4
+    within(got, model, 0, q, None, [100], 2)
 
 
 @pytest.mark.parametrize("half", [False, True])

@@ -39,7 +39,7 @@ def refused(rc, text=b""):
     (dict(n_kv_heads=0), b"n_kv_heads"), (dict(n_kv_heads=1025), b"n_kv_heads"), (dict(n_pages=0), b"n_pages"),
     (dict(n_pages=(1 << 24) + 1), b"n_pages"), (dict(n_seqs=0), b"n_seqs"), (dict(n_seqs=8193), b"n_seqs"),
     (dict(table_size=0), b"table_size"), (dict(table_size=(1 << 24) + 1), b"table_size"),
-    (dict(table_size=2147483647), b"table_size")])
+    (dict(table_size=2147483647), b"table_size"), (dict(n_seqs=8192, page_size=32, table_size=131073), b"table_size")])
 def test_caches_that_are_refused(change, text):
     lib, c = package().library(), made(**change)
     for call in calls(c):
