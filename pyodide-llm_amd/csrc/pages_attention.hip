@@ -383,7 +383,7 @@ __global__ __launch_bounds__(64 * WAVES, occupancy(HS, HALF)) void attend_kernel
   typedef typename Kind<HALF>::type T;
   constexpr int HEADS = Kind<HALF>::heads;
   __shared__ float tops[WAVES][HEADS], sums[WAVES][HEADS];
-  __shared__ float outs[WAVES][HEADS][HS];
+  __shared__ float outs[WAVES][HEADS][HS + 4];  // (a column's lanes four banks apart)
   const PagesView &c = a.c;
   const int group = a.nh / c.nkv, tiles = (group + HEADS - 1) / HEADS;
   const int g = blockIdx.y / tiles, first = g * group + blockIdx.y % tiles * HEADS;
