@@ -263,42 +263,50 @@ __device__ __forceinline__ void finish(const FourArgs &a, const float4 *sums, in
   }
 }
 
-// Up to 16 tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves sharing
-// their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One workgroup a
-// CU: two have twice the loads on their way and came out slower (14336 rows of 4096 columns 18.8 us against 15.0). 16 tokens of
-// these take 14.3 us, 34 MB; of 128,256 rows 67 (4.1 TB/s; the weights' 64 bytes a row and load cost a sixth of it, measured
-// with as many in one piece).
-template <int DEEP, int GROUP, bool HALF>
+// Up to 16 TILES tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves
+// sharing their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One
+// workgroup a CU: two have twice the loads on their way and came out slower (16 tokens by 14336 rows of 4096 columns 18.8 us
+// against 15.0). 16 tokens of these take 13.6 us, 34 MB: 6 until the first rows are done, 2 a turn; of 128,256 rows 64 (4.2 TB/s;
+// the weights' 64 bytes a row and load cost a sixth of it, measured with as many in one piece). 32 tokens: 19 and 85.
+template <int TILES, int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a) {
-  __shared__ Tokens<1, GEMM_WAVES * DEEP> tokens;
-  __shared__ float4 sums[GEMM_THREADS];
+  __shared__ Tokens<TILES, GEMM_WAVES * DEEP> tokens;
+  __shared__ float4 sums[2][GEMM_THREADS];
   const int nc = (a.k + 127) / 128, first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * DEEP, mine = threadIdx.x & 15;
   const int64_t step = (int64_t)gridDim.x * 16;
   Weights<GROUP, HALF> w[DEEP];
   auto row = [&](int64_t row0) { return min(row0 + mine, (int64_t)a.rows - 1); };
-#pragma unroll
-  for (int d = 0; d < DEEP; ++d) w[d].read(a, row((int64_t)blockIdx.x * 16), min(first + d, nc - 1), nc);
   {
-    Carrier<1, GEMM_WAVES * DEEP> carrier;
-    carrier.read(a, 0, 0);
+    Carrier<TILES, GEMM_WAVES * DEEP> carrier;
+    carrier.read(a, 0, 0);  // (before the weights, for which it would wait otherwise)
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) w[d].read(a, row((int64_t)blockIdx.x * 16), min(first + d, nc - 1), nc);
+    __builtin_amdgcn_sched_barrier(0);
     carrier.write(a, 0, tokens);
   }
   __syncthreads();
+  int turn = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * 16; row0 < a.rows; row0 += step) {
     const int64_t next = row(row0 + step);
-    float4 acc = make_float4(0, 0, 0, 0);
+    float4 acc[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) acc[t] = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {  // (places past the columns: zeros)
       const Weights<GROUP, HALF> now = w[d];
-      const Operand x = operand(tokens, 0, first + d);
-      now.multiply(x, acc);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) now.multiply(operand(tokens, t, first + d), acc[t]);
       w[d].read(a, next, min(first + d, nc - 1), nc);
       __builtin_amdgcn_sched_barrier(0);
     }
-    sums[threadIdx.x] = acc;
-    __syncthreads();
-    finish<1>(a, sums, 0, row0);
-    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      sums[turn][threadIdx.x] = acc[t];
+      __syncthreads();  // (the next go to the other half)
+      finish<1>(a, sums[turn], 16 * t, row0);
+      turn ^= 1;
+    }
   }
 }
 
@@ -361,13 +369,13 @@ void launch_gemv(const FourArgs &a, hipStream_t s) {
   hipLaunchKernelGGL((gemv_kernel<LANES, STEPS, HALF>), dim3(blocks), dim3(64 * WAVES), 0, s, a);
 }
 
-template <int DEEP, bool HALF>
+template <int TILES, int DEEP, bool HALF>
 void launch_rows(const FourArgs &a, hipStream_t s) {
   // as many turns for every workgroup as for the most
   const int blocks = (a.rows + 15) / 16, turns = (blocks + 255) / 256, grid = (blocks + turns - 1) / turns;
-  if (a.group == 32) hipLaunchKernelGGL((rows_kernel<DEEP, 32, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
-  else if (a.group == 64) hipLaunchKernelGGL((rows_kernel<DEEP, 64, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((rows_kernel<DEEP, 128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  if (a.group == 32) hipLaunchKernelGGL((rows_kernel<TILES, DEEP, 32, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else if (a.group == 64) hipLaunchKernelGGL((rows_kernel<TILES, DEEP, 64, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((rows_kernel<TILES, DEEP, 128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
 }
 
 template <int RT, int TILES, bool HALF>
@@ -381,7 +389,7 @@ void launch_stages(const FourArgs &a, hipStream_t s) {
 template <int TILES, bool HALF>
 void launch_gemm(const FourArgs &a, hipStream_t s) {
   // rows a workgroup: as many as leave about one workgroup a CU, since each brings the activations to LDS for itself (64 tokens by
-  // 14336 rows: 62 us at 16, 45 at 32, 33 at 64; by 4096 rows 21, 23, 31); with one tile of tokens two of rows take more
+  // 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 20, 23, 30); with one tile of tokens two of rows take more
   // registers than two workgroups a CU leave (4096 rows of 14336 columns: 21 us, 35)
   if constexpr (TILES == 1) {
     launch_stages<1, 1, HALF>(a, s);
@@ -405,9 +413,13 @@ void launch(const FourArgs &a, hipStream_t s) {
     else if (chunks <= 512) launch_gemv<256, 2, HALF>(a, s);
     else launch_gemv<256, 4, HALF>(a, s);
   } else if (a.m <= 16 && chunks <= 128) {
-    if (chunks <= 32) launch_rows<1, HALF>(a, s);
-    else if (chunks <= 64) launch_rows<2, HALF>(a, s);
-    else launch_rows<4, HALF>(a, s);
+    if (chunks <= 32) launch_rows<1, 1, HALF>(a, s);
+    else if (chunks <= 64) launch_rows<1, 2, HALF>(a, s);
+    else launch_rows<1, 4, HALF>(a, s);
+  } else if (a.m <= 32 && chunks <= 128) {
+    if (chunks <= 32) launch_rows<2, 1, HALF>(a, s);
+    else if (chunks <= 64) launch_rows<2, 2, HALF>(a, s);
+    else launch_rows<2, 4, HALF>(a, s);
   } else if (a.m <= 16) {
     launch_gemm<1, HALF>(a, s);
   } else if (a.m <= 32) {
