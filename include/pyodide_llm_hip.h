@@ -454,7 +454,7 @@ int64_t hk_pages_workspace(const hk_pages *pages);
 
 /* The keys and values of n rows into layer `layer`: row i to position positions[i] of sequence seqs[i] (seqs null: i). k and v
  * float32, n_kv_heads * head_size values a row, kv_stride floats apart (a multiple of 4; k and v 16-byte aligned), rounded to
- * the nearest, ties to even, where the cache is half. Rows whose sequence or position is outside the tables, or whose position
+ * the nearest, ties to even, where the cache is half (magnitudes of 65520 and above to infinity). Rows whose sequence or position is outside the tables, or whose position
  * has no page, are dropped. No two rows go to one position; a page that other sequences name too changes for them as well
  * (hk_pages_reserve parts it). */
 int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, const void *v, int32_t kv_stride,
@@ -478,7 +478,8 @@ int32_t hk_pages_attention(void *out, const void *q, const hk_pages *pages, int3
                            int32_t q_stride, int32_t out_stride, const void *seqs, const void *lengths, int32_t n,
                            int32_t longest, void *workspace, int64_t workspace_bytes, void *stream);
 
-/* the bytes of workspace an hk_pages_attention of n rows of at most `longest` positions takes (negative: HE_E_ARG) */
+/* the bytes of workspace an hk_pages_attention of at most n rows of at most `longest` positions takes: not less for more rows or
+ * longer ones (negative: HE_E_ARG) */
 int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int32_t n, int32_t longest);
 
 /* ---- 4-bit matrices (no counterpart in the reference: its matrices have 8 and 6 bits) ----

@@ -537,10 +537,15 @@ __global__ __launch_bounds__(256) void join_kernel(const PagesAttn a) {
   }
 }
 
+// workgroups that the heads of a row's piece take
+int tiles_of(const PagesView &c, int32_t nh) {
+  const int group = nh / c.nkv, most = c.half ? Kind<true>::heads : Kind<false>::heads;
+  return c.nkv * ((group + most - 1) / most);
+}
+
 template <int HS>
 void launch(const PagesAttn &a, hipStream_t s) {
-  const int group = a.nh / a.c.nkv, most = a.c.half ? 8 : 16;
-  const dim3 grid(a.most, a.c.nkv * ((group + most - 1) / most));
+  const dim3 grid(a.most, tiles_of(a.c, a.nh));
   if (a.c.half) hipLaunchKernelGGL((attend_kernel<HS, true>), grid, dim3(64 * WAVES), 0, s, a);
   else hipLaunchKernelGGL((attend_kernel<HS, false>), grid, dim3(64 * WAVES), 0, s, a);
   if (a.most > a.rows) hipLaunchKernelGGL(join_kernel<HS>, dim3(a.nh, a.rows), dim3(256), 0, s, a);
@@ -548,7 +553,7 @@ void launch(const PagesAttn &a, hipStream_t s) {
 
 // how a launch of `rows` rows of at most `longest` positions is cut
 void cut(PagesAttn &a) {
-  const int group = a.nh / a.c.nkv, most = a.c.half ? 8 : 16, tiles = a.c.nkv * ((group + most - 1) / most);
+  const int tiles = tiles_of(a.c, a.nh);
   a.parts = a.pieces = 0;
   // every row one piece where cutting it and joining its pieces takes longer: a block of a wave after another 1.3 us, the join
   // about 4 (one row of 512 positions 12.3 us against 9.7 and the join); where the rows fill the CUs by themselves up to twice
@@ -570,14 +575,14 @@ void cut(PagesAttn &a) {
 
 }  // namespace
 
+// for any launch of at most as many rows of at most as many positions: a program's largest step sizes it once
 int64_t pages_attention_workspace(const PagesView &c, int32_t nh, int32_t rows, int32_t longest) {
-  PagesAttn a = {};
-  a.c = c;
-  a.nh = nh;
-  a.rows = rows;
-  a.longest = longest;
-  cut(a);
-  return a.most > rows ? 4 * (((a.most * nh * 2 + 3) & ~3) + a.most * nh * c.hs) : 0;
+  if (longest <= 5 * UNIT) return 0;
+  const int tiles = tiles_of(c, nh);
+  const int64_t planned = std::min(rows, PLANNED), two = (longest + LEAST * UNIT - 1) / (LEAST * UNIT);
+  int64_t most = std::min(256 * occupancy(c.hs, c.half) / tiles + 1 + planned, planned * two);
+  if (rows > PLANNED && longest > 2048) most = std::max<int64_t>(most, std::min<int64_t>(16384 / tiles, (int64_t)rows * ((longest + 2047) / 2048)));
+  return 4 * (((most * nh * 2 + 3) & ~3) + most * nh * c.hs);
 }
 
 hipError_t launch_pages_attention(const PagesAttn &args, hipStream_t s) {

@@ -117,6 +117,18 @@ def test_attention_workspaces_that_are_refused():
     refused(lib.hk_pages_attention_workspace(ref, 8, 2, 6400001), b"longest")
 
 
+@pytest.mark.parametrize("half, heads, kv_heads, head_size", [(1, 8, 2, 64), (0, 32, 8, 128), (1, 1024, 1024, 16), (1, 32, 1, 256)])
+def test_a_workspace_serves_every_smaller_call(half, heads, kv_heads, head_size):
+    lib = package().library()
+    ref = ctypes.byref(made(half=half, n_kv_heads=kv_heads, head_size=head_size, page_size=32, table_size=100000, n_pages=100000))
+    rows, lengths = [1, 2, 31, 64, 255, 256, 257, 300, 5000, 65535], [0, 1, 640, 641, 1024, 1025, 2048, 2049, 50000, 3200000]
+    need = [[lib.hk_pages_attention_workspace(ref, heads, n, longest) for longest in lengths] for n in rows]
+    for i in range(len(rows)):
+        for j in range(len(lengths)):
+            assert need[i][j] >= (need[i - 1][j] if i else 0) and need[i][j] >= (need[i][j - 1] if j else 0)
+            assert need[i][j] <= 1 << 33
+
+
 @pytest.mark.parametrize("change, text", [
     (dict(m=0), b"m is in"), (dict(m=65536), b"m is in"), (dict(rows=0), b"rows"), (dict(rows=(1 << 26) + 1), b"rows"),
     (dict(k=0), b"k a multiple"), (dict(k=48), b"k a multiple"), (dict(k=(1 << 24) + 32), b"k a multiple"), (dict(bias=1), b"bias"),
