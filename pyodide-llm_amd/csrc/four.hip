@@ -18,6 +18,7 @@ namespace ple {
 namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
@@ -266,8 +267,7 @@ __device__ __forceinline__ void finish(const FourArgs &a, const float4 *sums, in
 // Up to 16 TILES tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves
 // sharing their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One
 // workgroup a CU: two have twice the loads on their way and came out slower (16 tokens by 14336 rows of 4096 columns 18.8 us
-// against 15.0). 16 tokens of these take 13.6 us, 34 MB: 6 until the first rows are done, 2 a turn; of 128,256 rows 64 (4.2 TB/s;
-// the weights' 64 bytes a row and load cost a sixth of it, measured with as many in one piece). 32 tokens: 19 and 85.
+// against 15.0). 16 tokens by 2304 rows of 768 columns take 3.6 us; 32 by 14336 of 4096 19, by 128,256 83.
 template <int TILES, int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a) {
   __shared__ Tokens<TILES, GEMM_WAVES * DEEP> tokens;
@@ -307,6 +307,68 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a)
       finish<1>(a, sums[turn], 16 * t, row0);
       turn ^= 1;
     }
+  }
+}
+
+// Up to 16 tokens of 1025 to 4096 columns: as rows_kernel, with the tokens in registers (a wave's columns stay the same) and the
+// weights on their way there through LDS. A wave's load takes 64 DEEP bytes of a row, whole cache lines, from 16 / DEEP rows; the
+// products' order, 64 bytes of each of 16, is LDS's: chunk k of row r lies at place k ^ r of the row's, so that neither side meets
+// a bank twice. 128,256 rows of 4096 columns, 271 MB, take 57 us (64 with loads of 64 bytes of 16 rows, 57 of them the loads'; 29
+// without any loads), 14336 12.9, of which about 6 pass until the first rows are done, 4096 7.7. Rows two turns ahead: the same.
+template <int DEEP, int GROUP, bool HALF>
+__global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a) {
+  typedef typename Weights<GROUP, HALF>::scales scales;
+  constexpr int CHUNKS = 4 * DEEP, ROWS = 64 / CHUNKS;  // of a row a load, and rows a load
+  __shared__ Tokens<1, GEMM_WAVES * DEEP> tokens;
+  __shared__ float4 sums[2][GEMM_THREADS];
+  __shared__ u32x4 chunks[GEMM_WAVES][16 * CHUNKS];
+  __shared__ scales factors[GEMM_WAVES][DEEP][16];
+  const int nc = (a.k + 127) / 128, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = wave * DEEP;
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4, d_mine = min(j, DEEP - 1);
+  const int64_t step = (int64_t)gridDim.x * 16;
+  u32x4 in[DEEP];
+  scales sc;
+  auto read = [&](int64_t row0) {
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      const int r = ROWS * i + lane / CHUNKS, k = lane % CHUNKS ^ r % CHUNKS;
+      const int64_t row = min(row0 + r, (int64_t)a.rows - 1);
+      in[i] = reinterpret_cast<const u32x4 *>(a.w)[row * nc * 4 + min(first * 4 + k, nc * 4 - 1)];
+    }
+    sc = reinterpret_cast<const scales *>(a.ws)[min(row0 + c, (int64_t)a.rows - 1) * nc + min(first + d_mine, nc - 1)];
+  };
+  {
+    Carrier<1, GEMM_WAVES * DEEP> carrier;
+    carrier.read(a, 0, 0);  // (before the weights, for which it would wait otherwise)
+    __builtin_amdgcn_sched_barrier(0);
+    read((int64_t)blockIdx.x * 16);
+    __builtin_amdgcn_sched_barrier(0);
+    carrier.write(a, 0, tokens);
+  }
+  __syncthreads();
+  Operand x[DEEP];
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d) x[d] = operand(tokens, 0, first + d);
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * 16; row0 < a.rows; row0 += step, turn ^= 1) {
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) chunks[wave][64 * i + lane] = in[i];
+    factors[wave][d_mine][c] = sc;
+    __builtin_amdgcn_wave_barrier();  // (a wave's own: LDS keeps its order)
+    read(row0 + step);
+    __builtin_amdgcn_sched_barrier(0);
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {  // (places past the columns: zeros)
+      Weights<GROUP, HALF> w;
+      w.in = __builtin_bit_cast(uint4, chunks[wave][c * CHUNKS + ((4 * d + j) ^ c % CHUNKS)]);
+      w.sc = factors[wave][d][c];
+      w.multiply(x[d], acc);
+    }
+    __builtin_amdgcn_wave_barrier();
+    sums[turn][threadIdx.x] = acc;
+    __syncthreads();  // (the next go to the other half)
+    finish<1>(a, sums[turn], 0, row0);
   }
 }
 
@@ -378,6 +440,14 @@ void launch_rows(const FourArgs &a, hipStream_t s) {
   else hipLaunchKernelGGL((rows_kernel<TILES, DEEP, 128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
 }
 
+template <int DEEP, bool HALF>
+void launch_lines(const FourArgs &a, hipStream_t s) {
+  const int blocks = (a.rows + 15) / 16, turns = (blocks + 255) / 256, grid = (blocks + turns - 1) / turns;
+  if (a.group == 32) hipLaunchKernelGGL((lines_kernel<DEEP, 32, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else if (a.group == 64) hipLaunchKernelGGL((lines_kernel<DEEP, 64, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((lines_kernel<DEEP, 128, HALF>), dim3(grid), dim3(GEMM_THREADS), 0, s, a);
+}
+
 template <int RT, int TILES, bool HALF>
 void launch_stages(const FourArgs &a, hipStream_t s) {
   const dim3 grid((a.rows + 16 * RT - 1) / (16 * RT), (a.m + 16 * TILES - 1) / (16 * TILES)), block(GEMM_THREADS);
@@ -414,8 +484,8 @@ void launch(const FourArgs &a, hipStream_t s) {
     else launch_gemv<256, 4, HALF>(a, s);
   } else if (a.m <= 16 && chunks <= 128) {
     if (chunks <= 32) launch_rows<1, 1, HALF>(a, s);
-    else if (chunks <= 64) launch_rows<1, 2, HALF>(a, s);
-    else launch_rows<1, 4, HALF>(a, s);
+    else if (chunks <= 64) launch_lines<2, HALF>(a, s);
+    else launch_lines<4, HALF>(a, s);
   } else if (a.m <= 32 && chunks <= 128) {
     if (chunks <= 32) launch_rows<2, 1, HALF>(a, s);
     else if (chunks <= 64) launch_rows<2, 2, HALF>(a, s);
