@@ -78,15 +78,21 @@ def quantize_four(matrix, group=32, half_scales=False):
     if group not in (32, 64, 128):
         raise ValueError("quantize_four(): group is 32, 64 or 128")
     rows, k = x.shape
-    x = np.pad(x, ((0, 0), (0, -k % 128))).reshape(rows, -1, group)
-    with np.errstate(over="ignore", invalid="ignore"):
-        ws = (np.abs(x).max(-1) / np.float32(7)).astype(np.float16 if half_scales else np.float32)
-        ws = np.where(np.isfinite(ws), ws, ws.dtype.type(0))
-        wide = ws.astype(np.float64)[..., None]
-        q = np.where(wide > 0, np.rint(np.clip(x / np.where(wide > 0, wide, 1.0), -8, 7)), 0.0).astype(np.int8)
-    # [row][of 128][t][low / high][j][i] -> [row][of 128][j][t][i]
-    q = q.reshape(rows, -1, 4, 2, 4, 4).transpose(3, 0, 1, 4, 2, 5).astype(np.uint8) & 15
-    return np.ascontiguousarray((q[0] | q[1] << 4).reshape(rows, -1)), ws
+    wide = k + -k % 128
+    w, ws = np.empty((rows, wide // 2), np.uint8), np.empty((rows, wide // group), np.float16 if half_scales else np.float32)
+    step = max(1, (1 << 24) // wide)  # rows at a time (float64 beside a large matrix)
+    for at in range(0, rows, step):
+        part = x[at:at + step]
+        part = np.pad(part, ((0, 0), (0, wide - k))).reshape(len(part), -1, group)
+        with np.errstate(over="ignore", invalid="ignore"):
+            s = (np.abs(part).max(-1) / np.float32(7)).astype(ws.dtype)
+            s = np.where(np.isfinite(s), s, s.dtype.type(0))
+            scale = s.astype(np.float64)[..., None]
+            q = np.where(scale > 0, np.rint(np.clip(part / np.where(scale > 0, scale, 1.0), -8, 7)), 0.0).astype(np.int8)
+        # [row][of 128][t][low / high][j][i] -> [row][of 128][j][t][i]
+        q = q.reshape(len(part), -1, 4, 2, 4, 4).transpose(3, 0, 1, 4, 2, 5).astype(np.uint8) & 15
+        w[at:at + step], ws[at:at + step] = (q[0] | q[1] << 4).reshape(len(part), -1), s
+    return w, ws
 
 
 def cache_shapes(n_kv_heads, head_size, seq_len):

@@ -98,6 +98,35 @@ def test_every_pair_of_values():
             np.testing.assert_array_equal(got, np.tile((vals * x).sum(-1), (m, 1)).astype(np.float32))
 
 
+@pytest.mark.parametrize("m, rows, k", [(1, 300, 4096), (1, 40, 9000 // 32 * 32), (16, 300, 4096), (7, 100, 768), (20, 300, 2048), (40, 70, 1024),
+                                        (5, 40, 8192)])
+def test_products_replayed_from_a_graph(m, rows, k):
+    import ctypes
+    from gpu_lib import hip, hip_check
+    h, rng = hip(), np.random.default_rng(m + k)
+    stream, graph, run = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    hip_check(h.hipStreamCreate(ctypes.byref(stream)))
+    xq, xs, w, ws = inputs(rng, m, rows, k, 64, 32, True)
+    args, y = [upload(a) for a in (xq, xs, w, ws)], Dev((m, rows), np.float32)
+    hip_check(h.hipDeviceSynchronize())
+    hip_check(h.hipStreamBeginCapture(stream, 2))
+    check(package().library().hk_matmul_four(y.ptr, *(a.ptr for a in args), m, rows, k, 64, 32, 1, stream))
+    hip_check(h.hipStreamEndCapture(stream, ctypes.byref(graph)))
+    hip_check(h.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0))
+    for _ in range(3):
+        xq, xs, _, _ = inputs(rng, m, 1, k, 64, 32, True)
+        for dev, x in zip(args, (xq, xs)):
+            hip_check(h.hipMemcpy(dev.ptr, ctypes.c_void_p(x.ctypes.data), dev.nbytes, 1))
+        hip_check(h.hipGraphLaunch(run, stream))
+        hip_check(h.hipStreamSynchronize(stream))
+        np.testing.assert_array_equal(y.numpy(), four(xq, xs, w, ws, rows, k, 64, 32))  # (an eager call between the replays)
+        want, off = product(xq, xs, w, ws, k, 64, 32)
+        assert (np.abs(y.numpy() - want) <= off).all()
+    hip_check(h.hipGraphExecDestroy(run))
+    hip_check(h.hipGraphDestroy(graph))
+    hip_check(h.hipStreamDestroy(stream))
+
+
 def test_a_step_of_conversations():
     """one layer of a decode step, as a program that answers several conversations makes it: quantized activations, q, k and v
     by 4-bit matrices, room and rows in the pages, attention, the output's product; against the same in float64 on the

@@ -446,6 +446,52 @@ def test_steps_replayed_from_a_graph():
     hip_check(h.hipStreamDestroy(stream))
 
 
+def test_housekeeping_replayed_from_a_graph():
+    """sequences ended, forked, given room and compacted by one captured graph, the lists changing between its replays"""
+    lib, h, rng = package().library(), hip(), np.random.default_rng(16)
+    model = filled(rng, 2, 2, 32, 16, False, [70, 40, 100, 0, 0, 33], spare=20, slots=8)
+    pages, lens, n = Pages(model), [70, 40, 100, 0, 0, 33], 3
+    lists = {name: ints([0] * n) for name in ("ended", "to", "source", "lengths", "ends")}
+    status, used = ints([7, 7]), ints([7])
+    stream, graph, run = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    hip_check(h.hipStreamCreate(ctypes.byref(stream)))
+    hip_check(h.hipDeviceSynchronize())
+    hip_check(h.hipStreamBeginCapture(stream, 2))
+    check(lib.hk_pages_free(pages.ref, lists["ended"].ptr, None, n, stream))
+    check(lib.hk_pages_fork(pages.ref, lists["to"].ptr, lists["source"].ptr, lists["lengths"].ptr, n, status.ptr, stream))
+    check(lib.hk_pages_reserve(pages.ref, lists["to"].ptr, lists["lengths"].ptr, lists["ends"].ptr, n, status.ptr.value + 4,
+                               pages.space.ptr, pages.need, stream))
+    check(lib.hk_pages_compact(pages.ref, used.ptr, pages.space.ptr, pages.need, stream))
+    hip_check(h.hipStreamEndCapture(stream, ctypes.byref(graph)))
+    hip_check(h.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0))
+    for _ in range(5):
+        order = rng.permutation(6).tolist()
+        ended, to = order[:1] + [-1, -1], order[1:4]
+        lens[ended[0]] = 0
+        source = [int(rng.choice(6)) for _ in to]
+        cut = [int(rng.integers(0, lens[f] + 1)) for f in source]
+        ends = [min(256, a + int(rng.integers(1, 40))) for a in cut]
+        for name, x in zip(lists, (ended, to, source, cut, ends)):
+            x = np.asarray(x, dtype=np.int32)
+            hip_check(h.hipMemcpy(lists[name].ptr, ctypes.c_void_p(x.ctypes.data), x.nbytes, 1))
+        hip_check(h.hipGraphLaunch(run, stream))
+        hip_check(h.hipStreamSynchronize(stream))
+        model.free(ended)
+        want = [model.fork(to, source, cut), model.reserve(to, cut, ends)]
+        assert status.numpy().tolist() == want and want[0] == 0
+        assert used.numpy()[0] == model.compact()
+        pages.same()
+        for s, a, b in zip(to, cut, ends):
+            lens[s] = b if want[1] == 0 else a
+        for x in (pages, model):  # an eager call between the replays
+            x.free([order[5]], [lens[order[5]] // 2])
+        lens[order[5]] //= 2
+        pages.same()
+    hip_check(h.hipGraphExecDestroy(run))
+    hip_check(h.hipGraphDestroy(graph))
+    hip_check(h.hipStreamDestroy(stream))
+
+
 def test_two_streams_at_once():
     """two layers' attention on two streams, each with its own workspace: the results of the calls one after the other"""
     lib, h, rng = package().library(), hip(), np.random.default_rng(11)
