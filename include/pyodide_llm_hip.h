@@ -440,8 +440,9 @@ int32_t hk_pages_fork(const hk_pages *pages, const void *to, const void *from, c
 int32_t hk_pages_reserve(const hk_pages *pages, const void *seqs, const void *starts, const void *ends, int32_t n,
                          void *status, void *workspace, int64_t workspace_bytes, void *stream);
 
-/* Sequences that end, or are cut: sequence seqs[i] keeps the pages of its first kept[i] positions (kept null: none) and gives
- * the others back. Sequences past the tables are passed over; of one listed twice the smaller number holds. */
+/* Sequences that end, or are cut: for each i < n (1..HK_PAGES_SEQS_MOST), sequence seqs[i] keeps the pages of its
+ * first kept[i] positions (kept null: none) and gives the others back. Sequences past the tables are passed over; of one listed
+ * twice the smaller number holds. */
 int32_t hk_pages_free(const hk_pages *pages, const void *seqs, const void *kept, int32_t n, void *stream);
 
 /* The pages in use together at the pool's beginning: of u pages in use, those at u or past it go to the free places below, in
@@ -452,11 +453,11 @@ int32_t hk_pages_compact(const hk_pages *pages, void *used, void *workspace, int
 /* the bytes of workspace that hk_pages_reserve and hk_pages_compact take (negative: HE_E_ARG) */
 int64_t hk_pages_workspace(const hk_pages *pages);
 
-/* The keys and values of n rows into layer `layer`: row i to position positions[i] of sequence seqs[i] (seqs null: i). k and v
- * float32, n_kv_heads * head_size values a row, kv_stride floats apart (a multiple of 4; k and v 16-byte aligned), rounded to
- * the nearest, ties to even, where the cache is half (magnitudes of 65520 and above to infinity). Rows whose sequence or position is outside the tables, or whose position
- * has no page, are dropped. No two rows go to one position; a page that other sequences name too changes for them as well
- * (hk_pages_reserve parts it). */
+/* The keys and values of n rows (1..2^20) into layer `layer`: row i to position positions[i] of sequence seqs[i] (seqs null:
+ * i). k and v float32, n_kv_heads * head_size values a row, kv_stride floats apart (a multiple of 4; k and v 16-byte aligned),
+ * rounded to the nearest, ties to even, where the cache is half (magnitudes of 65520 and above to infinity). Rows whose
+ * sequence or position is outside the tables, or whose position has no page, are dropped. No two rows go to one position; a
+ * page that other sequences name too changes for them as well (hk_pages_reserve parts it). */
 int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, const void *v, int32_t kv_stride,
                         const void *seqs, const void *positions, int32_t n, void *stream);
 
@@ -487,10 +488,12 @@ int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int
  * y[t][r] = sum_g ws xs[t][g] (sum over the 32 columns i of group g of w[r][i] (xq[t][i] - bias)) for m tokens and rows
  * r < rows: w in -8..7, its scale ws one a row and `group` (32, 64 or 128) columns; xq [m][k] and xs [m][k / 32] as
  * hk_quantize_x leaves them with the same bias (64 or 0). The sums within a group are exact in int32; those over the groups
- * float32's, in an order of the kernel's own. y is [m][rows] float32. k is a multiple of 32.
+ * float32's, in an order of the kernel's own. y is [m][rows] float32; m in 1..65535, rows in 1..2^26, k a multiple of 32 up to
+ * 2^24. The scales of w are finite (a row with one that is not is not finite either); an xs that is not concerns its token alone.
  *
- * A row of w, and its scales, are filled up with zeros to a multiple of 128 columns. 128 columns are 64 bytes; the 16-byte chunk j of them holds
- * in byte 4 t + i column 32 t + 4 j + i in its low four bits and column 32 t + 16 + 4 j + i in its high four (two's complement).
+ * A row of w, and its scales, are filled up with zeros to a multiple of 128 columns. 128 columns are 64 bytes; the 16-byte chunk
+ * j of them holds in byte 4 t + i column 32 t + 4 j + i in its low four bits and column 32 t + 16 + 4 j + i in its high four
+ * (two's complement).
  * ws is [rows][those columns / group], float32, or float16 with half_scales. w, ws and xq are 16-byte aligned, y and xs
  * 4-byte. Neither allocates nor waits. */
 int32_t hk_matmul_four(void *y, const void *xq, const void *xs, const void *w, const void *ws, int32_t m, int32_t rows,

@@ -340,8 +340,9 @@ __device__ __forceinline__ Piece piece_of(const PagesAttn &a, int find, int lane
     read(base + lane);
     total += (uint32_t)__builtin_amdgcn_readlane((int)wave_up_to(units), 63);
   }
-  // units a piece
-  const int each = min(max(LEAST, (int)((total + a.pieces - 1) / a.pieces)), (a.longest + UNIT - 1) / UNIT);
+  // units a piece (the total may be 2^31)
+  const uint32_t row_most = (a.longest + UNIT - 1) / UNIT;
+  const int each = max(LEAST, (int)min((total + a.pieces - 1) / a.pieces, row_most));
   p.chunk = each * UNIT;
   p.row = -1;
   for (int base = 0, before = 0; base < a.rows; base += 64) {

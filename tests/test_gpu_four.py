@@ -98,6 +98,21 @@ def test_every_pair_of_values():
             np.testing.assert_array_equal(got, np.tile((vals * x).sum(-1), (m, 1)).astype(np.float32))
 
 
+@pytest.mark.parametrize("m, rows, k", [(3, 40, 768), (5, 40, 2048), (20, 40, 2048), (17, 40, 768), (40, 70, 1024), (6, 40, 8192)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_scale_that_is_not_finite_concerns_its_token_alone(m, rows, k, bad):
+    rng = np.random.default_rng(m + k)
+    xq, xs, w, ws = inputs(rng, m, rows, k, 64, 64, False)
+    want = four(xq, xs, w, ws, rows, k, 64, 64)
+    for t in {0, m // 2, m - 1}:
+        other = xs.copy()
+        other[t, k // 64] = bad
+        y = four(xq, other, w, ws, rows, k, 64, 64)
+        assert not np.isfinite(y[t]).any()
+        keep = np.arange(m) != t
+        np.testing.assert_array_equal(y[keep], want[keep])
+
+
 @pytest.mark.parametrize("m, rows, k", [(1, 300, 4096), (1, 40, 9000 // 32 * 32), (16, 300, 4096), (7, 100, 768), (20, 300, 2048), (40, 70, 1024),
                                         (5, 40, 8192)])
 def test_products_replayed_from_a_graph(m, rows, k):
