@@ -459,13 +459,14 @@ void launch_stages(const FourArgs &a, hipStream_t s) {
 template <int TILES, bool HALF>
 void launch_gemm(const FourArgs &a, hipStream_t s) {
   // rows a workgroup: as many as leave about one workgroup a CU, since each brings the activations to LDS for itself (64 tokens by
-  // 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 20, 23, 30); with one tile of tokens two of rows take more
-  // registers than two workgroups a CU leave (4096 rows of 14336 columns: 21 us, 35)
+  // 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 20, 23, 30; 2048 tokens by 4096 rows 408 at 16, 222 at 64); with
+  // one tile of tokens two of rows take more registers than two workgroups a CU leave (4096 rows of 14336 columns: 21 us, 35)
   if constexpr (TILES == 1) {
     launch_stages<1, 1, HALF>(a, s);
   } else {
-    if (a.rows >= 12800) launch_stages<4, TILES, HALF>(a, s);
-    else if (a.rows >= 6400) launch_stages<2, TILES, HALF>(a, s);
+    const int64_t rows = (int64_t)a.rows * ((a.m + 16 * TILES - 1) / (16 * TILES));  // times the tiles of tokens
+    if (rows >= 12800) launch_stages<4, TILES, HALF>(a, s);
+    else if (rows >= 6400) launch_stages<2, TILES, HALF>(a, s);
     else launch_stages<1, TILES, HALF>(a, s);
   }
 }
