@@ -18,6 +18,7 @@ namespace ple {
 namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -139,7 +140,7 @@ constexpr int GEMM_WAVES = 8, GEMM_THREADS = 64 * GEMM_WAVES;
 template <int TILES, int PLACES>
 struct Tokens {
   uint4 x[TILES][PLACES][2][64];
-  float4 xs[TILES][PLACES][4][4];
+  float xs[TILES][PLACES][64];
 };
 
 // a thread's part in bringing them there: 16 columns of a token, and a group's scale, a load; all loads before the stores
@@ -180,7 +181,7 @@ struct Carrier {
 #pragma unroll
     for (int i = 0; i < SCALES; ++i) {
       const int q = scale(i) / TILES;
-      reinterpret_cast<float *>(to.xs[scale(i) % TILES][q][part()])[token()] = (c0 + q) * 4 + part() < a.k / 32 ? f[i] : 0.0f;
+      to.xs[scale(i) % TILES][q][part() * 16 + token()] = (c0 + q) * 4 + part() < a.k / 32 ? f[i] : 0.0f;
     }
   }
 };
@@ -188,7 +189,7 @@ struct Carrier {
 // what a product of 16 tokens and 128 columns takes of them, of one lane
 struct Operand {
   uint4 lo, hi;
-  float4 f[4];
+  float f;
 };
 template <int TILES, int PLACES>
 __device__ __forceinline__ Operand operand(const Tokens<TILES, PLACES> &tokens, int tile, int place) {
@@ -196,55 +197,42 @@ __device__ __forceinline__ Operand operand(const Tokens<TILES, PLACES> &tokens, 
   Operand x;
   x.lo = tokens.x[tile][place][0][lane];
   x.hi = tokens.x[tile][place][1][lane];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) x.f[g] = tokens.xs[tile][place][g][lane >> 4];
+  x.f = tokens.xs[tile][place][lane];
   return x;
 }
 
-// a lane's weights of 128 columns and their scales, a row's
+// a lane's weights of 128 columns, and the scale of its quarter's group, of a row
 template <int GROUP, bool HALF>
 struct Weights {
-  static constexpr int EACH = 128 / GROUP;
-  typedef typename Scale<HALF>::type scales __attribute__((ext_vector_type(EACH)));
+  typedef typename Scale<HALF>::type scale;
+  static constexpr int EACH = 128 / GROUP;  // scales of a row's 128 columns
   uint4 in;
-  scales sc;
+  scale sc;
 
   __device__ __forceinline__ void read(const FourArgs &a, int64_t row, int place, int nc) {
-    in = reinterpret_cast<const uint4 *>(a.w)[(row * nc + place) * 4 + ((threadIdx.x & 63) >> 4)];
-    sc = reinterpret_cast<const scales *>(a.ws)[row * nc + place];
+    const int j = (threadIdx.x & 63) >> 4;
+    in = reinterpret_cast<const uint4 *>(a.w)[(row * nc + place) * 4 + j];
+    sc = reinterpret_cast<const scale *>(a.ws)[(row * nc + place) * EACH + j * EACH / 4];
   }
-  // D = X W^T, 16 tokens by 16 rows: a lane has one row's sums for four tokens, so that the row's scales are its own and the
-  // tokens' come four at a time
+  // D = X W^T, 16 tokens by 16 rows, a group a product; and so the scales: one product of single columns has xs ws of the four
+  // groups, each in the place of its sum, and leaves a conversion and an fma a sum (16 tokens by 4096 rows of 4096 columns 7.7 ->
+  // 7.2 us, 32 by 14336 19 -> 17, against scaling by the tokens' and the rows' one after the other)
   __device__ __forceinline__ void multiply(const Operand &x, float4 &acc) const {
     const uint32_t bits[4] = {in.x, in.y, in.z, in.w};
     const long av[4] = {(long)((uint64_t)x.lo.y << 32 | x.lo.x), (long)((uint64_t)x.lo.w << 32 | x.lo.z),
                         (long)((uint64_t)x.hi.y << 32 | x.hi.x), (long)((uint64_t)x.hi.w << 32 | x.hi.z)};
+    const f32x16 f = __builtin_amdgcn_mfma_f32_16x16x1f32(x.f, (float)sc, f32x16{}, 0, 0, 0);
     i32x4 s[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       s[g] = __builtin_amdgcn_mfma_i32_16x16x32_i8(av[g], (long)((uint64_t)high_bits(bits[g]) << 32 | low_bits(bits[g])),
                                                    i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-    for (int g = 0; g < 4; g += 4 / EACH) {
-      float4 y;  // of the groups that share a scale
-#pragma unroll
-      for (int i = 0; i < 4 / EACH; ++i) {
-        const i32x4 v = s[g + i];
-        const float4 f = x.f[g + i];
-        if (i == 0) {
-          y = make_float4((float)v[0] * f.x, (float)v[1] * f.y, (float)v[2] * f.z, (float)v[3] * f.w);
-        } else {
-          y.x = __builtin_fmaf((float)v[0], f.x, y.x);
-          y.y = __builtin_fmaf((float)v[1], f.y, y.y);
-          y.z = __builtin_fmaf((float)v[2], f.z, y.z);
-          y.w = __builtin_fmaf((float)v[3], f.w, y.w);
-        }
-      }
-      const float scale = (float)sc[g * EACH / 4];
-      acc.x = __builtin_fmaf(y.x, scale, acc.x);
-      acc.y = __builtin_fmaf(y.y, scale, acc.y);
-      acc.z = __builtin_fmaf(y.z, scale, acc.z);
-      acc.w = __builtin_fmaf(y.w, scale, acc.w);
+    for (int g = 0; g < 4; ++g) {
+      acc.x = __builtin_fmaf((float)s[g][0], f[4 * g], acc.x);
+      acc.y = __builtin_fmaf((float)s[g][1], f[4 * g + 1], acc.y);
+      acc.z = __builtin_fmaf((float)s[g][2], f[4 * g + 2], acc.z);
+      acc.w = __builtin_fmaf((float)s[g][3], f[4 * g + 3], acc.w);
     }
   }
 };
@@ -267,7 +255,7 @@ __device__ __forceinline__ void finish(const FourArgs &a, const float4 *sums, in
 // Up to 16 TILES tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves
 // sharing their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One
 // workgroup a CU: two have twice the loads on their way and came out slower (16 tokens by 14336 rows of 4096 columns 18.8 us
-// against 15.0). 16 tokens by 2304 rows of 768 columns take 3.6 us; 32 by 14336 of 4096 19, by 128,256 83.
+// against 15.0). 16 tokens by 2304 rows of 768 columns take 3.6 us; 32 by 14336 of 4096 17.
 template <int TILES, int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a) {
   __shared__ Tokens<TILES, GEMM_WAVES * DEEP> tokens;
@@ -313,11 +301,12 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a)
 // Up to 16 tokens of 1025 to 4096 columns: as rows_kernel, with the tokens in registers (a wave's columns stay the same) and the
 // weights on their way there through LDS. A wave's load takes 64 DEEP bytes of a row, whole cache lines, from 16 / DEEP rows; the
 // products' order, 64 bytes of each of 16, is LDS's: chunk k of row r lies at place k ^ r of the row's, so that neither side meets
-// a bank twice. 128,256 rows of 4096 columns, 271 MB, take 57 us (64 with loads of 64 bytes of 16 rows, 57 of them the loads'; 29
-// without any loads), 14336 12.9, of which about 6 pass until the first rows are done, 4096 7.7. Rows two turns ahead: the same.
+// a bank twice. 128,256 rows of 4096 columns, 271 MB, take 57 us (64 with loads of 64 bytes of 16 rows), 14336 11.8, of which
+// about 6 pass until the first rows are done, 4096 7.2. Rows two turns ahead: the same.
 template <int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a) {
-  typedef typename Weights<GROUP, HALF>::scales scales;
+  constexpr int EACH = Weights<GROUP, HALF>::EACH;
+  typedef typename Scale<HALF>::type scales __attribute__((ext_vector_type(EACH)));
   constexpr int CHUNKS = 4 * DEEP, ROWS = 64 / CHUNKS;  // of a row a load, and rows a load
   __shared__ Tokens<1, GEMM_WAVES * DEEP> tokens;
   __shared__ float4 sums[2][GEMM_THREADS];
@@ -362,7 +351,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a
     for (int d = 0; d < DEEP; ++d) {  // (places past the columns: zeros)
       Weights<GROUP, HALF> w;
       w.in = __builtin_bit_cast(uint4, chunks[wave][c * CHUNKS + ((4 * d + j) ^ c % CHUNKS)]);
-      w.sc = factors[wave][d][c];
+      w.sc = reinterpret_cast<const typename Scale<HALF>::type *>(&factors[wave][d][c])[j * EACH / 4];
       w.multiply(x[d], acc);
     }
     __builtin_amdgcn_wave_barrier();
@@ -458,15 +447,16 @@ void launch_stages(const FourArgs &a, hipStream_t s) {
 
 template <int TILES, bool HALF>
 void launch_gemm(const FourArgs &a, hipStream_t s) {
-  // rows a workgroup: as many as leave about one workgroup a CU, since each brings the activations to LDS for itself (64 tokens by
-  // 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 20, 23, 30; 2048 tokens by 4096 rows 408 at 16, 222 at 64); with
-  // one tile of tokens two of rows take more registers than two workgroups a CU leave (4096 rows of 14336 columns: 21 us, 35)
+  // rows a workgroup: the fewest whose workgroups are not more than the CUs, since each brings the activations to LDS for itself
+  // (64 tokens by 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 19, 23, 30; 2048 tokens by 4096 rows 408 at 16, 217
+  // at 64); with one tile of tokens two of rows take more registers than two workgroups a CU leave (4096 rows of 14336 columns:
+  // 21 us, 35)
   if constexpr (TILES == 1) {
     launch_stages<1, 1, HALF>(a, s);
   } else {
     const int64_t rows = (int64_t)a.rows * ((a.m + 16 * TILES - 1) / (16 * TILES));  // times the tiles of tokens
-    if (rows >= 12800) launch_stages<4, TILES, HALF>(a, s);
-    else if (rows >= 6400) launch_stages<2, TILES, HALF>(a, s);
+    if (rows > 8192) launch_stages<4, TILES, HALF>(a, s);
+    else if (rows > 4096) launch_stages<2, TILES, HALF>(a, s);
     else launch_stages<1, TILES, HALF>(a, s);
   }
 }
