@@ -79,6 +79,22 @@ def test_rows_of_every_length(m, k):
     assert (np.abs(four(xq, xs, w, ws, rows, k, 64, 64) - want) <= off).all()
 
 
+@pytest.mark.parametrize("group, half", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("m, rows, k", [(600, 411, 416), (600, 833, 416), (70, 2051, 1056), (130, 2739, 96), (49, 4101, 288), (40, 8209, 160),
+                                        (20, 4111, 4128), (31, 8195, 4160), (16, 2050, 2112), (16, 4099, 1056), (32, 4105, 1312)])
+def test_many_rows_of_many_tokens(m, rows, k, group, half):
+    """the rows that a workgroup takes go by the tokens too: 16, 32 and 64 of them, with rows, tokens and columns left over"""
+    rng = np.random.default_rng(m * rows + k)
+    xq, xs, w, ws = inputs(rng, m, rows, k, 64, group, half)
+    got = four(xq, xs, w, ws, rows, k, 64, group)
+    some = np.unique(np.r_[np.arange(70), rng.integers(0, rows, 120), np.arange(rows - 70, rows)])  # (of the rows: the oracle's time)
+    want, off = product(xq, xs, w[some], ws[some], k, 64, group)
+    assert (np.abs(got[:, some] - want) <= off).all()
+    alone = four(xq[m // 2:m // 2 + 1], xs[m // 2:m // 2 + 1], w, ws, rows, k, 64, group)  # (all the rows, by another kernel)
+    _, off = product(xq[m // 2:m // 2 + 1], xs[m // 2:m // 2 + 1], w, ws, k, 64, group)
+    assert (np.abs(got[m // 2] - alone[0]) <= 2 * off[0]).all()
+
+
 def test_every_pair_of_values():
     """all 4-bit values against all activations at the ends of their range"""
     rows, k = 16, 160
