@@ -42,7 +42,7 @@ template <>
 struct Kind<false> {
   typedef float type;
   static constexpr int heads = 16;
-  static constexpr float ahead = 0.0f;  // (values of any size: no probability is above 1)
+  static constexpr float ahead = 0.0f;  // (values may be large: no probability is above 1, but for the reference's rounding)
 };
 
 // lane ^ 8 within 16: the other half of a column's products
@@ -258,17 +258,20 @@ struct Wave {
   __device__ __forceinline__ void probabilities(const f32x4 (&s)[2], int left, f16x8 &ph, f32x4 (&p)[2]) {
     const float most = scores(s, p, left);
     if (__any(most > bar)) {
-      const float next = column_max(most);
-      if (next > -INF) {
-        const float more = bar > -INF ? __builtin_fmaxf(next, 0.0f) : next;
-        const float less = bar > -INF ? __builtin_amdgcn_exp2f(-more) : 0.0f;
-        reference += more;
-        bar = Kind<HALF>::ahead;
+      const float top = column_max(most);
+      float next = reference;
+      if (top > -INF) next = bar > -INF ? reference + __builtin_fmaxf(top, 0.0f) : top;
+      // what is held follows the reference as it is rounded: a score that lies above it by less (the same one, block after block:
+      // the reference is its float32) moves nothing
+      if (__any(next != reference || (bar == -INF && top > -INF))) {
+        const float less = bar > -INF ? __builtin_amdgcn_exp2f(reference - next) : 0.0f;
+        reference = next;
+        if (top > -INF) bar = Kind<HALF>::ahead;
         sum *= less;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) o[t] *= less;
+        scores(s, p, left);
       }
-      scores(s, p, left);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
