@@ -28,14 +28,16 @@ constexpr int UNIT = BLOCK * WAVES, LEAST = 2;  // positions of a piece: a multi
 constexpr int PLANNED = 256;  // rows a launch's workgroups look through
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float INF = __builtin_inff();
-constexpr float PIECE_UP = 64.0f;  // what float16 halves of probabilities are raised by: up to 2^14
+constexpr float PIECE_UP = 64.0f;  // what float16 halves of probabilities are raised by: up to 2^15
 constexpr float LOW = 2048.0f;     // the second half's scale
+constexpr float WHOLE = 0x1p24f;   // from here on float32 has not every whole number
+constexpr float LOWEST = -3.402823466e38f;
 
 template <bool HALF>
 struct Kind {
   typedef _Float16 type;
   static constexpr int heads = 8;
-  // how far (log2) a score may lie above the reference before that moves
+  // how far (log2) a score may lie above the reference (and its rounding) before that moves
   static constexpr float ahead = 8.0f;
 };
 template <>
@@ -141,7 +143,7 @@ struct Wave {
   chunk k[2][KEYS];
   Values<HS, HALF> v;
   float up, up_low;  // what a product is multiplied by: a score in log2
-  // the scores' reference, and how far above it one may lie (-INF: there is no reference yet)
+  // the scores' reference, and how far above it one may lie (-INF: there is no reference yet; LOWEST: none is taken as it is)
   float reference = 0.0f, bar = -INF, sum = 0.0f;
   f32x4 o[TILES];
   int c, j;  // the lane's column and quarter
@@ -232,9 +234,8 @@ struct Wave {
       }
   }
 
-  // the products' scores (log2) over the reference, and the largest of the lane's: one rounding at their own size, not at the
-  // scores'
-  __device__ __forceinline__ float scores(const f32x4 (&s)[2], f32x4 (&x)[2], int left) const {
+  // the products' scores (log2) over `from`, and the largest of the lane's: one rounding at their own size, not at the scores'
+  __device__ __forceinline__ float scores(const f32x4 (&s)[2], f32x4 (&x)[2], int left, float from) const {
     float most = -INF;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -243,9 +244,9 @@ struct Wave {
         float y;
         if constexpr (HALF) {
           const float other = other_half(s[t][r]);
-          y = __builtin_fmaf(c < 8 ? other : s[t][r], up_low, __builtin_fmaf(c < 8 ? s[t][r] : other, up, -reference));
+          y = __builtin_fmaf(c < 8 ? other : s[t][r], up_low, __builtin_fmaf(c < 8 ? s[t][r] : other, up, -from));
         } else {
-          y = __builtin_fmaf(s[t][r], up, -reference);
+          y = __builtin_fmaf(s[t][r], up, -from);
         }
         if (16 * t + 4 * j + r >= left) y = -INF;
         x[t][r] = y;
@@ -256,22 +257,30 @@ struct Wave {
 
   // the probabilities of the products' scores, as the second product takes them; `left` of the positions are the row's
   __device__ __forceinline__ void probabilities(const f32x4 (&s)[2], int left, f16x8 &ph, f32x4 (&p)[2]) {
-    const float most = scores(s, p, left);
+    const float most = scores(s, p, left, reference);
     if (__any(most > bar)) {
-      const float top = column_max(most);
-      float next = reference;
-      if (top > -INF) next = bar > -INF ? reference + __builtin_fmaxf(top, 0.0f) : top;
-      // what is held follows the reference as it is rounded: a score that lies above it by less (the same one, block after block:
-      // the reference is its float32) moves nothing
-      if (__any(next != reference || (bar == -INF && top > -INF))) {
-        const float less = bar > -INF ? __builtin_amdgcn_exp2f(reference - next) : 0.0f;
-        reference = next;
-        if (top > -INF) bar = Kind<HALF>::ahead;
+      // the reference is the largest score as float32 has it, and what is held follows that: a score that is met again, and lies
+      // above its float32, moves nothing
+      const bool held = bar > -INF;
+      const float top = column_max(__any(held) ? scores(s, p, left, 0.0f) : most);
+      const float next = held ? __builtin_fmaxf(reference, top) : top > -INF ? top : 0.0f;
+      if (__any(held && next != reference)) {
+        const float less = held ? __builtin_amdgcn_exp2f(reference - next) : 1.0f;
         sum *= less;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) o[t] *= less;
-        scores(s, p, left);
       }
+      reference = next;
+      // From 2^24 on float32's numbers are two apart, and what a rounding leaves of a score is no exponent any more (from 2^28 on it
+      // made infinities, or zeros everywhere): there the scores are float32's too, block by block
+      const bool whole = __builtin_fabsf(next) >= WHOLE;
+      if (top > -INF) bar = whole ? LOWEST : __builtin_fmaf(__builtin_fabsf(next), 0x1p-24f, Kind<HALF>::ahead);
+      const f32x4 rounded[2] = {p[0], p[1]};
+      scores(s, p, left, next);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[t][r] = whole ? rounded[t][r] - next : p[t][r];
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)

@@ -77,3 +77,51 @@ def test_keys_that_repeat_beside_a_score_that_grows(half):
     weight = np.exp(-2.0 * np.arange(n // 32))[::-1].repeat(32)
     want = (weight[n // 2:].sum() / weight.sum())
     assert (np.abs(got[:, [0, 8], 32:] - want) <= 2 * off).all() and (got[:, [0, 8], :32] <= 1e-30).all()
+
+
+# (float32's whole numbers are two apart from 2^24 on; ordinary scores beside them in the same products)
+HUGE = [1e7, -2.3e7, 3e8, 3.3, 1.1e9, -1.1e9, 30.3, 5.3e10, 7.7e20, -100.7, -7.7e30, 377.3] * 2 + [-5.3e10, 2.0 ** 30, 0.0, -2.0 ** 40] * 2
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows, n", [(1, 512), (1, 8192), (96, 8192)])
+def test_huge_scores_that_repeat_weigh_the_same(rows, n, half):
+    got = Pages(halves(half, 8, n)).attention(0, queries(HUGE, rows, 4), [0] * rows, [n] * rows, 32)
+    means(got, (n / 4 + 4 + 16 + 32 + 1) * U)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("score", [1e7, 3e8, 1.1e9, 5.3e10, 7.7e20, 7.7e30])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_one_huge_score_takes_all(score, sign, half):
+    """a key of 2 among keys of 1 (of 1 among keys of 2, where the scores are negative): its values. Off by the roundings of its
+    probability's halves (2^-23), of their products with the value and their sums (4), of the joins (2) and the division"""
+    rng, n = np.random.default_rng(21), 1030
+    model = Model(1, 20, 1, 64, CHANNELS, half, 1, 17, rng)
+    model.tables[0] = rng.permutation(20)[:17]
+    q = queries([sign * score, 0.25 * sign * score], 1, 2)
+    for position in (0, 31, 500, 511, 1029):
+        model.keys[:] = 1 if sign > 0 else 2
+        held = model.tables[0, position // 64]
+        model.keys[0, held, 0, position % 64] = 2 if sign > 0 else 1
+        want = model.values[0, held, 0, position % 64].astype(np.float64)
+        got = Pages(model).attention(0, q, None, [n], 2)
+        assert (np.abs(got - want) <= 10 * U * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("step", [1e7, -1e7, 1e9, -1e9, 1e20])
+def test_huge_scores_that_rise_and_fall(step, half):
+    """from position to position by more than float32 leaves between them: the first's or the last's values"""
+    rng, n = np.random.default_rng(22), 1030
+    model = Model(1, 17, 1, 64, CHANNELS, half, 1, 17, rng)
+    model.tables[0] = rng.permutation(17)
+    model.keys[:] = 0
+    for slot, held in enumerate(model.tables[0]):
+        model.keys[0, held, 0, :, 3] = slot * 64 + np.arange(64)
+    q = np.zeros((1, 2 * CHANNELS), dtype=np.float32)
+    q[0, [3, CHANNELS + 3]] = np.float32(8 * step) * np.float32([1, 0.5])
+    best = n - 1 if step > 0 else 0
+    want = model.values[0, model.tables[0, best // 64], 0, best % 64].astype(np.float64)
+    got = Pages(model).attention(0, q, None, [n], 2)
+    assert (np.abs(got - want) <= 10 * U * np.abs(want)).all()
