@@ -18,6 +18,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int THREADS = 1024;  // of the workgroup that decides
 constexpr int BATCH = 16;      // counts a thread reads at a time
 constexpr int COPIERS = 2048, MOVERS = 4096;  // workgroups of a launch that copies rows, and of one that moves pages
+constexpr int FORKERS = 1 << 16;  // of one that forks, at most (a launch has fewer than 2^32 threads, a table up to 2^25 slots)
 
 __device__ __forceinline__ bool a_page(const PagesView &c, int32_t p) { return (uint32_t)p < (uint32_t)c.n_pages; }
 
@@ -73,8 +74,8 @@ __device__ __forceinline__ void counts(const PagesView &c, int32_t p, int32_t pa
 
 // ---- fork ----
 
-// A workgroup takes `cols` slots of every listed sequence: what their rows shall hold is read before any of it is written, so that
-// a sequence may be read and written by one call. Latency: the lists, the tables, the counts (16 sequences 4.4 us).
+// A workgroup takes `cols` slots of every listed sequence, and goes on a launch further: what their rows shall hold is read before
+// any of it is written, so that a sequence may be read and written by one call. Latency: the lists, the tables, the counts (16 sequences 4.4 us).
 __global__ __launch_bounds__(256) void fork_kernel(const PagesView c, const int32_t *to, const int32_t *from,
                                                    const int32_t *lengths, int n, int cols, int32_t *status) {
   extern __shared__ int32_t lds[];
@@ -85,23 +86,24 @@ __global__ __launch_bounds__(256) void fork_kernel(const PagesView c, const int3
   });
   if (blockIdx.x == 0 && threadIdx.x == 0 && status) *status = good ? 0 : -1;
   if (!good) return;
-  const int first = blockIdx.x * cols;
-  for (int e = threadIdx.x; e < n * cols; e += 256) {
-    const int i = e / cols, slot = first + e % cols;
-    int32_t a = -1;
-    if (to[i] >= 0 && slot < c.slots && slot * c.page < lengths[i]) a = c.tables[entry(c, from[i], slot)];
-    next[e] = a_page(c, a) ? a : -1;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < n * cols; e += 256) {
-    const int32_t s = to[e / cols], slot = first + e % cols, a = next[e];
-    if (s < 0 || slot >= c.slots) continue;
-    int32_t *at = &c.tables[entry(c, s, slot)];
-    const int32_t b = *at;
-    if (a == b) continue;
-    if (a >= 0) atomicAdd(&c.refs[a], 1);
-    if (a_page(c, b)) atomicSub(&c.refs[b], 1);
-    *at = a;
+  for (int first = blockIdx.x * cols; first < c.slots; first += gridDim.x * cols) {
+    for (int e = threadIdx.x; e < n * cols; e += 256) {
+      const int i = e / cols, slot = first + e % cols;
+      int32_t a = -1;
+      if (to[i] >= 0 && slot < c.slots && slot * c.page < lengths[i]) a = c.tables[entry(c, from[i], slot)];
+      next[e] = a_page(c, a) ? a : -1;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n * cols; e += 256) {  // (a thread's own entries of `next`)
+      const int32_t s = to[e / cols], slot = first + e % cols, a = next[e];
+      if (s < 0 || slot >= c.slots) continue;
+      int32_t *at = &c.tables[entry(c, s, slot)];
+      const int32_t b = *at;
+      if (a == b) continue;
+      if (a >= 0) atomicAdd(&c.refs[a], 1);
+      if (a_page(c, b)) atomicSub(&c.refs[b], 1);
+      *at = a;
+    }
   }
 }
 
@@ -385,8 +387,8 @@ int64_t pages_workspace(const PagesView &c) {
 hipError_t launch_pages_fork(const PagesView &c, const int32_t *to, const int32_t *from, const int32_t *lengths, int32_t n,
                              int32_t *status, hipStream_t s) {
   const int cols = std::max(1, std::min(16, 8192 / n));
-  hipLaunchKernelGGL(fork_kernel, dim3((c.slots + cols - 1) / cols), dim3(256), PAGES_SEQS_MOST / 8 + 4 * n * cols, s, c, to, from,
-                     lengths, n, cols, status);
+  hipLaunchKernelGGL(fork_kernel, dim3(std::min((c.slots + cols - 1) / cols, FORKERS)), dim3(256), PAGES_SEQS_MOST / 8 + 4 * n * cols,
+                     s, c, to, from, lengths, n, cols, status);
   return hipGetLastError();
 }
 
