@@ -343,7 +343,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) chunks[wave][64 * i + lane] = in[i];
     factors[wave][d_mine][c] = sc;
-    __builtin_amdgcn_wave_barrier();  // (a wave's own: LDS keeps its order)
+    wave_sync_lds();  // (a wave's own part)
     read(row0 + step);
     __builtin_amdgcn_sched_barrier(0);
     float4 acc = make_float4(0, 0, 0, 0);
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a
       w.sc = reinterpret_cast<const typename Scale<HALF>::type *>(&factors[wave][d][c])[j * EACH / 4];
       w.multiply(x[d], acc);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync_lds();
     sums[turn][threadIdx.x] = acc;
     __syncthreads();  // (the next go to the other half)
     finish<1>(a, sums[turn], 0, row0);
