@@ -399,6 +399,8 @@ int64_t hk_logprobs_workspace(int32_t m, int32_t n, int32_t top);
  * list is passed over: lists may be filled up. None of these calls allocates or waits: they may be captured into a graph.
  * Calls on one cache are ordered by the caller (one stream, or events); hk_pages_append and hk_pages_attention of different
  * layers may overlap.
+ * A call writes its *status whatever it was: calls that are queued one after another, and looked at later, take a word each (a
+ * fork that is refused leaves its sequences without the pages, and the reserve behind it may well succeed).
  *
  * A step of a program that answers n sequences: hk_pages_reserve for each one's next position, then layer by layer
  * hk_pages_append of the new keys and values and hk_pages_attention over one position more. */

@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from pages_lib import Model, Pages
+from gpu_lib import check
+from pages_lib import Model, Pages, filled, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -26,4 +27,19 @@ def test_a_fork_of_the_longest_tables_by_a_list_that_is_filled_up():
         held = -(-length // 32)
         model.tables[1, :held], model.tables[1, held:] = model.tables[0, :held], -1
         model.refs[:] = np.bincount(model.tables[model.tables >= 0], minlength=40)
+        pages.same()
+
+
+def test_a_refused_fork_shows_in_a_status_of_its_own():
+    """a fork and a reserve queued one after the other, the fork's lists such as are refused: a word each tells both; one word would
+    say that all is well, over a sequence that never got the pages"""
+    pages = Pages(filled(np.random.default_rng(2), 1, 1, 32, 16, True, [70, 0, 0]))
+    model, lib = pages.m, pages.lib
+    to, source, starts, ends, status = ints([1, 2]), ints([0, 3]), ints([70, 70]), ints([71, 71]), ints([77, 77])
+    for words in ((0, 4), (0, 0)):
+        check(lib.hk_pages_fork(pages.ref, to.ptr, source.ptr, starts.ptr, 2, status.ptr.value + words[0], None))
+        check(lib.hk_pages_reserve(pages.ref, to.ptr, starts.ptr, ends.ptr, 2, status.ptr.value + words[1], pages.space.ptr, pages.need, None))
+        assert status.numpy().tolist() == ([-1, 0] if words[1] else [0, 0])
+        assert model.reserve([1, 2], [70, 70], [71, 71]) == 0
+        assert (model.tables[1:, :2] < 0).all()
         pages.same()
