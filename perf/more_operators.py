@@ -286,6 +286,8 @@ def _handle(state):
         else:
             need = pk.library().hk_pages_workspace(ctypes.byref(pages))
         space = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
+        if case["kind"] == "branch":  # (a fork's status beside the reserve's: each call writes its own)
+            state["forked"] = torch.zeros_like(state["status"])
         state["handle"] = (pk.library(), pk.hip_engine.check, ctypes.byref(pages), space, need)
     return state["handle"]
 
@@ -295,7 +297,7 @@ def _own_branch(state):
     stream, n, to = torch.cuda.current_stream().cuda_stream, state["to"].numel(), state["to"].data_ptr()
     starts, status = state["starts"].data_ptr(), state["status"].data_ptr()
     check(lib.hk_pages_free(pages, to, state["none"].data_ptr(), n, stream))
-    check(lib.hk_pages_fork(pages, to, state["source"].data_ptr(), starts, n, status, stream))
+    check(lib.hk_pages_fork(pages, to, state["source"].data_ptr(), starts, n, state["forked"].data_ptr(), stream))
     check(lib.hk_pages_reserve(pages, to, starts, state["ends"].data_ptr(), n, status, space.data_ptr(), need, stream))
     return {name: state[name] for name in ("tables", "refs", "status", "keys", "values")}
 
