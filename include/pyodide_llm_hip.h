@@ -425,17 +425,18 @@ typedef struct hk_pages {
 /* Sequences that go on from others: for each i < n (1..HK_PAGES_SEQS_MOST), sequence to[i] holds the pages of sequence from[i]
  * that its first lengths[i] positions lie in, and no others; what it held before is given back. Nothing is copied: the pages
  * are shared until hk_pages_reserve parts them. All entries take from the tables as they were before the call, so that beams
- * may change places in one call. A sequence may be in `from` often, in `to` once. *status (device int32, or null): 0, or -1
- * where the lists are not such as this (a sequence past the tables, or in `to` twice; a length outside 0..table_size *
- * page_size): then nothing is changed. */
+ * may change places in one call. A sequence may be in `from` often, in `to` once; an entry whose `to` is negative is passed over.
+ * *status (device int32, or null): 0, or -1 where the lists are not such as this (a sequence past the tables, or in `to` twice; a
+ * negative one in `from`; a length outside 0..table_size * page_size): then nothing is changed. */
 int32_t hk_pages_fork(const hk_pages *pages, const void *to, const void *from, const void *lengths, int32_t n, void *status,
                       void *stream);
 
 /* Room to write: for each i < n (1..HK_PAGES_SEQS_MOST), every position starts[i]..ends[i] - 1 of sequence seqs[i] gets a page
  * that it alone names. Where there is none yet, or one that is shared as the call begins, the lowest free page is taken, in
  * the order of the list and of its positions; of a shared page with positions before starts[i], those rows are copied, in all
- * layers (what the sequence held from starts[i] on does not come along: the sequence goes on from there). A sequence may be
- * listed once. *status (device int32, or null): 0; or how many free pages are lacking, or -1 where
+ * layers (what the sequence held from starts[i] on does not come along: the sequence goes on from there). Sequences that alone
+ * share a page and are listed together all leave it: as many pages and copies as there are of them, and that page is free then. A
+ * sequence may be listed once. *status (device int32, or null): 0; or how many free pages are lacking, or -1 where
  * the lists are not such as this (a sequence past the tables or listed twice, a position outside 0..table_size * page_size):
  * then nothing is changed. workspace: at least hk_pages_workspace bytes (16-byte aligned), not shared by calls that may
  * overlap. */
@@ -470,10 +471,11 @@ int32_t hk_pages_append(const hk_pages *pages, int32_t layer, const void *k, con
  * rows may be of one sequence (the tokens of a turn, at lengths one apart). lengths[i] is at most `longest`, which the
  * launches are made for. A row of length 0 (or less), or of a negative sequence, is zeros; one whose length is past `longest`
  * or the tables, or whose sequence is, or a position of which has no page, is NaN. What lies behind a row's length has no
- * part in it, whatever it is. A q that is not finite makes its own row NaN; a key that is not finite changes the rows that see it
- * alone (NaN, unless it takes their score to minus infinity, which has no weight), a value that is not finite makes their channel
- * not finite. Sums are float32's, of values weighted by exp(score - the largest score so far); a half cache's products keep
- * float32's bits. The same call gives the same bits; how a row's sums are split, and so their last ones, goes by all rows'
+ * part in it, whatever it is. A q that is not finite makes its own head of its own row NaN; a key that is not finite changes the
+ * heads that see it in the rows that see it alone (NaN, unless it takes their score to minus infinity, which has no weight; over a
+ * half cache such a score may be NaN too), a value that is not finite makes their channel not finite. Sums are float32's, of values
+ * weighted by exp(score - the largest score so far), divided at the end alone: such a sum of a row's |v| is to stay within float32.
+ * A half cache's products keep float32's bits. The same call gives the same bits; how a row's sums are split, and so their last ones, goes by all rows'
  * lengths.
  * workspace: at least hk_pages_attention_workspace bytes (16-byte aligned; nothing in it is kept from one call to the next),
  * not shared by calls that may overlap. */
@@ -490,7 +492,7 @@ int64_t hk_pages_attention_workspace(const hk_pages *pages, int32_t n_heads, int
  * y[t][r] = sum_g ws xs[t][g] (sum over the 32 columns i of group g of w[r][i] (xq[t][i] - bias)) for m tokens and rows
  * r < rows: w in -8..7, its scale ws one a row and `group` (32, 64 or 128) columns; xq [m][k] and xs [m][k / 32] as
  * hk_quantize_x leaves them with the same bias (64 or 0). The sums within a group are exact in int32; those over the groups
- * float32's, in an order of the kernel's own. y is [m][rows] float32; m in 1..65535, rows in 1..2^26, k a multiple of 32 up to
+ * float32's, in an order of the kernel's own, of sixteen times the values (16 y is to stay within float32). y is [m][rows] float32; m in 1..65535, rows in 1..2^26, k a multiple of 32 up to
  * 2^24. The scales of w are finite (a row with one that is not is not finite either); an xs that is not concerns its token alone.
  *
  * A row of w, and its scales, are filled up with zeros to a multiple of 128 columns. 128 columns are 64 bytes; the 16-byte chunk

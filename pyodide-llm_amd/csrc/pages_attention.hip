@@ -9,7 +9,8 @@
 //   O^T = V^T P^T: the probabilities go from the first product's output registers to the second's input. A lane reads a
 //     few neighbouring channels of its positions' value rows; channel i of each is one product's.
 // A float16 cache's products are float16's, with float32's bits: queries and probabilities go in two halves, x = hi + lo / 2048,
-// each rounded to nearest (2^-24 of x is left), in columns 0-7 and 8-15 of one product. A float32 cache's are float32's.
+// each rounded to nearest (2^-23 of x is left at most), in columns 0-7 and 8-15 of one product. A float32 cache's are float32's.
+// Outputs are divided by the probabilities' sum at the end alone: what they add up to before has float32's range too.
 #include <algorithm>
 
 #include "common.hpp"
@@ -44,7 +45,7 @@ template <>
 struct Kind<false> {
   typedef float type;
   static constexpr int heads = 16;
-  static constexpr float ahead = 0.0f;  // (values may be large: no probability is above 1, but for the reference's rounding)
+  static constexpr float ahead = 0.0f;  // (values may be large: no probability is above 1, but for a score's rounding)
 };
 
 // lane ^ 8 within 16: the other half of a column's products
