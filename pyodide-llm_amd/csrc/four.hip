@@ -56,7 +56,7 @@ __device__ __forceinline__ T quad_sums(const T (&s)[4], int j) {
 // LANES lanes a row (16, 64 or all waves'), which take its chunks LANES apart, STEPS of them at most; they take four rows at a
 // time and go on the launch's rows further. A lane's activations stay in its registers from row to row. No load is conditional,
 // which would wait for each: what lies past the columns is taken as zero. Bound by the weights' bytes where there are many
-// (128,256 rows of 4096 columns, 271 MB in 48.1 us, 5.6 TB/s), by latency where not (4096 rows, 10.5 MB, 4.0 us; 5.5 with
+// (128,256 rows of 4096 columns, 271 MB in 48.4 us, 5.6 TB/s), by latency where not (4096 rows, 10.5 MB, 4.0 us; 5.5 with
 // conditional loads).
 template <int LANES, int STEPS, bool HALF>
 __global__ __launch_bounds__(64 * WAVES) void gemv_kernel(const FourArgs a) {
@@ -254,8 +254,8 @@ __device__ __forceinline__ void finish(const FourArgs &a, const float4 *sums, in
 
 // Up to 16 TILES tokens of up to 1024 DEEP columns: they stay in LDS, and the workgroup goes from 16 rows to 16 rows, its waves
 // sharing their columns. A wave's loads for its next rows go out as its present weights are used, into their registers. One
-// workgroup a CU: two have twice the loads on their way and came out slower (16 tokens by 14336 rows of 4096 columns 18.8 us
-// against 15.0). 16 tokens by 2304 rows of 768 columns take 3.6 us; 32 by 14336 of 4096 17.
+// workgroup a CU, whose waves all wait for the tokens before the first product. 16 tokens by 2304 rows of 768 columns take 3.7 us;
+// 32 by 14336 of 4096 18, by 4096 12.
 template <int TILES, int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a) {
   __shared__ Tokens<TILES, GEMM_WAVES * DEEP> tokens;
@@ -301,8 +301,8 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void rows_kernel(const FourArgs a)
 // Up to 16 tokens of 1025 to 4096 columns: as rows_kernel, with the tokens in registers (a wave's columns stay the same) and the
 // weights on their way there through LDS. A wave's load takes 64 DEEP bytes of a row, whole cache lines, from 16 / DEEP rows; the
 // products' order, 64 bytes of each of 16, is LDS's: chunk k of row r lies at place k ^ r of the row's, so that neither side meets
-// a bank twice. 128,256 rows of 4096 columns, 271 MB, take 57 us (64 with loads of 64 bytes of 16 rows), 14336 11.8, of which
-// about 6 pass until the first rows are done, 4096 7.2. Rows two turns ahead: the same.
+// a bank twice. 128,256 rows of 4096 columns, 271 MB, take 59 us (64 with loads of 64 bytes of 16 rows), 14336 12.0, of which
+// about 6 pass until the first rows are done, 4096 7.5. Rows two turns ahead: the same.
 template <int DEEP, int GROUP, bool HALF>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void lines_kernel(const FourArgs a) {
   constexpr int EACH = Weights<GROUP, HALF>::EACH;
@@ -450,7 +450,8 @@ void launch_gemm(const FourArgs &a, hipStream_t s) {
   // rows a workgroup: the fewest whose workgroups are not more than the CUs, since each brings the activations to LDS for itself
   // (64 tokens by 14336 rows: 62 us at 16, 45 at 32, 29 at 64; by 4096 rows 19, 23, 30; 2048 tokens by 4096 rows 408 at 16, 217
   // at 64); with one tile of tokens two of rows take more registers than two workgroups a CU leave (4096 rows of 14336 columns:
-  // 21 us, 35)
+  // 21 us, 35). Past 64 rows a workgroup there is no larger shape: 128 tokens by 8192 rows, 256 workgroups, take 31 us, by 9000
+  // rows, 282 of them, 58.
   if constexpr (TILES == 1) {
     launch_stages<1, 1, HALF>(a, s);
   } else {
@@ -464,7 +465,6 @@ void launch_gemm(const FourArgs &a, hipStream_t s) {
 template <bool HALF>
 void launch(const FourArgs &a, hipStream_t s) {
   const int chunks = (a.k + 127) / 128 * 4;
-  // (two tokens by the first kernel: 4096 rows of 4096 columns 7.3 us against 6.9, of 14336 17.8, 13.8; 32000 of 768 the same)
   if (a.m == 1 && chunks <= 1024) {
     if (chunks <= 16) launch_gemv<16, 1, HALF>(a, s);
     else if (chunks <= 32) launch_gemv<16, 2, HALF>(a, s);

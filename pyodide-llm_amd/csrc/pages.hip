@@ -75,7 +75,8 @@ __device__ __forceinline__ void counts(const PagesView &c, int32_t p, int32_t pa
 // ---- fork ----
 
 // A workgroup takes `cols` slots of every listed sequence, and goes on a launch further: what their rows shall hold is read before
-// any of it is written, so that a sequence may be read and written by one call. Latency: the lists, the tables, the counts (16 sequences 4.4 us).
+// any of it is written, so that a sequence may be read and written by one call. Latency: the lists, the tables, the counts (16
+// sequences 4.8 us).
 __global__ __launch_bounds__(256) void fork_kernel(const PagesView c, const int32_t *to, const int32_t *from,
                                                    const int32_t *lengths, int n, int cols, int32_t *status) {
   extern __shared__ int32_t lds[];
@@ -138,7 +139,8 @@ constexpr int HERE = 2048;  // pages whose lists stay in LDS
 
 // One workgroup. The slots that the listed positions lie in, in order, make pairs (entry, slot); those without a page, or with
 // one that other entries name, ask for one, and the k-th asks for the k-th free page. Nothing is written before all are found.
-// Latency: the lists, the tables, the counts (6.8 us); the first counts are asked for before it is known how many are needed.
+// Latency: the lists, the tables, the counts (7.1 us; 64 sequences with one position more and nothing to copy 5.4); the first
+// counts are asked for before it is known how many are needed.
 __global__ __launch_bounds__(THREADS) void reserve_kernel(const PagesView c, const int32_t *seqs, const int32_t *starts,
                                                           const int32_t *ends, int n, int32_t *status, int32_t *workspace) {
   __shared__ uint32_t seen[PAGES_SEQS_MOST / 32];
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(THREADS) void moves_kernel(const PagesView c, int32
 
 constexpr int PIECE = 256 * 4 * 16;  // bytes a workgroup copies at a time
 
-// Pages to their places: a piece of one layer's keys or values a workgroup and turn. Bound by HBM, both ways: 470 MB in 94 us (5.0
+// Pages to their places: a piece of one layer's keys or values a workgroup and turn. Bound by HBM, both ways: 470 MB in 97 us (4.9
 // TB/s; read and written past the caches, which hold nothing of them: 104 through them). The last row of workgroups takes the
 // tables and the counts.
 __global__ __launch_bounds__(256) void move_kernel(const PagesView c, int32_t *workspace) {
@@ -350,8 +352,8 @@ __global__ __launch_bounds__(256) void move_kernel(const PagesView c, int32_t *w
 
 // ---- append ----
 
-// A thread takes four channels of a row's keys and values. A step's rows are latency (64 rows 2.9 us), a prompt's bound by HBM
-// (2048 rows of 8 heads of 128 in float32, 34 MB, 7.6).
+// A thread takes four channels of a row's keys and values. A step's rows are latency (64 rows 3.0 us), a prompt's bound by HBM
+// (2048 rows of 8 heads of 128 in float32, 34 MB, 7.3).
 template <bool HALF>
 __global__ __launch_bounds__(256) void append_kernel(const PagesRows a) {
   const PagesView &c = a.c;

@@ -580,7 +580,7 @@ void cut(PagesAttn &a) {
     const int places = 256 * occupancy(a.c.hs, a.c.half) / tiles;
     a.pieces = std::max(1, places - std::min(a.rows, places) / 2);
     a.most = std::min<int64_t>(a.pieces + a.rows, (int64_t)a.rows * ((a.longest + LEAST * UNIT - 1) / (LEAST * UNIT)));
-  } else {
+  } else {  // (by the longest: one row of 131,072 positions among 511 of 200 takes 1042 us, among 255, planned, 174)
     a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(16384 / ((int64_t)a.rows * tiles), (a.longest + 2047) / 2048));
     a.chunk = ((a.longest + a.parts - 1) / a.parts + UNIT - 1) / UNIT * UNIT;
     a.most = (int64_t)a.rows * a.parts;
